@@ -24,9 +24,9 @@ from __future__ import annotations
 import torch
 from torch.utils.checkpoint import checkpoint
 
-from . import node_ops, ops
+from . import mlp_ops, node_ops, ops
 
-__all__ = ["res_plus_layer", "ResPlusLayer", "ComposedEdgeEmbedding"]
+__all__ = ["res_plus_layer", "ResPlusLayer", "ComposedEdgeEmbedding", "ResMLP", "ResMLPE4M3"]
 
 
 def _active_partition():
@@ -118,6 +118,53 @@ class ResPlusLayer(torch.nn.Module):
     def forward(self, h, edge_index, edge_attr=None, stats=None):
         return res_plus_layer(self.norm, self.conv, h, edge_index, edge_attr, p=self.dropout, training=self.training,
                               stats=stats, use_checkpoint=self.use_checkpoint)
+
+
+class ResMLP(torch.nn.Module):
+    """``h + W2 act(W1 rmsnorm(h) + b1) + b2`` over node rows in three launches: the norm (which also adds ``residual``, the
+    rows an aggregation leaves: ``h = x + residual``), the product with bias and activation, the product with bias and
+    ``h``.  fp32, bf16 or fp16; ``act`` one of ``mlp_ops.ACTIVATIONS``.  ``e4m3()``: the same block in 8 bits, for serving."""
+
+    def __init__(self, channels: int, hidden: int, act: str = "gelu", bias: bool = True, eps: float = 1e-6):
+        super().__init__()
+        if act not in mlp_ops.ACTIVATIONS:
+            raise ValueError(f"act must be one of {', '.join(mlp_ops.ACTIVATIONS)}, got {act!r}")
+        self.norm = mlp_ops.RMSNorm(channels, eps)
+        self.lin1 = torch.nn.Linear(channels, hidden, bias=bias)
+        self.lin2 = torch.nn.Linear(hidden, channels, bias=bias)
+        self.act = act
+
+    def forward(self, x, residual=None):
+        y, h = (self.norm(x), x) if residual is None else self.norm(x, residual)
+        u = mlp_ops.linear_act(y, self.lin1.weight, self.lin1.bias, act=self.act)
+        return mlp_ops.linear_act(u, self.lin2.weight, self.lin2.bias, residual=h)
+
+    @torch.no_grad()
+    def e4m3(self) -> "ResMLPE4M3":
+        return ResMLPE4M3(self)
+
+
+class ResMLPE4M3(torch.nn.Module):
+    """A :class:`ResMLP` whose two products run in 8 bits: the weights' rows are laid out once, the norm's output and the
+    activations are rounded row by row on the way.  The stream ``h`` keeps its type.  No gradient."""
+
+    def __init__(self, mlp: ResMLP):
+        super().__init__()
+        self.act, self.eps = mlp.act, mlp.norm.eps
+        self.register_buffer("norm_weight", mlp.norm.weight.detach().clone())
+        for i, lin in ((1, mlp.lin1), (2, mlp.lin2)):
+            w = mlp_ops.quantize_rows(lin.weight.detach())
+            self.register_buffer(f"weight{i}", w.data)
+            self.register_buffer(f"scale{i}", w.scale)
+            self.register_buffer(f"bias{i}", None if lin.bias is None else lin.bias.detach().clone())
+
+    @torch.no_grad()
+    def forward(self, x, residual=None):
+        out = mlp_ops.rms_norm_rows_e4m3(x, self.norm_weight, self.eps, residual)
+        y, h = (out, x) if residual is None else out
+        w1, w2 = mlp_ops.RowsE4M3(self.weight1, self.scale1), mlp_ops.RowsE4M3(self.weight2, self.scale2)
+        u = mlp_ops.linear_act_e4m3(y, w1, self.bias1, act=self.act, out_dtype=x.dtype)
+        return mlp_ops.linear_act_e4m3(mlp_ops.quantize_rows(u), w2, self.bias2, residual=h, out_dtype=x.dtype)
 
 
 class _ComposeEncoder(torch.autograd.Function):

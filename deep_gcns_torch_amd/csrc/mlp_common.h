@@ -1,0 +1,130 @@
+// Element types, eight-element chunks and activations shared by the node-wise MLP kernels (rms_norm.hip,
+// linear_act.hip).  Everything is computed in fp32; a 16-bit value is rounded once, to nearest even, where it is stored.
+#pragma once
+
+#include "dgcn_common.h"
+
+namespace dgcn {
+
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Vector accesses at the element's own alignment: the device runs in unaligned-access mode, a global dwordx4 may start
+// at any byte.  Rows of odd length or stride take the same wide loads as aligned ones.
+typedef u4v u4v_any2 __attribute__((aligned(2)));
+typedef u4v u4v_any4 __attribute__((aligned(4)));
+typedef u2v u2v_any1 __attribute__((aligned(1)));
+
+template <class T> struct Vec8;
+template <> struct Vec8<__bf16> { typedef bf16x8 type; };
+template <> struct Vec8<_Float16> { typedef f16x8 type; };
+
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 a = __builtin_bit_cast(f32x4, *reinterpret_cast<const u4v_any4*>(p));
+    const f32x4 b = __builtin_bit_cast(f32x4, *reinterpret_cast<const u4v_any4*>(p + 4));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+  } else {
+    const auto a = __builtin_bit_cast(typename Vec8<T>::type, *reinterpret_cast<const u4v_any2*>(p));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(a[e]);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<u4v_any4*>(p) = __builtin_bit_cast(u4v, f32x4{v[0], v[1], v[2], v[3]});
+    *reinterpret_cast<u4v_any4*>(p + 4) = __builtin_bit_cast(u4v, f32x4{v[4], v[5], v[6], v[7]});
+  } else {
+    typename Vec8<T>::type a;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = static_cast<T>(v[e]);
+    *reinterpret_cast<u4v_any2*>(p) = __builtin_bit_cast(u4v, a);
+  }
+}
+
+// elements [start, start + 8) of a row of n (the part behind the end reads as `fill`, and is not written)
+template <class T>
+__device__ __forceinline__ void load_chunk(const T* row, int start, int n, float (&v)[8], float fill = 0.f) {
+  if (start + 8 <= n) {
+    load8(row + start, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = start + e < n ? static_cast<float>(row[start + e]) : fill;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store_chunk(T* row, int start, int n, const float (&v)[8]) {
+  if (start + 8 <= n) {
+    store8(row + start, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (start + e < n) row[start + e] = static_cast<T>(v[e]);
+    }
+  }
+}
+
+// parameters (weight, bias) come in the rows' type or in fp32
+template <class T>
+__device__ __forceinline__ void load_param_chunk(const void* p, bool f32, int start, int n, float (&v)[8], float none) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = none;
+  } else if (f32) {
+    load_chunk(static_cast<const float*>(p), start, n, v, none);
+  } else {
+    load_chunk(static_cast<const T*>(p), start, n, v, none);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ float load_param(const void* p, bool f32, int64_t i) {
+  return f32 ? static_cast<const float*>(p)[i] : static_cast<float>(static_cast<const T*>(p)[i]);
+}
+
+// four fp32 values -> four e4m3 bytes, to nearest even (|v| <= 448 up to rounding; anything not finite -> NaN, 0x7f)
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true));
+}
+
+// ---- activations: act(z) and act'(z), in fp32 ----
+// EXACT: libm's exp (the fp32 type); otherwise the hardware's 2^x, whose error of |z| 2^-24 is far below a 16-bit step
+template <bool EXACT>
+__device__ __forceinline__ float act_exp(float x) { return EXACT ? expf(x) : fast_exp(x); }
+
+template <bool EXACT>
+__device__ __forceinline__ float act_fwd(float z, int act, float slope) {
+  switch (act) {
+    case DGCN_ACT_RELU: return z < 0.f ? 0.f : z;                        // (NaN stays NaN)
+    case DGCN_ACT_LEAKY_RELU: return z > 0.f ? z : slope * z;
+    case DGCN_ACT_GELU: return 0.5f * z * erfcf(z * -0.70710678118654752f);   // (1 + erf would cancel for z < 0)
+    case DGCN_ACT_SILU: return z / (1.f + act_exp<EXACT>(-z));
+    default: return z;
+  }
+}
+
+template <bool EXACT>
+__device__ __forceinline__ float act_slope(float z, int act, float slope) {
+  switch (act) {
+    case DGCN_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+    case DGCN_ACT_LEAKY_RELU: return z > 0.f ? 1.f : slope;
+    case DGCN_ACT_GELU:
+      return 0.5f * erfcf(z * -0.70710678118654752f) + z * 0.39894228040143268f * act_exp<EXACT>(-0.5f * z * z);
+    case DGCN_ACT_SILU: {
+      const float s = 1.f / (1.f + act_exp<EXACT>(-z));
+      return s * (1.f + z * (1.f - s));
+    }
+    default: return 1.f;
+  }
+}
+
+}  // namespace dgcn

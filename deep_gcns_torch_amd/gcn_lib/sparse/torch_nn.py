@@ -8,6 +8,7 @@ norm, act, [dropout] per hidden layer; nothing after the last Linear when ``last
 import torch
 from torch import nn
 
+from ...mlp_ops import RMSNorm
 from ...nn_util import TallLinear
 from ...node_ops import BatchNorm1d, CouplingResidual, LayerNorm
 from ...utils.data_util import get_atom_feature_dims, get_bond_feature_dims
@@ -28,7 +29,7 @@ def act_layer(act_type, inplace=False, neg_slope=0.2, n_prelu=1):
 
 
 def norm_layer(norm_type, nc):
-    """1-D normalisation factory: batch | layer | instance."""
+    """1-D normalisation factory: batch | layer | instance, and rms (extension)."""
     kind = norm_type.lower()
     if kind == "batch":
         return BatchNorm1d(nc, affine=True)          # an nn.BatchNorm1d; (rows, C) inputs run on the HIP kernels
@@ -36,6 +37,8 @@ def norm_layer(norm_type, nc):
         return LayerNorm(nc, elementwise_affine=True)    # an nn.LayerNorm; device rows run on the HIP kernels
     if kind == "instance":
         return nn.InstanceNorm1d(nc, affine=False)
+    if kind == "rms":
+        return RMSNorm(nc)                           # fp32 / bf16 / fp16 rows; device rows only
     raise NotImplementedError("normalization layer [%s] is not found" % kind)
 
 

@@ -1,0 +1,380 @@
+"""The node-wise MLP in 32, 16 and 8 bits: root-mean-square norm with the residual's addition, and the product with bias,
+activation and residual in its epilogue (csrc/rms_norm.hip, csrc/linear_act.hip).
+
+``node_ops`` holds the fp32 row operators that the reference's own models use; these are the ones around them for models
+whose rows are wider than 256 channels, or kept in bf16, fp16 or 8 bits:
+
+    h = x + r;  y = h * rsqrt(mean(h^2) + eps) * w     rms_norm_rows(x, w, eps, residual=r)        forward and backward
+    the same y as e4m3 rows, one fp32 scale each       rms_norm_rows_e4m3(x, w, eps, residual=r)   forward
+    x as e4m3 rows                                     quantize_rows(x)                            forward
+    act(x W^T + b) + r                                 linear_act(x, W, b, act, residual=r)        forward and backward
+    the same of e4m3 rows and an e4m3 weight           linear_act_e4m3(x, W, b, act, residual=r)   forward
+
+Rows are the last dimension; leading dimensions are free and may be empty.  Sums and statistics are fp32, every result is
+rounded once to its type.  Work runs on the current stream of the inputs' device; results do not depend on timing (no
+atomics).  What an operator does not take raises, nothing falls back.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+__all__ = ["ACTIVATIONS", "RMSNorm", "RowsE4M3", "linear_act", "linear_act_e4m3", "quantize_rows", "rms_norm_rows",
+           "rms_norm_rows_e4m3"]
+
+#: activation name -> code (include/dgcn.h)
+ACTIVATIONS = {"none": 0, "relu": 1, "leakyrelu": 2, "gelu": 3, "silu": 4}
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_E4M3 = 3
+_MAX_NORM_C = 32768
+_MAX_K = 1 << 20
+
+
+class RowsE4M3(NamedTuple):
+    """Rows in 8 bits: the row's values are ``data * scale``.  ``data`` (..., C) ``torch.float8_e4m3fn``, ``scale`` (...)
+    fp32."""
+    data: torch.Tensor
+    scale: torch.Tensor
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        return (self.data.to(torch.float32) * self.scale.unsqueeze(-1)).to(dtype)
+
+
+def _row_type(x: torch.Tensor, what: str) -> int:
+    t = _TYPES.get(x.dtype)
+    if t is None:
+        raise TypeError(f"{what}: rows must be float32, bfloat16 or float16, got {x.dtype}")
+    if x.dim() < 1 or x.size(-1) < 1:
+        raise ValueError(f"{what}: rows need a last dimension of at least 1, got {tuple(x.shape)}")
+    return t
+
+
+def _rows2d(x: torch.Tensor):
+    """``x`` as (rows, C) with unit stride in a row, and its row stride.  Rows that repeat (stride 0) are taken as they are."""
+    C = x.size(-1)
+    x2 = x if x.dim() == 2 else x.reshape(-1, C)
+    if C > 1 and x2.stride(1) != 1 or x2.stride(0) < 0:
+        x2 = x2.contiguous()
+    return x2, x2.stride(0) if x2.size(0) > 1 else C
+
+
+def _param(p, n: int, like: torch.Tensor, what: str):
+    """A (n,) parameter in the rows' type or fp32 -> (contiguous tensor, is it fp32)."""
+    if p is None:
+        return None, 0
+    if p.dim() != 1 or p.size(0) != n:
+        raise ValueError(f"{what} must have shape ({n},), got {tuple(p.shape)}")
+    if p.dtype != like.dtype and p.dtype != torch.float32:
+        raise TypeError(f"{what} must be {like.dtype} or float32, got {p.dtype}")
+    return p.detach().contiguous(), 1 if p.dtype == torch.float32 else 0
+
+
+def _same_rows(r, x: torch.Tensor, n: int, dtype, what: str) -> None:
+    want = (*x.shape[:-1], n)
+    if r.shape != want:
+        raise ValueError(f"{what} must have shape {tuple(want)}, got {tuple(r.shape)}")
+    if r.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, got {r.dtype}")
+
+
+def _param_sum(parts: torch.Tensor, dtype) -> torch.Tensor:
+    out = torch.empty(parts.size(1), device=parts.device, dtype=dtype)
+    _lib.check(_lib.load().dgcn_param_sum(parts.data_ptr(), parts.size(0), parts.size(1), _TYPES[dtype], out.data_ptr(),
+                                          _lib.current_stream_handle(parts.device)), "dgcn_param_sum")
+    return out
+
+
+# ---- root-mean-square norm ------------------------------------------------------------------------------------------
+def _rms_launch(x, weight, eps, residual, e4m3: bool, want_rstd: bool):
+    """-> (y or (q, scale), h or None, rstd or None), contiguous, h and y of x's shape."""
+    lib = _lib.load()
+    dev = _lib.require_device(x, weight, residual)
+    x2, ldx = _rows2d(x)
+    r2, ldr = _rows2d(residual) if residual is not None else (None, 0)
+    rows, C = x2.shape
+    w, w_f32 = _param(weight, C, x, "weight")
+    h = torch.empty(x.shape, device=dev, dtype=x.dtype) if residual is not None else None
+    rstd = torch.empty(rows, device=dev, dtype=torch.float32) if want_rstd else None
+    y = q = scale = None
+    if e4m3:
+        q = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
+        scale = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32)
+    else:
+        y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    if rows == 0:
+        return (RowsE4M3(q, scale) if e4m3 else y), h, rstd
+    with _lib.device_ctx(dev):
+        _lib.check(lib.dgcn_rms_norm_fwd(x2.data_ptr(), ldx, _lib.ptr(r2), ldr, _lib.ptr(w), w_f32, eps, _TYPES[x.dtype],
+                                         _lib.ptr(y), _lib.ptr(h), _lib.ptr(q), _lib.ptr(scale), _lib.ptr(rstd), rows, C,
+                                         _lib.current_stream_handle(dev)), "dgcn_rms_norm_fwd")
+    return (RowsE4M3(q, scale) if e4m3 else y), h, rstd
+
+
+class _RMSNormRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps: float):
+        ctx.set_materialize_grads(False)
+        y, h, rstd = _rms_launch(x, weight, eps, residual, False, True)
+        ctx.save_for_backward(x if h is None else h, weight, rstd)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, gh=None):
+        h, weight, rstd = ctx.saved_tensors
+        need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[2]
+        need_w = weight is not None and ctx.needs_input_grad[1]
+        if g is None or h.numel() == 0:          # only the sum was used: its gradient is both inputs'
+            gh = torch.zeros_like(h) if gh is None else gh
+            gw = torch.zeros_like(weight) if need_w else None
+            return (gh if ctx.needs_input_grad[0] else None), gw, (gh if ctx.needs_input_grad[2] else None), None
+        lib = _lib.load()
+        dev = h.device
+        h2, ldh = _rows2d(h)
+        g2, ldg = _rows2d(g)
+        gh2, ldgh = _rows2d(gh) if gh is not None else (None, 0)
+        rows, C = h2.shape
+        w, w_f32 = _param(weight, C, h, "weight")
+        dx = torch.empty(h.shape, device=dev, dtype=h.dtype) if need_x else None
+        gw = None
+        with _lib.device_ctx(dev):
+            parts = None
+            if need_w:
+                parts = torch.empty(lib.dgcn_rms_norm_num_partials(rows, C), C, device=dev, dtype=torch.float32)
+            if need_x or need_w:
+                _lib.check(lib.dgcn_rms_norm_bwd(g2.data_ptr(), ldg, _lib.ptr(gh2), ldgh, h2.data_ptr(), ldh, _lib.ptr(w),
+                                                 w_f32, rstd.data_ptr(), _TYPES[h.dtype], _lib.ptr(dx), _lib.ptr(parts),
+                                                 rows, C, _lib.current_stream_handle(dev)), "dgcn_rms_norm_bwd")
+            if need_w:
+                gw = _param_sum(parts, weight.dtype)
+        return (dx if ctx.needs_input_grad[0] else None), gw, (dx if ctx.needs_input_grad[2] else None), None
+
+
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _rms_checks(what, x, weight, residual):
+    _row_type(x, what)
+    C = x.size(-1)
+    if C > _MAX_NORM_C:
+        raise ValueError(f"{what}: rows of at most {_MAX_NORM_C} channels, got {C}")
+    _param(weight, C, x, "weight")
+    if residual is not None:
+        _same_rows(residual, x, C, x.dtype, "residual")
+    _lib.require_device(x, weight, residual)
+
+
+def rms_norm_rows(x, weight=None, eps: float = 1e-6, residual=None):
+    """``h = x [+ residual]``, ``y = h * rsqrt(mean(h^2) + eps) [* weight]`` over the last dimension.
+
+    Returns ``y``, or ``(y, h)`` with a residual: ``h`` is the stream that the next layer adds to.  ``x`` (..., C) fp32,
+    bf16 or fp16, C <= 32768; ``residual`` of the same shape and type; ``weight`` (C,) in the rows' type or fp32.  ``y`` is
+    computed from the fp32 sum; its gradient (of x, weight and residual) from the stored ``h``."""
+    _rms_checks("rms_norm_rows", x, weight, residual)
+    if _needs_grad(x, weight, residual):
+        return _RMSNormRows.apply(x, weight, residual, float(eps))
+    y, h, _ = _rms_launch(x, weight, float(eps), residual, False, False)
+    return y if residual is None else (y, h)
+
+
+def _no_grad_only(what, *tensors):
+    if _needs_grad(*tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or on tensors that require none")
+
+
+def rms_norm_rows_e4m3(x, weight=None, eps: float = 1e-6, residual=None):
+    """``rms_norm_rows`` whose ``y`` leaves as :class:`RowsE4M3`: ``scale = max|y| / 448`` per row (1 for a row of zeros).
+    Returns the rows, or ``(rows, h)`` with a residual.  A NaN or an infinity becomes NaN in its own place.  No gradient."""
+    _rms_checks("rms_norm_rows_e4m3", x, weight, residual)
+    _no_grad_only("rms_norm_rows_e4m3", x, weight, residual)
+    y, h, _ = _rms_launch(x, weight, float(eps), residual, True, False)
+    return y if residual is None else (y, h)
+
+
+def quantize_rows(x) -> RowsE4M3:
+    """``x`` (..., C) as e4m3 rows with one scale each: activations between two products in 8 bits, or the rows of a weight
+    (C_out, C_in) that is laid out once.  C <= 32768.  No gradient."""
+    t = _row_type(x, "quantize_rows")
+    if x.size(-1) > _MAX_NORM_C:
+        raise ValueError(f"quantize_rows: rows of at most {_MAX_NORM_C} channels, got {x.size(-1)}")
+    dev = _lib.require_device(x)
+    _no_grad_only("quantize_rows", x)
+    x2, ldx = _rows2d(x)
+    q = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
+    scale = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32)
+    if x.numel() == 0:
+        return RowsE4M3(q, scale)
+    with _lib.device_ctx(dev):
+        _lib.check(_lib.load().dgcn_quantize_rows_e4m3(x2.data_ptr(), ldx, t, q.data_ptr(), scale.data_ptr(), x2.size(0),
+                                                       x2.size(1), _lib.current_stream_handle(dev)),
+                   "dgcn_quantize_rows_e4m3")
+    return RowsE4M3(q, scale)
+
+
+class RMSNorm(nn.Module):
+    """``rms_norm_rows`` with its weight: ``norm_layer('rms', C)``.  ``forward(x, residual=None)`` returns ``y`` or
+    ``(y, h)``; ``forward_e4m3`` the same in 8 bits."""
+
+    def __init__(self, channels: int, eps: float = 1e-6):
+        super().__init__()
+        self.channels, self.eps = int(channels), float(eps)
+        self.weight = nn.Parameter(torch.ones(self.channels))
+
+    def forward(self, x, residual=None):
+        return rms_norm_rows(x, self.weight, self.eps, residual)
+
+    def forward_e4m3(self, x, residual=None):
+        return rms_norm_rows_e4m3(x, self.weight, self.eps, residual)
+
+    def extra_repr(self):
+        return f"{self.channels}, eps={self.eps}"
+
+
+# ---- product with epilogue ------------------------------------------------------------------------------------------
+def _linear_launch(x2, ldx, w2, ldw, sx, sw, bias, bias_f32, r2, ldr, act, slope, in_type, out_type, z, y, K, N):
+    dev = y.device
+    if y.numel() == 0:
+        return
+    with _lib.device_ctx(dev):
+        _lib.check(_lib.load().dgcn_linear_act(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _lib.ptr(sx), _lib.ptr(sw),
+                                               _lib.ptr(bias), bias_f32, _lib.ptr(r2), ldr, act, slope, in_type, out_type,
+                                               _lib.ptr(z), y.data_ptr(), x2.size(0), K, N,
+                                               _lib.current_stream_handle(dev)), "dgcn_linear_act")
+
+
+def _linear_forward(x, weight, bias, residual, act, slope, keep_z: bool):
+    x2, ldx = _rows2d(x)
+    w2, ldw = _rows2d(weight)
+    N, K = w2.shape
+    b, b_f32 = _param(bias, N, x, "bias")
+    r2, ldr = _rows2d(residual) if residual is not None else (None, 0)
+    t = _TYPES[x.dtype]
+    y = torch.empty((*x.shape[:-1], N), device=x.device, dtype=x.dtype)
+    z = torch.empty_like(y) if keep_z and act != 0 else None
+    _linear_launch(x2, ldx, w2, ldw, None, None, b, b_f32, r2, ldr, act, slope, t, t, z, y, K, N)
+    return y, z
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act: int, slope: float):
+        y, z = _linear_forward(x, weight, bias, residual, act, slope, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, z)
+        ctx.cfg = (act, slope, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight, z = ctx.saved_tensors
+        act, slope, bias_type = ctx.cfg
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        gx = gw = gb = None
+        if g.numel() == 0:                       # no rows: sums over nothing
+            gx = torch.zeros_like(x) if need_x else None
+            gw = torch.zeros_like(weight) if need_w else None
+            gb = torch.zeros(weight.size(0), device=g.device, dtype=bias_type) if need_b else None
+        elif need_x or need_w or need_b:
+            lib = _lib.load()
+            dev, t = x.device, _TYPES[x.dtype]
+            x2, ldx = _rows2d(x)
+            w2, ldw = _rows2d(weight)
+            g2, ldg = _rows2d(g)
+            rows, K = x2.shape
+            N = w2.size(0)
+            with _lib.device_ctx(dev):
+                stream = _lib.current_stream_handle(dev)
+                d2, ldd = g2, ldg
+                if act != 0 or need_b:
+                    parts = None
+                    if act != 0:
+                        d2, ldd = torch.empty(rows, N, device=dev, dtype=x.dtype), N
+                    if need_b:
+                        parts = torch.empty(lib.dgcn_linear_gate_num_partials(rows, N), N, device=dev, dtype=torch.float32)
+                    _lib.check(lib.dgcn_linear_gate(g2.data_ptr(), ldg, _lib.ptr(z), act, slope, t,
+                                                    d2.data_ptr() if act != 0 else None, _lib.ptr(parts), rows, N, stream),
+                               "dgcn_linear_gate")
+                    if need_b:
+                        gb = _param_sum(parts, bias_type)
+                if need_x:
+                    gx = torch.empty(x.shape, device=dev, dtype=x.dtype)
+                    _lib.check(lib.dgcn_linear_dx(d2.data_ptr(), ldd, w2.data_ptr(), ldw, t, gx.data_ptr(), rows, K, N,
+                                                  stream), "dgcn_linear_dx")
+                if need_w:
+                    gw = torch.empty(N, K, device=dev, dtype=weight.dtype)
+                    _lib.check(lib.dgcn_linear_dw(d2.data_ptr(), ldd, x2.data_ptr(), ldx, t, gw.data_ptr(), rows, K, N,
+                                                  stream), "dgcn_linear_dw")
+        return gx, gw, gb, (g if need_r else None), None, None
+
+
+def _linear_checks(what, x, weight, bias, residual, act, out_dtype):
+    code = ACTIVATIONS.get(act)
+    if code is None:
+        raise ValueError(f"{what}: act must be one of {', '.join(ACTIVATIONS)}, got {act!r}")
+    if weight.dim() != 2 or x.dim() < 1 or weight.size(1) != x.size(-1) or weight.size(0) < 1 or weight.size(1) < 1:
+        raise ValueError(f"{what}: rows (..., K) and a weight (N, K) with K, N >= 1, got {tuple(x.shape)} and "
+                         f"{tuple(weight.shape)}")
+    if max(weight.shape) > _MAX_K:
+        raise ValueError(f"{what}: at most {_MAX_K} channels, got {tuple(weight.shape)}")
+    N = weight.size(0)
+    if bias is not None:
+        if bias.dim() != 1 or bias.size(0) != N:
+            raise ValueError(f"bias must have shape ({N},), got {tuple(bias.shape)}")
+        if bias.dtype != out_dtype and bias.dtype != torch.float32:
+            raise TypeError(f"bias must be {out_dtype} or float32, got {bias.dtype}")
+    if residual is not None:
+        _same_rows(residual, x, N, out_dtype, "residual")
+    return code
+
+
+def linear_act(x, weight, bias=None, act: str = "none", residual=None, neg_slope: float = 0.2):
+    """``act(x @ weight.T + bias) + residual`` in one launch.
+
+    ``x`` (..., K) and ``weight`` (N, K) in one of fp32, bf16, fp16; ``bias`` (N,) in that type or fp32; ``residual``
+    (..., N) in that type; ``act`` one of :data:`ACTIVATIONS` (``neg_slope``: of leakyrelu, gelu: ``z Phi(z)``).  Gradients
+    of all four; the pre-activation is kept in the rows' type for them where there is an activation."""
+    _row_type(x, "linear_act")
+    if weight.dtype != x.dtype:
+        raise TypeError(f"linear_act: weight must be {x.dtype} as the rows are, got {weight.dtype}")
+    code = _linear_checks("linear_act", x, weight, bias, residual, act, x.dtype)
+    _lib.require_device(x, weight, bias, residual)
+    if _needs_grad(x, weight, bias, residual):
+        return _LinearAct.apply(x, weight, bias, residual, code, float(neg_slope))
+    return _linear_forward(x, weight, bias, residual, code, float(neg_slope), False)[0]
+
+
+def linear_act_e4m3(x: RowsE4M3, weight: RowsE4M3, bias=None, act: str = "none", residual=None,
+                    out_dtype=torch.bfloat16, neg_slope: float = 0.2):
+    """``act((x.data * x.scale) @ (weight.data * weight.scale).T + bias) + residual``: the products of e4m3 values are
+    exact, their sum is fp32, the scales join behind it.  ``x`` rows (..., K), ``weight`` rows (N, K) (``quantize_rows`` of
+    an nn.Linear weight, once); the result, ``residual`` and ``bias`` (or an fp32 bias) in ``out_dtype``.  No gradient."""
+    what = "linear_act_e4m3"
+    t = _TYPES.get(out_dtype)
+    if t is None:
+        raise TypeError(f"{what}: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    for name, r in (("x", x), ("weight", weight)):
+        if r.data.dtype != torch.float8_e4m3fn or r.scale.dtype != torch.float32:
+            raise TypeError(f"{what}: {name} must be float8_e4m3fn rows with float32 scales, got {r.data.dtype} and "
+                            f"{r.scale.dtype}")
+        if r.scale.shape != r.data.shape[:-1]:
+            raise ValueError(f"{what}: {name} of shape {tuple(r.data.shape)} needs scales of shape "
+                             f"{tuple(r.data.shape[:-1])}, got {tuple(r.scale.shape)}")
+    code = _linear_checks(what, x.data, weight.data, bias, residual, act, out_dtype)
+    dev = _lib.require_device(x.data, x.scale, weight.data, weight.scale, bias, residual)
+    _no_grad_only(what, bias, residual, x.scale, weight.scale)
+    x2, ldx = _rows2d(x.data)
+    w2, ldw = _rows2d(weight.data)
+    N, K = w2.shape
+    b = None if bias is None else bias.contiguous()
+    r2, ldr = _rows2d(residual) if residual is not None else (None, 0)
+    y = torch.empty((*x.data.shape[:-1], N), device=dev, dtype=out_dtype)
+    _linear_launch(x2, ldx, w2, ldw, x.scale.contiguous(), weight.scale.contiguous(), b,
+                   1 if b is not None and b.dtype == torch.float32 else 0, r2, ldr, code, float(neg_slope), _E4M3, t, None, y,
+                   K, N)
+    return y

@@ -35,6 +35,19 @@ extern "C" {
 #define DGCN_E_MODE (-4)      /* unknown mode / flag combination */
 #define DGCN_E_WORKSPACE (-5) /* workspace too small */
 
+/* element types of the node-wise MLP entry points (dgcn_rms_norm_*, dgcn_quantize_rows_e4m3, dgcn_linear_*) */
+#define DGCN_T_F32 0
+#define DGCN_T_BF16 1
+#define DGCN_T_F16 2
+#define DGCN_T_E4M3 3 /* 8 bits: 4 exponent, 3 mantissa bits, no infinities, largest 448 */
+
+/* activations of dgcn_linear_act */
+#define DGCN_ACT_NONE 0
+#define DGCN_ACT_RELU 1
+#define DGCN_ACT_LEAKY_RELU 2 /* z > 0 ? z : slope z */
+#define DGCN_ACT_GELU 3       /* z Phi(z), Phi the normal distribution function */
+#define DGCN_ACT_SILU 4       /* z / (1 + exp(-z)) */
+
 /* aggregation modes: gcn_lib/sparse/torch_message.py:44-85 */
 #define DGCN_AGGR_ADD 0     /* :46-47 -> PyG base scatter(reduce='add')  */
 #define DGCN_AGGR_MEAN 1    /* :46-47 -> scatter(reduce='mean')          */
@@ -701,6 +714,52 @@ int dgcn_rows_tn_f32(const float* g, int64_t ldg, const float* x, int64_t ldx, i
 int dgcn_rows_tn_colsum_f32(const float* g, int64_t ldg, const float* x, int64_t ldx, int64_t rows, int32_t C, int32_t K,
                             float* partials, float* out, int64_t ldo, int32_t transposed, int32_t colsum_of,
                             float* colsum, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Root-mean-square norm of rows with the residual's addition (csrc/rms_norm.hip):
+ *     h = x [+ res]      y = h * rstd * w      rstd = (mean over C of h^2 + eps)^(-1/2)
+ *   x, res (rows, C) in dtype, row strides ldx, ldr (any; 0 repeats a row); 1 <= C <= 32768
+ *   w (C) in dtype or, with w_f32, fp32; NULL = 1
+ *   y (rows, C) dtype contiguous, or instead of it q (rows, C) e4m3 contiguous and scale (rows): the row's y is q * scale,
+ *     scale = max |y| / 448 over the finite values of the row, at least 2^-126, and 1 where that maximum is 0; a NaN or
+ *     an infinity becomes NaN (0x7f) in its own place
+ *   h (rows, C) dtype contiguous or NULL (y does not depend on h's rounding); rstd (rows) or NULL
+ * Backward: dx = rstd (w g - xh mean(w g xh)) [+ gh], xh = h rstd, contiguous, or NULL; dw_part
+ *   [dgcn_rms_norm_num_partials(rows, C)][C] whose sum over the first axis (dgcn_param_sum) is the weight's gradient, or NULL.
+ * dgcn_quantize_rows_e4m3: q and scale of x itself.
+ * dgcn_param_sum: out[c] = sum over p of parts[p][c], c < width, rounded to dtype; fixed order. */
+int dgcn_rms_norm_fwd(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, int32_t w_f32, float eps,
+                      int32_t dtype, void* y, void* h, uint8_t* q, float* scale, float* rstd, int64_t rows, int32_t C,
+                      void* stream);
+int32_t dgcn_rms_norm_num_partials(int64_t rows, int32_t C);
+int dgcn_rms_norm_bwd(const void* g, int64_t ldg, const void* gh, int64_t ldgh, const void* h, int64_t ldh, const void* w,
+                      int32_t w_f32, const float* rstd, int32_t dtype, void* dx, float* dw_part, int64_t rows, int32_t C,
+                      void* stream);
+int dgcn_quantize_rows_e4m3(const void* x, int64_t ldx, int32_t dtype, uint8_t* q, float* scale, int64_t rows, int32_t C,
+                            void* stream);
+int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width, int32_t dtype, void* out, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Product of rows with a weight, bias, activation and residual in its epilogue (csrc/linear_act.hip):
+ *     z = x_scale w_scale (x w^T) + bias      y = act(z) + res
+ *   x (rows, K) row stride ldx, w (N, K) row stride ldw, both in in_type; K, N <= 2^20
+ *   in_type DGCN_T_E4M3: x_scale (rows) and w_scale (N) are required and out_type is free; otherwise out_type = in_type
+ *   bias (N) in out_type or, with bias_f32, fp32, or NULL; res (rows, N) out_type, row stride ldr, or NULL
+ *   z (rows, N) out_type contiguous, or NULL: kept for dgcn_linear_gate; y (rows, N) out_type contiguous
+ * Backward, all in one dtype:
+ *   dgcn_linear_gate: dz = g act'(z) contiguous (neither z nor dz with DGCN_ACT_NONE: dz is g), and db_part
+ *     [dgcn_linear_gate_num_partials(rows, N)][N], whose sum is the bias gradient, or NULL
+ *   dgcn_linear_dx: dx (rows, K) = dz w        dgcn_linear_dw: dw (N, K) = dz^T x */
+int dgcn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* x_scale, const float* w_scale,
+                    const void* bias, int32_t bias_f32, const void* res, int64_t ldr, int32_t act, float slope,
+                    int32_t in_type, int32_t out_type, void* z, void* y, int64_t rows, int32_t K, int32_t N, void* stream);
+int32_t dgcn_linear_gate_num_partials(int64_t rows, int32_t N);
+int dgcn_linear_gate(const void* g, int64_t ldg, const void* z, int32_t act, float slope, int32_t dtype, void* dz,
+                     float* db_part, int64_t rows, int32_t N, void* stream);
+int dgcn_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, int32_t dtype, void* dx, int64_t rows,
+                   int32_t K, int32_t N, void* stream);
+int dgcn_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, int32_t dtype, void* dw, int64_t rows,
+                   int32_t K, int32_t N, void* stream);
 
 #ifdef __cplusplus
 }

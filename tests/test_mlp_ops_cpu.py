@@ -1,0 +1,77 @@
+"""mlp_ops without a GPU: refusals of the entry points, and argument errors of the C entry points (nothing is launched)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from deep_gcns_torch_amd import _lib, blocks, mlp_ops
+from deep_gcns_torch_amd.mlp_ops import RowsE4M3
+
+X, W = torch.randn(3, 8), torch.randn(5, 8)
+
+
+def _e4m3(rows, k):
+    return RowsE4M3(torch.randn(rows, k).to(torch.float8_e4m3fn), torch.ones(rows))
+
+
+@pytest.mark.parametrize("call, error, text", [
+    (lambda: mlp_ops.rms_norm_rows(X.double()), TypeError, "float32, bfloat16 or float16"),
+    (lambda: mlp_ops.rms_norm_rows(torch.zeros(())), ValueError, "last dimension"),
+    (lambda: mlp_ops.rms_norm_rows(torch.zeros(3, 0)), ValueError, "last dimension"),
+    (lambda: mlp_ops.rms_norm_rows(torch.zeros(1, 32769)), ValueError, "at most 32768"),
+    (lambda: mlp_ops.rms_norm_rows(X, torch.ones(7)), ValueError, r"weight must have shape \(8,\)"),
+    (lambda: mlp_ops.rms_norm_rows(X, torch.ones(8, dtype=torch.float16)), TypeError, "weight must be"),
+    (lambda: mlp_ops.rms_norm_rows(X, residual=X[:2]), ValueError, "residual must have shape"),
+    (lambda: mlp_ops.rms_norm_rows(X, residual=X.half()), TypeError, "residual must be"),
+    (lambda: mlp_ops.rms_norm_rows(X), RuntimeError, "no CPU fallback"),
+    (lambda: mlp_ops.rms_norm_rows_e4m3(X), RuntimeError, "no CPU fallback"),
+    (lambda: mlp_ops.quantize_rows(torch.zeros(1, 32769)), ValueError, "at most 32768"),
+    (lambda: mlp_ops.quantize_rows(X.long()), TypeError, "float32, bfloat16 or float16"),
+    (lambda: mlp_ops.quantize_rows(X), RuntimeError, "no CPU fallback"),
+    (lambda: mlp_ops.linear_act(X, W.half()), TypeError, "weight must be"),
+    (lambda: mlp_ops.linear_act(X, W[:, :7]), ValueError, "weight"),
+    (lambda: mlp_ops.linear_act(X, W[0]), ValueError, "weight"),
+    (lambda: mlp_ops.linear_act(X, W[:0]), ValueError, "N >= 1"),
+    (lambda: mlp_ops.linear_act(X, torch.zeros(1, 8).expand((1 << 20) + 1, 8)), ValueError, "at most"),
+    (lambda: mlp_ops.linear_act(X, W, torch.ones(4)), ValueError, r"bias must have shape \(5,\)"),
+    (lambda: mlp_ops.linear_act(X, W, torch.ones(5).half()), TypeError, "bias must be"),
+    (lambda: mlp_ops.linear_act(X, W, act="tanh"), ValueError, "act must be one of"),
+    (lambda: mlp_ops.linear_act(X, W, residual=torch.ones(5)), ValueError, "residual must have shape"),
+    (lambda: mlp_ops.linear_act(X, W, residual=torch.ones(3, 5).half()), TypeError, "residual must be"),
+    (lambda: mlp_ops.linear_act(X, W), RuntimeError, "no CPU fallback"),
+    (lambda: mlp_ops.linear_act_e4m3(RowsE4M3(X, torch.ones(3)), _e4m3(5, 8)), TypeError, "float8_e4m3fn"),
+    (lambda: mlp_ops.linear_act_e4m3(_e4m3(3, 8), RowsE4M3(_e4m3(5, 8).data, torch.ones(4))), ValueError, "scales of shape"),
+    (lambda: mlp_ops.linear_act_e4m3(_e4m3(3, 8), _e4m3(5, 8), out_dtype=torch.float64), TypeError, "out_dtype"),
+    (lambda: mlp_ops.linear_act_e4m3(_e4m3(3, 8), _e4m3(5, 8), residual=torch.ones(3, 5)), TypeError, "residual must be"),
+    (lambda: mlp_ops.linear_act_e4m3(_e4m3(3, 8), _e4m3(5, 8)), RuntimeError, "no CPU fallback"),
+    (lambda: blocks.ResMLP(8, 16, act="tanh"), ValueError, "act must be one of"),
+])
+def test_refusals(call, error, text):
+    with pytest.raises(error, match=text):
+        call()
+
+
+def test_c_entry_argument_errors_do_not_launch():
+    lib = _lib.load()
+    buf = (C.c_float * 64)()
+    p = (C.addressof(buf) + 15) & ~15
+    norm = lib.dgcn_rms_norm_fwd
+    assert norm(None, 8, None, 0, None, 0, 1e-6, 0, p, None, None, None, None, 1, 8, None) == -1
+    assert norm(p, 8, None, 0, None, 0, 1e-6, 0, p, None, p, p, None, 1, 8, None) == -4        # y and q
+    assert norm(p, 8, None, 0, None, 0, 1e-6, 0, None, None, p, None, None, 1, 8, None) == -1  # q without scales
+    assert norm(p, 8, None, 0, None, 0, 1e-6, 3, p, None, None, None, None, 1, 8, None) == -4  # 8-bit rows have no norm
+    assert norm(p, 8, None, 0, None, 0, 1e-6, 0, p, None, None, None, None, 1, 32769, None) == -2
+    assert norm(p, 8, None, 0, None, 0, 1e-6, 0, p, None, None, None, None, 0, 8, None) == 0   # no rows: no launch
+    assert lib.dgcn_rms_norm_bwd(p, 8, None, 0, p, 8, None, 0, p, 0, None, None, 1, 8, None) == -1
+    assert lib.dgcn_quantize_rows_e4m3(p, 8, 0, p, None, 1, 8, None) == -1
+    assert lib.dgcn_param_sum(None, 1, 4, 0, p, None) == -1
+    assert lib.dgcn_rms_norm_num_partials(0, 8) == 0 and lib.dgcn_linear_gate_num_partials(0, 8) == 0
+    gate = lib.dgcn_linear_gate
+    assert gate(p, 8, None, 1, 0.2, 0, p, None, 1, 8, None) == -1                              # an activation needs z
+    assert gate(p, 8, p, 9, 0.2, 0, p, None, 1, 8, None) == -4
+
+
+def test_norm_layer_offers_rms():
+    from deep_gcns_torch_amd.gcn_lib.sparse.torch_nn import norm_layer
+    m = norm_layer("rms", 12)
+    assert isinstance(m, mlp_ops.RMSNorm) and list(m.state_dict()) == ["weight"] and m.weight.shape == (12,)
