@@ -1,0 +1,86 @@
+// What the product kernels share: the description of one product, and the epilogue of a run of consecutive channels.
+#pragma once
+
+#include "mlp_common.h"
+
+namespace dgcn {
+
+// Y(m, n) = epilogue( sum_k A(m, k) B(n, k) ).  An operand is K-contiguous, X(r, k) = x[r * ld + k] (t = 0: rows of a
+// Linear's input or weight), or K-strided, X(r, k) = x[k * ld + r] (t = 1: the weight under dx, both operands under dw).
+struct MatParams {
+  const void* a;
+  int64_t lda;
+  const void* b;
+  int64_t ldb;
+  const float* a_scale; // [M] or null
+  const float* b_scale; // [N] or null
+  const void* bias;     // [N] or null, in the output's type or fp32
+  int32_t bias_f32;
+  int32_t act;
+  float slope;
+  int32_t splits;       // > 1: the reduction in that many parts, fp32 partial sums part[split][M][N] instead of an epilogue
+  float* part;
+  const void* res;      // [M, N] row stride ldr, or null
+  int64_t ldr;
+  void* z;              // [M, N] contiguous, or null
+  void* y;              // [M, N] contiguous
+  int64_t M, N, K;
+};
+
+// bias, z, activation, residual and store of the channels n .. n + CNT - 1 of row m (v: the scaled sums)
+template <class O, int CNT>
+__device__ __forceinline__ void mat_epilogue(const MatParams& P, int64_t m, int64_t n, float (&v)[CNT]) {
+  constexpr bool EXACT = sizeof(O) == 4;
+  const int64_t at = m * P.N + n;
+  if (n + CNT <= P.N) {
+    if (P.bias) {
+#pragma unroll
+      for (int c = 0; c < CNT; c += 4) {
+        float b[4];
+        load_param4<O>(P.bias, P.bias_f32, n + c, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c + e] += b[e];
+      }
+    }
+    if (P.z) {
+#pragma unroll
+      for (int c = 0; c < CNT; c += 4) store4(static_cast<O*>(P.z) + at + c, v + c);
+    }
+    if (P.act != DGCN_ACT_NONE) {
+#pragma unroll
+      for (int e = 0; e < CNT; ++e) v[e] = act_fwd<EXACT>(v[e], P.act, P.slope);
+    }
+    if (P.res) {
+      const O* r = static_cast<const O*>(P.res) + m * P.ldr + n;
+#pragma unroll
+      for (int c = 0; c < CNT; c += 4) {
+        float b[4];
+        load4(r + c, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c + e] += b[e];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CNT; c += 4) store4(static_cast<O*>(P.y) + at + c, v + c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < CNT; ++e) {
+      if (n + e < P.N) {
+        float t = v[e];
+        if (P.bias) t += load_param<O>(P.bias, P.bias_f32, n + e);
+        if (P.z) static_cast<O*>(P.z)[at + e] = static_cast<O>(t);
+        t = act_fwd<EXACT>(t, P.act, P.slope);
+        if (P.res) t += static_cast<float>(static_cast<const O*>(P.res)[m * P.ldr + n + e]);
+        static_cast<O*>(P.y)[at + e] = static_cast<O>(t);
+      }
+    }
+  }
+}
+
+// The tiled product (linear_tile_*.hip), by operand type: 16-byte aligned operands, row strides a multiple of 16 bytes, the
+// contiguous extent of each operand a multiple of 16 bytes.  tile: 0 = 256 x 256, 1 = 128 x 128, 2 = 64 x 128 (K-contiguous A only)
+int mat_tile_bf16(const MatParams& P, int ta, int tb, int tile, hipStream_t s);
+int mat_tile_f16(const MatParams& P, int ta, int tb, int tile, hipStream_t s);
+int mat_tile_e4m3(const MatParams& P, int out_type, int tile, hipStream_t s);
+
+}  // namespace dgcn

@@ -7,28 +7,10 @@
 // Every sum is held in fp32.  z is kept for the backward rounded to the rows' type (half a step of z in act'(z)), and dz
 // is rounded to it before the two products, which take the rows' type on the matrix pipe.
 
-#include "mlp_common.h"
+#include "linear_act.h"
 
 namespace dgcn {
 namespace {
-
-struct MatParams {
-  const void* a;        // A(m, k) at a + m * am + k * ak
-  int64_t am, ak;
-  const void* b;        // B(n, k) at b + n * bn + k * bk
-  int64_t bn, bk;
-  const float* a_scale; // [M] or null
-  const float* b_scale; // [N] or null
-  const void* bias;     // [N] or null, in the output's type or fp32
-  int32_t bias_f32;
-  int32_t act;
-  float slope;
-  const void* res;      // [M, N] row stride ldr, or null
-  int64_t ldr;
-  void* z;              // [M, N] contiguous, or null
-  void* y;              // [M, N] contiguous
-  int64_t M, N, K;
-};
 
 __device__ __forceinline__ float elem(const uint8_t* p, int64_t i) {
   return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(p[i]), 0);
@@ -36,9 +18,9 @@ __device__ __forceinline__ float elem(const uint8_t* p, int64_t i) {
 template <class T>
 __device__ __forceinline__ float elem(const T* p, int64_t i) { return static_cast<float>(p[i]); }
 
-// The plain form of all three products: 64 x 64 tiles, fp32 operands in LDS, 4 x 4 sums a thread.
+// Products whose operands the tiled kernel does not take: 64 x 64 tiles, fp32 operands in LDS, 4 x 4 sums a thread.
 template <class T, class O>
-__global__ __launch_bounds__(256) void mat_simple_kernel(const MatParams P) {
+__global__ __launch_bounds__(256) void mat_simple_kernel(const MatParams P, int ta, int tb) {
   constexpr int BM = 64, BN = 64, BK = 16;
   __shared__ float As[BK][BM + 4], Bs[BK][BN + 4];
   const T* A = static_cast<const T*>(P.a);
@@ -51,10 +33,11 @@ __global__ __launch_bounds__(256) void mat_simple_kernel(const MatParams P) {
     for (int i = 0; i < 4; ++i) {
       const int idx = threadIdx.x + i * 256;
       // consecutive threads along the axis that is contiguous
-      const int ka = P.ak == 1 ? idx % BK : idx / BM, ma = P.ak == 1 ? idx / BK : idx % BM;
-      const int kb = P.bk == 1 ? idx % BK : idx / BN, nb = P.bk == 1 ? idx / BK : idx % BN;
-      As[ka][ma] = (m0 + ma < P.M && k0 + ka < P.K) ? elem(A, (m0 + ma) * P.am + (k0 + ka) * P.ak) : 0.f;
-      Bs[kb][nb] = (n0 + nb < P.N && k0 + kb < P.K) ? elem(B, (n0 + nb) * P.bn + (k0 + kb) * P.bk) : 0.f;
+      const int ka = ta ? idx / BM : idx % BK, ma = ta ? idx % BM : idx / BK;
+      const int kb = tb ? idx / BN : idx % BK, nb = tb ? idx % BN : idx / BK;
+      const int64_t m = m0 + ma, n = n0 + nb;
+      As[ka][ma] = (m < P.M && k0 + ka < P.K) ? elem(A, ta ? (k0 + ka) * P.lda + m : m * P.lda + k0 + ka) : 0.f;
+      Bs[kb][nb] = (n < P.N && k0 + kb < P.K) ? elem(B, tb ? (k0 + kb) * P.ldb + n : n * P.ldb + k0 + kb) : 0.f;
     }
     __syncthreads();
 #pragma unroll
@@ -72,37 +55,118 @@ __global__ __launch_bounds__(256) void mat_simple_kernel(const MatParams P) {
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + tm * 4 + i;
-    if (m >= P.M) continue;
+    const int64_t m = m0 + tm * 4 + i, n = n0 + tn * 4;
+    if (m >= P.M || n >= P.N) continue;
+    if (P.a_scale) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + tn * 4 + j;
-      if (n >= P.N) continue;
-      float z = acc[i][j];
-      if (P.a_scale) z *= P.a_scale[m];
-      if (P.b_scale) z *= P.b_scale[n];
-      if (P.bias) z += load_param<O>(P.bias, P.bias_f32, n);
-      if (P.z) static_cast<O*>(P.z)[m * P.N + n] = static_cast<O>(z);
-      float y = act_fwd<sizeof(O) == 4>(z, P.act, P.slope);
-      if (P.res) y += static_cast<float>(static_cast<const O*>(P.res)[m * P.ldr + n]);
-      static_cast<O*>(P.y)[m * P.N + n] = static_cast<O>(y);
+      for (int j = 0; j < 4; ++j) acc[i][j] *= P.a_scale[m] * (n + j < P.N ? P.b_scale[n + j] : 0.f);
     }
+    mat_epilogue<O, 4>(P, m, n, acc[i]);
+  }
+}
+
+// the epilogue of a product whose reduction was split: the partial sums are added in split order
+template <class O>
+__global__ __launch_bounds__(256) void split_join_kernel(const MatParams P) {
+  const int64_t per = (P.N + 3) / 4, total = P.M * per;
+  for (int64_t it = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; it < total; it += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t m = it / per, n = (it - m * per) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* p = P.part + m * P.N + n;
+    for (int s = 0; s < P.splits; ++s, p += P.M * P.N) {
+      float t[4];
+      if (n + 4 <= P.N) {
+        load4(p, t);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = n + j < P.N ? p[j] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += t[j];
+    }
+    mat_epilogue<O, 4>(P, m, n, v);
   }
 }
 
 template <class T, class O>
-int mat_launch(const MatParams& P, hipStream_t s) {
+int mat_simple(const MatParams& P, int ta, int tb, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>((P.M + 63) / 64), static_cast<unsigned>((P.N + 63) / 64));
-  hipLaunchKernelGGL((mat_simple_kernel<T, O>), grid, dim3(256), 0, s, P);
+  hipLaunchKernelGGL((mat_simple_kernel<T, O>), grid, dim3(256), 0, s, P, ta, tb);
   return launch_status();
 }
 
-int mat_same(const MatParams& P, int dtype, hipStream_t s) {
-  switch (dtype) {
-    case DGCN_T_F32: return mat_launch<float, float>(P, s);
-    case DGCN_T_BF16: return mat_launch<__bf16, __bf16>(P, s);
-    case DGCN_T_F16: return mat_launch<_Float16, _Float16>(P, s);
-    default: return DGCN_E_MODE;
+struct MatPlan {
+  int tile;             // tile size, or -1: the simple kernel
+  int splits;
+};
+
+// Tile and split by the cost of the alternatives, in cycles of a CU: a workgroup's step takes what its matrix instructions and LDS
+// traffic take (`work`, times the workgroups a CU holds), and at least the latency of the copies behind it; a split
+// writes and reads fp32 partial sums and launches once more.
+inline MatPlan mat_plan(int64_t M, int64_t N, int64_t K, int type, int ta) {
+  if (type == DGCN_T_F32) return {-1, 1};
+  struct { int bm, bn, held; double work; } tiles[3] = {{256, 256, 1, 3000.}, {128, 128, 2, 900.}, {64, 128, 3, 600.}};
+  const int64_t steps = (K + (type == DGCN_T_E4M3 ? 127 : 63)) / (type == DGCN_T_E4M3 ? 128 : 64);
+  const double cus = num_cus();
+  MatPlan best = {0, 1};
+  double least = 1e300;
+  for (int t = 0; t < (ta ? 2 : 3); ++t) {
+    const double wgs1 = static_cast<double>((M + tiles[t].bm - 1) / tiles[t].bm) * ((N + tiles[t].bn - 1) / tiles[t].bn);
+    for (int sp = 1; sp <= 64 && sp <= steps; sp *= 2) {
+      const double wgs = wgs1 * sp, per_cu = ceil(wgs / cus);
+      const double held = per_cu < tiles[t].held ? per_cu : tiles[t].held;
+      const double step = held * tiles[t].work > 2000. ? held * tiles[t].work : 2000.;
+      double c = ceil(per_cu / tiles[t].held) * ((steps + sp - 1) / sp * step + 4000.);
+      if (sp > 1) c += 8. * M * N * sp / 2000. + 10000.;
+      if (c < least) { least = c; best = {t, sp}; }
+    }
+  }
+  return best;
+}
+
+inline size_t plan_bytes(const MatPlan& p, int64_t M, int64_t N) {
+  return p.splits > 1 ? static_cast<size_t>(p.splits) * M * N * sizeof(float) : 0;
+}
+
+template <class O>
+int split_join(const MatParams& P, hipStream_t s) {
+  int64_t wgs = (P.M * ((P.N + 3) / 4) + 255) / 256;
+  if (wgs > 16 * num_cus()) wgs = 16 * num_cus();
+  hipLaunchKernelGGL((split_join_kernel<O>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, P);
+  return launch_status();
+}
+
+inline bool aligned16(const void* p, int64_t ld, int es) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * es % 16 == 0; }
+
+int mat_run(MatParams P, int ta, int tb, int in_type, int out_type, void* ws, size_t ws_bytes, hipStream_t s) {
+  MatPlan plan = mat_plan(P.M, P.N, P.K, in_type, ta);
+  const int es = in_type == DGCN_T_E4M3 ? 1 : 2;
+  const int64_t ca = ta ? P.M : P.K, cb = tb ? P.N : P.K;
+  if (!aligned16(P.a, P.lda, es) || !aligned16(P.b, P.ldb, es) || ca * es % 16 || cb * es % 16) plan = {-1, 1};
+  if (plan.splits > 1 && (ws_bytes < plan_bytes(plan, P.M, P.N) || !ws)) return DGCN_E_WORKSPACE;
+  P.splits = plan.splits;
+  P.part = static_cast<float*>(ws);
+  int rc = DGCN_E_MODE;
+  switch (in_type) {
+    case DGCN_T_F32: return mat_simple<float, float>(P, ta, tb, s);
+    case DGCN_T_BF16: rc = plan.tile < 0 ? mat_simple<__bf16, __bf16>(P, ta, tb, s) : mat_tile_bf16(P, ta, tb, plan.tile, s); break;
+    case DGCN_T_F16: rc = plan.tile < 0 ? mat_simple<_Float16, _Float16>(P, ta, tb, s) : mat_tile_f16(P, ta, tb, plan.tile, s); break;
+    case DGCN_T_E4M3:
+      if (plan.tile >= 0) {
+        rc = mat_tile_e4m3(P, out_type, plan.tile, s);
+      } else {
+        rc = out_type == DGCN_T_F32 ? mat_simple<uint8_t, float>(P, 0, 0, s)
+             : out_type == DGCN_T_BF16 ? mat_simple<uint8_t, __bf16>(P, 0, 0, s)
+             : out_type == DGCN_T_F16 ? mat_simple<uint8_t, _Float16>(P, 0, 0, s) : DGCN_E_MODE;
+      }
+      break;
+    default: break;
+  }
+  if (rc != DGCN_OK || plan.splits == 1) return rc;
+  switch (out_type) {
+    case DGCN_T_F32: return split_join<float>(P, s);
+    case DGCN_T_BF16: return split_join<__bf16>(P, s);
+    default: return split_join<_Float16>(P, s);
   }
 }
 
@@ -179,26 +243,28 @@ inline bool sizes_ok(int64_t rows, int32_t K, int32_t N) {
 
 using namespace dgcn;
 
+extern "C" size_t dgcn_linear_workspace(int32_t product, int64_t rows, int32_t K, int32_t N, int32_t in_type) {
+  if (rows <= 0 || K < 1 || N < 1) return 0;
+  switch (product) {
+    case 0: return plan_bytes(mat_plan(rows, N, K, in_type, 0), rows, N);
+    case 1: return plan_bytes(mat_plan(rows, K, N, in_type, 0), rows, K);
+    case 2: return plan_bytes(mat_plan(N, K, rows, in_type, 1), N, K);
+    default: return 0;
+  }
+}
+
 extern "C" int dgcn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* x_scale,
                                const float* w_scale, const void* bias, int32_t bias_f32, const void* res, int64_t ldr,
                                int32_t act, float slope, int32_t in_type, int32_t out_type, void* z, void* y, int64_t rows,
-                               int32_t K, int32_t N, void* stream) {
+                               int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream) {
   if (!x || !w || !y || (in_type == DGCN_T_E4M3 && (!x_scale || !w_scale))) return DGCN_E_NULL;
   if (!sizes_ok(rows, K, N) || ldx < 0 || ldw < 0 || (res && ldr < 0)) return DGCN_E_SHAPE;
-  if (!known_act(act) || (in_type != DGCN_T_E4M3 && in_type != out_type)) return DGCN_E_MODE;
+  if (!known_act(act) || out_type < DGCN_T_F32 || out_type > DGCN_T_F16 || (in_type != DGCN_T_E4M3 && in_type != out_type)) return DGCN_E_MODE;
   if (rows == 0) return DGCN_OK;
-  MatParams P = {x, ldx, 1, w, ldw, 1, x_scale, w_scale, bias, bias_f32, act, slope, res, ldr, z, y, rows, N, K};
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (in_type != DGCN_T_E4M3) {
-    P.a_scale = P.b_scale = nullptr;
-    return mat_same(P, in_type, s);
-  }
-  switch (out_type) {
-    case DGCN_T_F32: return mat_launch<uint8_t, float>(P, s);
-    case DGCN_T_BF16: return mat_launch<uint8_t, __bf16>(P, s);
-    case DGCN_T_F16: return mat_launch<uint8_t, _Float16>(P, s);
-    default: return DGCN_E_MODE;
-  }
+  const bool scaled = in_type == DGCN_T_E4M3;
+  const MatParams P = {x, ldx, w, ldw, scaled ? x_scale : nullptr, scaled ? w_scale : nullptr, bias, bias_f32, act, slope, 1,
+                       nullptr, res, ldr, z, y, rows, N, K};
+  return mat_run(P, 0, 0, in_type, out_type, ws, ws_bytes, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int32_t dgcn_linear_gate_num_partials(int64_t rows, int32_t N) {
@@ -234,18 +300,20 @@ extern "C" int dgcn_linear_gate(const void* g, int64_t ldg, const void* z, int32
 }
 
 extern "C" int dgcn_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, int32_t dtype, void* dx,
-                              int64_t rows, int32_t K, int32_t N, void* stream) {
+                              int64_t rows, int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream) {
   if (!dz || !w || !dx) return DGCN_E_NULL;
   if (!sizes_ok(rows, K, N) || lddz < 0 || ldw < 0) return DGCN_E_SHAPE;
+  if (dtype < DGCN_T_F32 || dtype > DGCN_T_F16) return DGCN_E_MODE;
   if (rows == 0) return DGCN_OK;
-  const MatParams P = {dz, lddz, 1, w, 1, ldw, nullptr, nullptr, nullptr, 0, DGCN_ACT_NONE, 0.f, nullptr, 0, nullptr, dx, rows, K, N};
-  return mat_same(P, dtype, static_cast<hipStream_t>(stream));
+  const MatParams P = {dz, lddz, w, ldw, nullptr, nullptr, nullptr, 0, DGCN_ACT_NONE, 0.f, 1, nullptr, nullptr, 0, nullptr, dx, rows, K, N};
+  return mat_run(P, 0, 1, dtype, dtype, ws, ws_bytes, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int dgcn_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, int32_t dtype, void* dw,
-                              int64_t rows, int32_t K, int32_t N, void* stream) {
+                              int64_t rows, int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream) {
   if (!dz || !x || !dw) return DGCN_E_NULL;
-  if (!sizes_ok(rows, K, N) || lddz < 0 || ldx < 0) return DGCN_E_SHAPE;
-  const MatParams P = {dz, 1, lddz, x, 1, ldx, nullptr, nullptr, nullptr, 0, DGCN_ACT_NONE, 0.f, nullptr, 0, nullptr, dw, N, K, rows};
-  return mat_same(P, dtype, static_cast<hipStream_t>(stream));
+  if (!sizes_ok(rows, K, N) || rows == 0 || lddz < 0 || ldx < 0) return DGCN_E_SHAPE;
+  if (dtype < DGCN_T_F32 || dtype > DGCN_T_F16) return DGCN_E_MODE;
+  const MatParams P = {dz, lddz, x, ldx, nullptr, nullptr, nullptr, 0, DGCN_ACT_NONE, 0.f, 1, nullptr, nullptr, 0, nullptr, dw, N, K, rows};
+  return mat_run(P, 1, 1, dtype, dtype, ws, ws_bytes, static_cast<hipStream_t>(stream));
 }

@@ -1,0 +1,288 @@
+// The tiled product on the matrix pipe: BM x BN tiles, 128 bytes of the reduction a step, operands copied straight from
+// memory into LDS (two buffers), 16 x 16 matrix instructions, fp32 sums.
+#pragma once
+
+#include <type_traits>
+
+#include "linear_act.h"
+
+namespace dgcn {
+namespace {
+
+typedef int i8v __attribute__((ext_vector_type(8)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s4v lds_s4;
+
+template <class T> struct MatIn;
+template <> struct MatIn<__bf16> {
+  static constexpr int ES = 2;
+  static __device__ __forceinline__ f32x4 mul(const u4v (&a)[2], const u4v (&b)[2], f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[0]), __builtin_bit_cast(bf16x8, b[0]), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[1]), __builtin_bit_cast(bf16x8, b[1]), c, 0, 0, 0);
+  }
+};
+template <> struct MatIn<_Float16> {
+  static constexpr int ES = 2;
+  static __device__ __forceinline__ f32x4 mul(const u4v (&a)[2], const u4v (&b)[2], f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[0]), __builtin_bit_cast(f16x8, b[0]), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[1]), __builtin_bit_cast(f16x8, b[1]), c, 0, 0, 0);
+  }
+};
+// e4m3 for a 16-bit result: one instruction of K = 128 at twice the 16-bit rate, its block scales held at 2^0.  It aligns
+// the products of eight neighbouring k to the largest one's exponent and drops what lies more than 13 bits below it
+// (measured, bit by bit), so a sum is off by up to 7 2^-13 of the largest product of each eight: 6e-5 of the result's
+// root mean square over normal rows, an order below a bf16 half step and under half of an fp16 one.
+template <> struct MatIn<uint8_t> {
+  static constexpr int ES = 1;
+  static __device__ __forceinline__ f32x4 mul(const u4v (&a)[2], const u4v (&b)[2], f32x4 c) {
+    const i8v aa = __builtin_bit_cast(i8v, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    const i8v bb = __builtin_bit_cast(i8v, __builtin_shufflevector(b[0], b[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(aa, bb, c, 0, 0, 0, 127, 0, 127);
+  }
+};
+// e4m3 for an fp32 result: every e4m3 value is an fp16 value; their products are exact and their sum is fp32
+struct WideE4m3 {};
+template <> struct MatIn<WideE4m3> {
+  static constexpr int ES = 1;
+  static __device__ __forceinline__ f16x8 widen(uint32_t lo, uint32_t hi) {
+    const u4v r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true))};
+    return __builtin_bit_cast(f16x8, r);
+  }
+  static __device__ __forceinline__ f32x4 mul(const u4v (&a)[2], const u4v (&b)[2], f32x4 c) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(a[s][0], a[s][1]), widen(b[s][0], b[s][1]), c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(a[s][2], a[s][3]), widen(b[s][2], b[s][3]), c, 0, 0, 0);
+    }
+    return c;
+  }
+};
+
+constexpr unsigned kRsrcFlags = 0x00027000;               // raw 32-bit buffer; a load behind its end gives zeros
+constexpr unsigned kBehind = 0x80000000u;                 // an offset behind any buffer here (at most 2^31 bytes)
+
+// Which rows / columns of an operand tile a 16-byte unit of LDS holds.
+//   K-contiguous, R rows of 128 bytes: unit u of row r holds the row's chunk u ^ f(r)
+//     (f = r & 7 for A; for B, whose fragments take rows 16 (i >> 2) + 4 t + (i & 3), f = (r & 3) | bit 4 of r << 2)
+//   K-strided, 64 k-rows of 2 R bytes: unit u of k-row k holds chunk u ^ 2 f(k), f = (k & 3) | bit 3 of k << 2
+// In both, lanes that read together fall on different banks.
+template <int T, int R, bool IS_B>
+__device__ __forceinline__ unsigned tile_offset(int inst, int lane, int64_t ld, int es) {
+  if constexpr (T == 0) {
+    const int row = inst * 8 + (lane >> 3);
+    const int f = IS_B ? ((row & 3) | ((row >> 4) & 1) << 2) : (row & 7);
+    return static_cast<unsigned>(row * ld * es) + (((lane & 7) ^ f) << 4);
+  } else {
+    constexpr int UNITS = R / 8;
+    const int k = inst * (64 / UNITS) + lane / UNITS;
+    const int f = (k & 3) | ((k >> 3) & 1) << 2;
+    return static_cast<unsigned>(k * ld * es) + (((lane % UNITS) ^ (2 * f)) << 4);
+  }
+}
+
+// T: operand type, O: output type, TA / TB: layouts; a wave owns 16 TM rows x 64 channels, a workgroup WM x WN waves
+template <class T, class O, int TA, int TB, int TM, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P) {
+  constexpr int ES = MatIn<T>::ES;
+  constexpr int BM = WM * TM * 16, BN = WN * 64, BK = 128 / ES, WAVES = WM * WN;
+  constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
+  constexpr int IA = BM / 8 / WAVES, IB = BN / 8 / WAVES;               // copies a wave makes per step
+  static_assert(IA * 8 * WAVES == BM && IB * 8 * WAVES == BN, "a step's copies divide over the waves");
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = lane_id(), wave = uni(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int i = lane & 15, q = lane >> 4;
+
+  // workgroup -> tile: consecutive tiles on one XCD (hardware deals workgroups to the XCDs in turn), in groups of eight
+  // tile rows, so that what an XCD works on at a time shares its operand panels in that XCD's L2
+  const int tm_n = static_cast<int>((P.M + BM - 1) / BM), tn_n = static_cast<int>((P.N + BN - 1) / BN);
+  int id = blockIdx.x;
+  {
+    const int total = tm_n * tn_n, xcd = id % kNumXCD, loc = id / kNumXCD, base = total / kNumXCD, extra = total % kNumXCD;
+    id = xcd * base + (xcd < extra ? xcd : extra) + loc;
+  }
+  const int group = id / (8 * tn_n), first = group * 8, high = tm_n - first < 8 ? tm_n - first : 8;
+  const int64_t m0 = static_cast<int64_t>(first + id % (8 * tn_n) % high) * BM;
+  const int64_t n0 = static_cast<int64_t>(id % (8 * tn_n) / high) * BN;
+
+  // this workgroup's part of the reduction
+  const int steps_all = static_cast<int>((P.K + BK - 1) / BK);
+  const int split = blockIdx.y;
+  const int s0 = static_cast<int>(static_cast<int64_t>(steps_all) * split / P.splits);
+  const int s1 = static_cast<int>(static_cast<int64_t>(steps_all) * (split + 1) / P.splits);
+
+  unsigned offa[IA], offb[IB];
+#pragma unroll
+  for (int c = 0; c < IA; ++c) offa[c] = tile_offset<TA, BM, false>(wave * IA + c, lane, P.lda, ES);
+#pragma unroll
+  for (int c = 0; c < IB; ++c) offb[c] = tile_offset<TB, BN, true>(wave * IB + c, lane, P.ldb, ES);
+  const int64_t rows_a = P.M - m0 < BM ? P.M - m0 : BM, rows_b = P.N - n0 < BN ? P.N - n0 : BN;
+
+  // Rows and k-rows behind the matrix lie behind the buffer's end and read as zeros; so do, by an offset of kBehind, the
+  // chunks of a K-contiguous row behind K.  Columns of a K-strided operand behind M or N read what is there: their sums
+  // are not stored.
+  auto copy = [&](int step, int buf) {
+    const int64_t k0 = static_cast<int64_t>(step) * BK;
+    const int64_t left = P.K - k0 < BK ? P.K - k0 : BK;
+    char* dst = lds + buf * STAGE;
+    auto one = [&](auto layout, auto count, const void* base, int64_t ld, int64_t line0, int64_t lines, const unsigned* off, char* to) {
+      constexpr int L = decltype(layout)::value, n = decltype(count)::value;
+      const char* p = static_cast<const char*>(base) + (L == 0 ? line0 * ld + k0 : k0 * ld + line0) * ES;
+      const int64_t bytes = (L == 0 ? (lines - 1) * ld + left : (left - 1) * ld + lines) * ES;
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, static_cast<int>(bytes), kRsrcFlags);
+      if (L == 0 && left < BK) {
+#pragma unroll
+        for (int c = 0; c < n; ++c) {
+          // byte of the row that this lane's chunk starts at
+          const unsigned at = off[c] - static_cast<unsigned>(((wave * n + c) * 8 + (lane >> 3)) * ld * ES);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(to + c * 1024), 16, at < left * ES ? off[c] : kBehind, 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < n; ++c) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(to + c * 1024), 16, off[c], 0, 0, 0);
+      }
+    };
+    one(std::integral_constant<int, TA>{}, std::integral_constant<int, IA>{}, P.a, P.lda, m0, rows_a, offa, dst + wave * IA * 1024);
+    one(std::integral_constant<int, TB>{}, std::integral_constant<int, IB>{}, P.b, P.ldb, n0, rows_b, offb, dst + A_BYTES + wave * IB * 1024);
+  };
+
+  f32x4 acc[TM][4];
+#pragma unroll
+  for (int tm = 0; tm < TM; ++tm) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[tm][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // fragment: element e of half s is k = 32 s + 8 q + e of operand row i (16-bit types; bytes likewise in e4m3)
+  const int rot = (q ^ (i & 7)) << 4;                                  // half 0; half 1 is the unit 4 further: ^ 64
+  const int kk = i >> 2, pc = i & 3, f2 = (kk | (q & 1) << 2) << 5;     // K-strided: this lane fetches 4 columns of k-row 8 q + kk
+  auto read = [&](auto layout, const char* base, int line, int rows, u4v (&out)[2]) {
+    constexpr int L = decltype(layout)::value;
+    if constexpr (L == 0) {
+      const char* p = base + line * 128;
+      out[0] = *reinterpret_cast<const u4v*>(p + rot);
+      out[1] = *reinterpret_cast<const u4v*>(p + (rot ^ 64));
+    } else {
+      // line: first of 16 columns; a row is rows * 2 bytes; h: k-rows 4 further
+      const char* p = base + (8 * q + kk) * rows * 2 + ((line * 2 + ((pc >> 1) << 4)) ^ f2) + (pc & 1) * 8;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (32 * s) * rows * 2));
+        const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (32 * s + 4) * rows * 2));
+        out[s] = __builtin_bit_cast(u4v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    }
+  };
+  // B's fragment t: with K-contiguous rows, matrix row r is channel 16 (r >> 2) + 4 t + (r & 3), so that a lane ends up with
+  // 16 consecutive channels; K-strided, channel 16 t + r
+  const int bline = TB == 0 ? wn * 64 + 16 * (i >> 2) + (i & 3) : wn * 64;
+
+  if (s0 < s1) copy(s0, 0);
+  for (int step = s0; step < s1; ++step) {
+    const int buf = (step - s0) & 1;
+    __builtin_amdgcn_s_waitcnt(0x0f70);                                // vmcnt(0): this wave's copies have landed
+    __syncthreads();                                                   // everyone's have; nobody still reads the other buffer
+    if (step + 1 < s1) copy(step + 1, buf ^ 1);
+    const char* sa = lds + buf * STAGE;
+    const char* sb = sa + A_BYTES;
+    u4v fb[4][2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) read(std::integral_constant<int, TB>{}, sb, bline + (TB == 0 ? 4 : 16) * t, BN, fb[t]);
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) {
+      u4v fa[2];
+      const int line = wm * TM * 16 + tm * 16 + (TA == 0 ? i : 0);
+      read(std::integral_constant<int, TA>{}, sa, line, BM, fa);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) acc[tm][t] = MatIn<T>::mul(fb[t], fa, acc[tm][t]);
+    }
+  }
+
+  // D: lane (i, q) holds row i of the tile's 16 and, of fragment t, matrix rows 4 q + j
+  float sc[16];
+  if constexpr (ES == 1) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int64_t n = n0 + wn * 64 + 16 * q + e;
+      sc[e] = n < P.N ? P.b_scale[n] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int tm = 0; tm < TM; ++tm) {
+    const int64_t m = m0 + wm * TM * 16 + tm * 16 + i;
+    if (m >= P.M) continue;
+    float as = 1.f;
+    if constexpr (ES == 1) as = P.a_scale[m];
+    if (P.splits > 1) {
+      float* out = P.part + (static_cast<int64_t>(split) * P.M + m) * P.N;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int64_t n = n0 + wn * 64 + (TB == 0 ? 16 * q + 4 * t : 16 * t + 4 * q);
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = acc[tm][t][j] * (ES == 1 ? as * sc[(4 * t + j) & 15] : 1.f);
+        if (n + 4 <= P.N) {
+          store4(out + n, v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (n + j < P.N) out[n + j] = v[j];
+          }
+        }
+      }
+    } else if constexpr (TB == 0) {
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = acc[tm][e >> 2][e & 3] * (ES == 1 ? as * sc[e] : 1.f);
+      mat_epilogue<O, 16>(P, m, n0 + wn * 64 + 16 * q, v);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = acc[tm][t][j];
+        mat_epilogue<O, 4>(P, m, n0 + wn * 64 + 16 * t + 4 * q, v);
+      }
+    }
+  }
+}
+
+template <class T, class O, int TA, int TB, int TM, int WM, int WN>
+int tile_launch(const MatParams& P, hipStream_t s) {
+  constexpr int BM = WM * TM * 16, BN = WN * 64;
+  constexpr int LDS = 2 * (BM + BN) * 128;
+  const int64_t tiles = ((P.M + BM - 1) / BM) * ((P.N + BN - 1) / BN);
+  // 32-bit offsets inside a tile's lines, 31-bit tile count
+  const int64_t far = MatIn<T>::ES * 256 * (P.lda > P.ldb ? P.lda : P.ldb);
+  if (tiles > 0x7fffffff || far + 2 * 128 * 256 > 0x7fffffff || P.splits < 1 || P.splits > 65535) return DGCN_E_SHAPE;
+  const void* fn = reinterpret_cast<const void*>(tile_kernel<T, O, TA, TB, TM, WM, WN>);
+  const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  if (e != hipSuccess) return static_cast<int>(e);
+  hipLaunchKernelGGL((tile_kernel<T, O, TA, TB, TM, WM, WN>), dim3(static_cast<unsigned>(tiles), P.splits), dim3(WM * WN * 64), LDS, s, P);
+  return launch_status();
+}
+
+template <class T, class O, int TA, int TB>
+int tile_size(const MatParams& P, int tile, hipStream_t s) {
+  if (tile == 0) return tile_launch<T, O, TA, TB, 8, 2, 4>(P, s);
+  if (tile == 1) return tile_launch<T, O, TA, TB, 4, 2, 2>(P, s);
+  if constexpr (TA == 0) {
+    if (tile == 2) return tile_launch<T, O, TA, TB, 2, 2, 2>(P, s);
+  }
+  return DGCN_E_MODE;
+}
+
+template <class T>
+int tile_layout(const MatParams& P, int ta, int tb, int tile, hipStream_t s) {
+  if (ta == 0 && tb == 0) return tile_size<T, T, 0, 0>(P, tile, s);
+  if (ta == 0 && tb == 1) return tile_size<T, T, 0, 1>(P, tile, s);
+  if (ta == 1 && tb == 1) return tile_size<T, T, 1, 1>(P, tile, s);
+  return DGCN_E_MODE;
+}
+
+}  // namespace
+}  // namespace dgcn

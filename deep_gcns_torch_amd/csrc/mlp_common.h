@@ -16,11 +16,15 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // at any byte.  Rows of odd length or stride take the same wide loads as aligned ones.
 typedef u4v u4v_any2 __attribute__((aligned(2)));
 typedef u4v u4v_any4 __attribute__((aligned(4)));
+typedef u2v u2v_any2 __attribute__((aligned(2)));
 typedef u2v u2v_any1 __attribute__((aligned(1)));
 
 template <class T> struct Vec8;
 template <> struct Vec8<__bf16> { typedef bf16x8 type; };
 template <> struct Vec8<_Float16> { typedef f16x8 type; };
+template <class T> struct Vec4;
+template <> struct Vec4<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4))); };
+template <> struct Vec4<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4))); };
 
 template <class T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
@@ -90,6 +94,40 @@ __device__ __forceinline__ float load_param(const void* p, bool f32, int64_t i) 
   return f32 ? static_cast<const float*>(p)[i] : static_cast<float>(static_cast<const T*>(p)[i]);
 }
 
+template <class T>
+__device__ __forceinline__ void load4(const T* p, float* v) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 a = __builtin_bit_cast(f32x4, *reinterpret_cast<const u4v_any4*>(p));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = a[e];
+  } else {
+    const auto a = __builtin_bit_cast(typename Vec4<T>::type, *reinterpret_cast<const u2v_any2*>(p));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(a[e]);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* p, const float* v) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<u4v_any4*>(p) = __builtin_bit_cast(u4v, f32x4{v[0], v[1], v[2], v[3]});
+  } else {
+    typename Vec4<T>::type a;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] = static_cast<T>(v[e]);
+    *reinterpret_cast<u2v_any2*>(p) = __builtin_bit_cast(u2v, a);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void load_param4(const void* p, bool f32, int64_t i, float* v) {
+  if (f32) {
+    load4(static_cast<const float*>(p) + i, v);
+  } else {
+    load4(static_cast<const T*>(p) + i, v);
+  }
+}
+
 // four fp32 values -> four e4m3 bytes, to nearest even (|v| <= 448 up to rounding; anything not finite -> NaN, 0x7f)
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
@@ -97,17 +135,39 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
 }
 
 // ---- activations: act(z) and act'(z), in fp32 ----
-// EXACT: libm's exp (the fp32 type); otherwise the hardware's 2^x, whose error of |z| 2^-24 is far below a 16-bit step
+// EXACT (the fp32 type): libm's exp and erfc.  Otherwise the hardware's 2^x, off by |z| 2^-24, and the normal distribution
+// function below, off by 1e-5 of its value: both far below a 16-bit half step (bf16 2^-9, fp16 2^-12 of a value in [1, 2)).
 template <bool EXACT>
 __device__ __forceinline__ float act_exp(float x) { return EXACT ? expf(x) : fast_exp(x); }
+
+// Phi(z) and, in `bell`, exp(-z^2 / 2).  Both sides come from erfc(|z| / sqrt 2), so that nothing cancels for z < 0:
+// erfc(x) = exp(-x^2) t P(t), t = 1 / (1 + 0.45 x), P of degree five fitted to the least relative error over 0 <= x <= 14
+// (9.6e-6); libm's erfc is some five times as many instructions, and a 256 x 256 tile evaluates 65,536 of them.
+template <bool EXACT>
+__device__ __forceinline__ float normal_cdf(float z, float& bell) {
+  bell = act_exp<EXACT>(-0.5f * z * z);
+  if constexpr (EXACT) return 0.5f * erfcf(z * -0.70710678118654752f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.45f * 0.70710678118654752f, fabsf(z), 1.f));
+  float p = -0.135856623f;
+  p = fmaf(p, t, 0.292237032f);
+  p = fmaf(p, t, 0.0894637792f);
+  p = fmaf(p, t, 0.248475618f);
+  p = fmaf(p, t, 0.251702589f);
+  p = fmaf(p, t, 0.25396813f);
+  const float tail = 0.5f * p * t * bell;                              // Phi(-|z|)
+  return z < 0.f ? tail : 1.f - tail;
+}
 
 template <bool EXACT>
 __device__ __forceinline__ float act_fwd(float z, int act, float slope) {
   switch (act) {
-    case DGCN_ACT_RELU: return z < 0.f ? 0.f : z;                        // (NaN stays NaN)
+    case DGCN_ACT_RELU: return z < 0.f ? 0.f : z;                       // (NaN stays NaN)
     case DGCN_ACT_LEAKY_RELU: return z > 0.f ? z : slope * z;
-    case DGCN_ACT_GELU: return 0.5f * z * erfcf(z * -0.70710678118654752f);   // (1 + erf would cancel for z < 0)
-    case DGCN_ACT_SILU: return z / (1.f + act_exp<EXACT>(-z));
+    case DGCN_ACT_GELU: {
+      float bell;
+      return z * normal_cdf<EXACT>(z, bell);
+    }
+    case DGCN_ACT_SILU: return EXACT ? z / (1.f + act_exp<EXACT>(-z)) : z * __builtin_amdgcn_rcpf(1.f + act_exp<EXACT>(-z));
     default: return z;
   }
 }
@@ -117,10 +177,13 @@ __device__ __forceinline__ float act_slope(float z, int act, float slope) {
   switch (act) {
     case DGCN_ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case DGCN_ACT_LEAKY_RELU: return z > 0.f ? 1.f : slope;
-    case DGCN_ACT_GELU:
-      return 0.5f * erfcf(z * -0.70710678118654752f) + z * 0.39894228040143268f * act_exp<EXACT>(-0.5f * z * z);
+    case DGCN_ACT_GELU: {
+      float bell;
+      const float cdf = normal_cdf<EXACT>(z, bell);
+      return fmaf(z * 0.39894228040143268f, bell, cdf);
+    }
     case DGCN_ACT_SILU: {
-      const float s = 1.f / (1.f + act_exp<EXACT>(-z));
+      const float s = EXACT ? 1.f / (1.f + act_exp<EXACT>(-z)) : __builtin_amdgcn_rcpf(1.f + act_exp<EXACT>(-z));
       return s * (1.f + z * (1.f - s));
     }
     default: return 1.f;

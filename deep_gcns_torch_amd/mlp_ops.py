@@ -237,14 +237,21 @@ class RMSNorm(nn.Module):
 
 
 # ---- product with epilogue ------------------------------------------------------------------------------------------
+def _workspace(product: int, rows: int, K: int, N: int, in_type: int, dev):
+    """(workspace or None, its bytes) of one product call: memory of that call alone, also inside a captured graph."""
+    n = _lib.load().dgcn_linear_workspace(product, rows, K, N, in_type)
+    return (torch.empty(n, device=dev, dtype=torch.uint8), n) if n else (None, 0)
+
+
 def _linear_launch(x2, ldx, w2, ldw, sx, sw, bias, bias_f32, r2, ldr, act, slope, in_type, out_type, z, y, K, N):
     dev = y.device
     if y.numel() == 0:
         return
+    ws, ws_bytes = _workspace(0, x2.size(0), K, N, in_type, dev)
     with _lib.device_ctx(dev):
         _lib.check(_lib.load().dgcn_linear_act(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _lib.ptr(sx), _lib.ptr(sw),
                                                _lib.ptr(bias), bias_f32, _lib.ptr(r2), ldr, act, slope, in_type, out_type,
-                                               _lib.ptr(z), y.data_ptr(), x2.size(0), K, N,
+                                               _lib.ptr(z), y.data_ptr(), x2.size(0), K, N, _lib.ptr(ws), ws_bytes,
                                                _lib.current_stream_handle(dev)), "dgcn_linear_act")
 
 
@@ -304,12 +311,14 @@ class _LinearAct(torch.autograd.Function):
                         gb = _param_sum(parts, bias_type)
                 if need_x:
                     gx = torch.empty(x.shape, device=dev, dtype=x.dtype)
+                    ws, ws_bytes = _workspace(1, rows, K, N, t, dev)
                     _lib.check(lib.dgcn_linear_dx(d2.data_ptr(), ldd, w2.data_ptr(), ldw, t, gx.data_ptr(), rows, K, N,
-                                                  stream), "dgcn_linear_dx")
+                                                  _lib.ptr(ws), ws_bytes, stream), "dgcn_linear_dx")
                 if need_w:
                     gw = torch.empty(N, K, device=dev, dtype=weight.dtype)
+                    ws, ws_bytes = _workspace(2, rows, K, N, t, dev)
                     _lib.check(lib.dgcn_linear_dw(d2.data_ptr(), ldd, x2.data_ptr(), ldx, t, gw.data_ptr(), rows, K, N,
-                                                  stream), "dgcn_linear_dw")
+                                                  _lib.ptr(ws), ws_bytes, stream), "dgcn_linear_dw")
         return gx, gw, gb, (g if need_r else None), None, None
 
 

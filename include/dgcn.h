@@ -749,17 +749,21 @@ int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width, int32_t dt
  * Backward, all in one dtype:
  *   dgcn_linear_gate: dz = g act'(z) contiguous (neither z nor dz with DGCN_ACT_NONE: dz is g), and db_part
  *     [dgcn_linear_gate_num_partials(rows, N)][N], whose sum is the bias gradient, or NULL
- *   dgcn_linear_dx: dx (rows, K) = dz w        dgcn_linear_dw: dw (N, K) = dz^T x */
+ *   dgcn_linear_dx: dx (rows, K) = dz w        dgcn_linear_dw: dw (N, K) = dz^T x
+ * ws: dgcn_linear_workspace(product, rows, K, N, in_type) bytes, 16-byte aligned, of this call's own (fp32 partial sums of a
+ *   split reduction; may be 0 and NULL); product 0: dgcn_linear_act, 1: dgcn_linear_dx, 2: dgcn_linear_dw. */
+size_t dgcn_linear_workspace(int32_t product, int64_t rows, int32_t K, int32_t N, int32_t in_type);
 int dgcn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* x_scale, const float* w_scale,
                     const void* bias, int32_t bias_f32, const void* res, int64_t ldr, int32_t act, float slope,
-                    int32_t in_type, int32_t out_type, void* z, void* y, int64_t rows, int32_t K, int32_t N, void* stream);
+                    int32_t in_type, int32_t out_type, void* z, void* y, int64_t rows, int32_t K, int32_t N, void* ws,
+                    size_t ws_bytes, void* stream);
 int32_t dgcn_linear_gate_num_partials(int64_t rows, int32_t N);
 int dgcn_linear_gate(const void* g, int64_t ldg, const void* z, int32_t act, float slope, int32_t dtype, void* dz,
                      float* db_part, int64_t rows, int32_t N, void* stream);
 int dgcn_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, int32_t dtype, void* dx, int64_t rows,
-                   int32_t K, int32_t N, void* stream);
+                   int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream);
 int dgcn_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, int32_t dtype, void* dw, int64_t rows,
-                   int32_t K, int32_t N, void* stream);
+                   int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -216,7 +216,9 @@ def check_linear_grads(x, w, b, r, act, g, grads, z, ez, dtype):
 
 LINEAR_SHAPES = [(1, 8, 8), (1, 1, 1), (1, 4096, 512), (2, 17, 5), (16, 256, 4096), (17, 129, 65), (33, 64, 300),
                  (65, 1000, 72), (128, 128, 128), (100, 2048, 40), (257, 520, 264), (300, 96, 1025), (1500, 112, 224),
-                 (5000, 128, 256), (1025, 13, 7), (0, 16, 24)]
+                 (5000, 128, 256), (1025, 13, 7), (0, 16, 24),
+                 # whole and ragged tiles of each size, long and split reductions
+                 (4096, 72, 4104), (2049, 1096, 2056), (60, 8192, 512), (700, 4096, 264), (129, 6152, 136), (9000, 264, 520)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -249,8 +251,27 @@ def test_linear_act_e4m3(out, rows, K, N, act, bias, residual):
     y = mlp_ops.linear_act_e4m3(x, w, b, act=act, residual=r, out_dtype=out)
     xd, wd = (t.data.double() * t.scale.double().unsqueeze(-1) for t in (x, w))
     z, ez, y64, ey = linear_bounds(xd, wd, b, act, out, torch.float8_e4m3fn)
+    if out != torch.float32:
+        # The 8-bit matrix instruction cuts each product to a multiple of 2^(E - 13), E the exponent of the largest of the
+        # eight neighbouring ones (test_e4m3_products_share_an_exponent_by_eight): seven products of each eight are off by
+        # less than 2^-13 of the largest, which is at most max|x| max|w| over the eight.
+        top = [torch.nn.functional.pad(t.abs(), (0, -K % 8)).unflatten(1, (-1, 8)).amax(-1) for t in (xd, wd)]
+        ey = ey + LIP[act][0] * 7 * 2.0 ** -13 * (top[0] @ top[1].t())
     y64 = y64 if r is None else y64 + r.double()
     within(y, y64, ey * 1.01 + z.abs() * 4 * U + y64.abs() * (half_step(out) * 1.01 + U) + TINY[out], "y")
+
+
+def test_e4m3_products_share_an_exponent_by_eight():
+    """What the tolerance above says of the instruction, and that an fp32 result does not have it: 2^16 - 2^16 + 2^(16 - d)."""
+    for where, d, kept in ((2, 13, True), (2, 14, False), (7, 14, False), (8, 20, True), (40, 26, True)):
+        x, w = torch.zeros(64, 128, device="cuda"), torch.zeros(64, 128, device="cuda")
+        x[:, 0], w[:, 0], x[:, 1], w[:, 1] = 256.0, 256.0, 256.0, -256.0
+        x[:, where], w[:, where] = 2.0 ** ((17 - d) // 2), 2.0 ** (16 - d - (17 - d) // 2)
+        one = torch.ones(64, device="cuda")
+        rows = [RowsE4M3(t.to(torch.float8_e4m3fn), one) for t in (x, w)]
+        full = torch.full((64, 64), 2.0 ** (16 - d), device="cuda")
+        assert torch.equal(mlp_ops.linear_act_e4m3(*rows, out_dtype=torch.float32), full)
+        assert torch.equal(mlp_ops.linear_act_e4m3(*rows, out_dtype=torch.bfloat16).float(), full if kept else 0 * full)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
