@@ -31,50 +31,23 @@ struct MatParams {
 template <class O, int CNT>
 __device__ __forceinline__ void mat_epilogue(const MatParams& P, int64_t m, int64_t n, float (&v)[CNT]) {
   constexpr bool EXACT = sizeof(O) == 4;
-  const int64_t at = m * P.N + n;
-  if (n + CNT <= P.N) {
-    if (P.bias) {
+  const int64_t at = m * P.N;
+  const int first = static_cast<int>(n), N = static_cast<int>(P.N);
+  if (P.bias) {
+    float b[CNT];
+    load_param_run<O, CNT>(P.bias, P.bias_f32, first, N, b);
 #pragma unroll
-      for (int c = 0; c < CNT; c += 4) {
-        float b[4];
-        load_param4<O>(P.bias, P.bias_f32, n + c, b);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[c + e] += b[e];
-      }
-    }
-    if (P.z) {
-#pragma unroll
-      for (int c = 0; c < CNT; c += 4) store4(static_cast<O*>(P.z) + at + c, v + c);
-    }
-    if (P.act != DGCN_ACT_NONE) {
-#pragma unroll
-      for (int e = 0; e < CNT; ++e) v[e] = act_fwd<EXACT>(v[e], P.act, P.slope);
-    }
-    if (P.res) {
-      const O* r = static_cast<const O*>(P.res) + m * P.ldr + n;
-#pragma unroll
-      for (int c = 0; c < CNT; c += 4) {
-        float b[4];
-        load4(r + c, b);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[c + e] += b[e];
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < CNT; c += 4) store4(static_cast<O*>(P.y) + at + c, v + c);
-  } else {
-#pragma unroll
-    for (int e = 0; e < CNT; ++e) {
-      if (n + e < P.N) {
-        float t = v[e];
-        if (P.bias) t += load_param<O>(P.bias, P.bias_f32, n + e);
-        if (P.z) static_cast<O*>(P.z)[at + e] = static_cast<O>(t);
-        t = act_fwd<EXACT>(t, P.act, P.slope);
-        if (P.res) t += static_cast<float>(static_cast<const O*>(P.res)[m * P.ldr + n + e]);
-        static_cast<O*>(P.y)[at + e] = static_cast<O>(t);
-      }
-    }
+    for (int e = 0; e < CNT; ++e) v[e] += b[e];
   }
+  if (P.z) store_run<O, CNT>(static_cast<O*>(P.z) + at, first, N, v);
+  act_run<EXACT, CNT>(v, P.act, P.slope);
+  if (P.res) {
+    float r[CNT];
+    load_run<O, CNT>(static_cast<const O*>(P.res) + m * P.ldr, first, N, r);
+#pragma unroll
+    for (int e = 0; e < CNT; ++e) v[e] += r[e];
+  }
+  store_run<O, CNT>(static_cast<O*>(P.y) + at, first, N, v);
 }
 
 // The tiled product (linear_tile_*.hip), by operand type: 16-byte aligned operands, row strides a multiple of 16 bytes, the

@@ -202,50 +202,46 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
     }
   }
 
-  // D: lane (i, q) holds row i of the tile's 16 and, of fragment t, matrix rows 4 q + j
-  float sc[16];
-  if constexpr (ES == 1) {
+  // Epilogue, through LDS (the operand buffers are free): a wave writes its sums as rows of 64 channels, up to 64 rows at a
+  // time, and takes them back eight rows by eight channels a lane, so that a store fills whole lines and the code is one
+  // rolled loop.  Lane (i, q) holds row i of each 16 and, of fragment t, matrix rows 4 q .. 4 q + 3.  16-byte unit u of row
+  // r lies at u ^ (r & 15).  A wave reads only what it wrote.
+  constexpr int PASS = TM < 4 ? TM : 4;
+  __syncthreads();
+  char* mine = lds + wave * (PASS * 16 * 256);
+  const int64_t mw = m0 + wm * TM * 16, n = n0 + wn * 64 + 8 * (lane & 7);
+  float bs[8];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int64_t n = n0 + wn * 64 + 16 * q + e;
-      sc[e] = n < P.N ? P.b_scale[n] : 0.f;
-    }
-  }
+  for (int e = 0; e < 8; ++e) bs[e] = (ES == 1 && n + e < P.N) ? P.b_scale[n + e] : 1.f;
 #pragma unroll
-  for (int tm = 0; tm < TM; ++tm) {
-    const int64_t m = m0 + wm * TM * 16 + tm * 16 + i;
-    if (m >= P.M) continue;
-    float as = 1.f;
-    if constexpr (ES == 1) as = P.a_scale[m];
-    if (P.splits > 1) {
-      float* out = P.part + (static_cast<int64_t>(split) * P.M + m) * P.N;
+  for (int p = 0; p < TM / PASS; ++p) {
+#pragma unroll
+    for (int tm = 0; tm < PASS; ++tm) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int64_t n = n0 + wn * 64 + (TB == 0 ? 16 * q + 4 * t : 16 * t + 4 * q);
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = acc[tm][t][j] * (ES == 1 ? as * sc[(4 * t + j) & 15] : 1.f);
-        if (n + 4 <= P.N) {
-          store4(out + n, v);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (n + j < P.N) out[n + j] = v[j];
-          }
-        }
+        const int unit = TB == 0 ? 4 * q + t : 4 * t + q;
+        *reinterpret_cast<f32x4*>(mine + (tm * 16 + i) * 256 + ((unit ^ i) << 4)) = acc[p * PASS + tm][t];
       }
-    } else if constexpr (TB == 0) {
-      float v[16];
+    }
+#pragma unroll 1
+    for (int r0 = 0; r0 < PASS * 16; r0 += 8) {
+      const int r = r0 + (lane >> 3), u = 2 * (lane & 7);
+      const int64_t m = mw + p * PASS * 16 + r;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + r * 256 + ((u ^ (r & 15)) << 4));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((u + 1) ^ (r & 15)) << 4));
+      if (m < P.M && n < P.N) {
+        const float as = ES == 1 ? P.a_scale[m] : 1.f;
+        float v[8];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = acc[tm][e >> 2][e & 3] * (ES == 1 ? as * sc[e] : 1.f);
-      mat_epilogue<O, 16>(P, m, n0 + wn * 64 + 16 * q, v);
-    } else {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = acc[tm][t][j];
-        mat_epilogue<O, 4>(P, m, n0 + wn * 64 + 16 * t + 4 * q, v);
+        for (int e = 0; e < 4; ++e) {
+          v[e] = ES == 1 ? lo[e] * (as * bs[e]) : lo[e];
+          v[4 + e] = ES == 1 ? hi[e] * (as * bs[4 + e]) : hi[e];
+        }
+        if (P.splits > 1) {
+          store_chunk(P.part + (static_cast<int64_t>(split) * P.M + m) * P.N, n, P.N, v);
+        } else {
+          mat_epilogue<O, 8>(P, m, n, v);
+        }
       }
     }
   }

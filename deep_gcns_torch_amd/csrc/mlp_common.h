@@ -53,47 +53,6 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   }
 }
 
-// elements [start, start + 8) of a row of n (the part behind the end reads as `fill`, and is not written)
-template <class T>
-__device__ __forceinline__ void load_chunk(const T* row, int start, int n, float (&v)[8], float fill = 0.f) {
-  if (start + 8 <= n) {
-    load8(row + start, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = start + e < n ? static_cast<float>(row[start + e]) : fill;
-  }
-}
-
-template <class T>
-__device__ __forceinline__ void store_chunk(T* row, int start, int n, const float (&v)[8]) {
-  if (start + 8 <= n) {
-    store8(row + start, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (start + e < n) row[start + e] = static_cast<T>(v[e]);
-    }
-  }
-}
-
-// parameters (weight, bias) come in the rows' type or in fp32
-template <class T>
-__device__ __forceinline__ void load_param_chunk(const void* p, bool f32, int start, int n, float (&v)[8], float none) {
-  if (!p) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = none;
-  } else if (f32) {
-    load_chunk(static_cast<const float*>(p), start, n, v, none);
-  } else {
-    load_chunk(static_cast<const T*>(p), start, n, v, none);
-  }
-}
-
-template <class T>
-__device__ __forceinline__ float load_param(const void* p, bool f32, int64_t i) {
-  return f32 ? static_cast<const float*>(p)[i] : static_cast<float>(static_cast<const T*>(p)[i]);
-}
-
 template <class T>
 __device__ __forceinline__ void load4(const T* p, float* v) {
   if constexpr (sizeof(T) == 4) {
@@ -119,13 +78,63 @@ __device__ __forceinline__ void store4(T* p, const float* v) {
   }
 }
 
-template <class T>
-__device__ __forceinline__ void load_param4(const void* p, bool f32, int64_t i, float* v) {
-  if (f32) {
-    load4(static_cast<const float*>(p) + i, v);
+// elements [start, start + CNT) of a row of n, CNT = 4 or 8 (behind the end: reads as `fill`, is not written)
+template <class T, int CNT>
+__device__ __forceinline__ void load_run(const T* row, int start, int n, float (&v)[CNT], float fill = 0.f) {
+  if (start + CNT <= n) {
+    if constexpr (CNT == 8) load8(row + start, v); else load4(row + start, v);
   } else {
-    load4(static_cast<const T*>(p) + i, v);
+#pragma unroll
+    for (int e = 0; e < CNT; ++e) v[e] = start + e < n ? static_cast<float>(row[start + e]) : fill;
   }
+}
+
+template <class T, int CNT>
+__device__ __forceinline__ void store_run(T* row, int start, int n, const float (&v)[CNT]) {
+  if (start + CNT <= n) {
+    if constexpr (CNT == 8) store8(row + start, v); else store4(row + start, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < CNT; ++e) {
+      if (start + e < n) row[start + e] = static_cast<T>(v[e]);
+    }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void load_chunk(const T* row, int start, int n, float (&v)[8], float fill = 0.f) {
+  load_run<T, 8>(row, start, n, v, fill);
+}
+template <class T>
+__device__ __forceinline__ void store_chunk(T* row, int start, int n, const float (&v)[8]) {
+  store_run<T, 8>(row, start, n, v);
+}
+
+template <class T, int CNT>
+__device__ __forceinline__ void load_param_run(const void* p, bool f32, int start, int n, float (&v)[CNT]) {
+  if (f32) {
+    load_run<float, CNT>(static_cast<const float*>(p), start, n, v);
+  } else {
+    load_run<T, CNT>(static_cast<const T*>(p), start, n, v);
+  }
+}
+
+// parameters (weight, bias) come in the rows' type or in fp32
+template <class T>
+__device__ __forceinline__ void load_param_chunk(const void* p, bool f32, int start, int n, float (&v)[8], float none) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = none;
+  } else if (f32) {
+    load_chunk(static_cast<const float*>(p), start, n, v, none);
+  } else {
+    load_chunk(static_cast<const T*>(p), start, n, v, none);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ float load_param(const void* p, bool f32, int64_t i) {
+  return f32 ? static_cast<const float*>(p)[i] : static_cast<float>(static_cast<const T*>(p)[i]);
 }
 
 // four fp32 values -> four e4m3 bytes, to nearest even (|v| <= 448 up to rounding; anything not finite -> NaN, 0x7f)
@@ -169,6 +178,20 @@ __device__ __forceinline__ float act_fwd(float z, int act, float slope) {
     }
     case DGCN_ACT_SILU: return EXACT ? z / (1.f + act_exp<EXACT>(-z)) : z * __builtin_amdgcn_rcpf(1.f + act_exp<EXACT>(-z));
     default: return z;
+  }
+}
+
+// a run of values under one (uniform) activation: the branch is outside the run
+template <bool EXACT, int CNT>
+__device__ __forceinline__ void act_run(float (&v)[CNT], int act, float slope) {
+  switch (act) {
+#define DGCN_ACT_CASE(A) case A: { _Pragma("unroll") for (int e = 0; e < CNT; ++e) v[e] = act_fwd<EXACT>(v[e], A, slope); break; }
+    DGCN_ACT_CASE(DGCN_ACT_RELU)
+    DGCN_ACT_CASE(DGCN_ACT_LEAKY_RELU)
+    DGCN_ACT_CASE(DGCN_ACT_GELU)
+    DGCN_ACT_CASE(DGCN_ACT_SILU)
+#undef DGCN_ACT_CASE
+    default: break;
   }
 }
 
