@@ -213,8 +213,10 @@ _SIGNATURES = {
                                   C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]),
     "dgcn_linear_workspace": (C.c_size_t, [C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
     "dgcn_linear_gate_num_partials": (C.c_int32, [C.c_int64, C.c_int32]),
-    "dgcn_linear_gate": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_float, C.c_int32, C.c_void_p, C.c_void_p,
-                                   C.c_int64, C.c_int32, C.c_void_p]),
+    "dgcn_linear_gate": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_float, C.c_int32, C.c_void_p, C.c_int64,
+                                   C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
+    "dgcn_linear_small_rows": (C.c_int32, []),
+    "dgcn_pad_rows": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p]),
     "dgcn_linear_dx": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_int32,
                                  C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]),
     "dgcn_linear_dw": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_int32,

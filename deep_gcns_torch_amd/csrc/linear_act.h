@@ -22,7 +22,7 @@ struct MatParams {
   float* part;
   const void* res;      // [M, N] row stride ldr, or null
   int64_t ldr;
-  void* z;              // [M, N] contiguous, or null
+  void* z;              // [M, N] contiguous, or null: what the backward keeps (fp32: z; 16 bits: gate codes, mlp_common.h)
   void* y;              // [M, N] contiguous
   int64_t M, N, K;
 };
@@ -39,7 +39,13 @@ __device__ __forceinline__ void mat_epilogue(const MatParams& P, int64_t m, int6
 #pragma unroll
     for (int e = 0; e < CNT; ++e) v[e] += b[e];
   }
-  if (P.z) store_run<O, CNT>(static_cast<O*>(P.z) + at, first, N, v);
+  if (P.z) {
+    if constexpr (EXACT) {
+      store_run<O, CNT>(static_cast<O*>(P.z) + at, first, N, v);
+    } else {
+      store_gates<CNT>(static_cast<uint16_t*>(P.z) + at, first, N, v, P.act);
+    }
+  }
   act_run<EXACT, CNT>(v, P.act, P.slope);
   if (P.res) {
     float r[CNT];
@@ -50,10 +56,19 @@ __device__ __forceinline__ void mat_epilogue(const MatParams& P, int64_t m, int6
   store_run<O, CNT>(static_cast<O*>(P.y) + at, first, N, v);
 }
 
-// The tiled product (linear_tile_*.hip), by operand type: 16-byte aligned operands, row strides a multiple of 16 bytes, the
-// contiguous extent of each operand a multiple of 16 bytes.  tile: 0 = 256 x 256, 1 = 128 x 128, 2 = 64 x 128 (K-contiguous A only)
+// The tiled product (linear_tile_*.hip), by operand type.  Operands start on 16 bytes and their row strides are multiples of
+// 16 bytes; where the contiguous extent of an operand is none, the values up to the next one are there, and are zeros along K.
+// tile: 0 = 256 x 256, 1 = 128 x 128, 2 = 64 x 128 (K-contiguous A only)
+int mat_tile_f32(const MatParams& P, int ta, int tb, int tile, hipStream_t s);
 int mat_tile_bf16(const MatParams& P, int ta, int tb, int tile, hipStream_t s);
 int mat_tile_f16(const MatParams& P, int ta, int tb, int tile, hipStream_t s);
 int mat_tile_e4m3(const MatParams& P, int out_type, int tile, hipStream_t s);
+
+// The product of a few K-contiguous rows, M <= kSmallRows (linear_small.h): operands at any byte
+constexpr int kSmallRows = 64;
+int mat_small_f32(const MatParams& P, hipStream_t s);
+int mat_small_bf16(const MatParams& P, hipStream_t s);
+int mat_small_f16(const MatParams& P, hipStream_t s);
+int mat_small_e4m3(const MatParams& P, int out_type, hipStream_t s);
 
 }  // namespace dgcn

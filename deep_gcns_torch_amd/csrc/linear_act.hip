@@ -4,66 +4,13 @@
 //   z = s_x s_w (x w^T) + b        y = act(z) + r              (s_x, s_w: the scales of e4m3 rows, else 1)
 //   dz = g act'(z)     gb = sum over rows of dz     gx = dz w     gw = dz^T x     gr = g
 //
-// Every sum is held in fp32.  z is kept for the backward rounded to the rows' type (half a step of z in act'(z)), and dz
-// is rounded to it before the two products, which take the rows' type on the matrix pipe.
+// Every sum is held in fp32.  For the backward the forward keeps z in fp32, or act'(z) in 16-bit fixed point where the rows
+// have 16 bits (mlp_common.h); dz is rounded to the rows' type before the two products, which take that on the matrix pipe.
 
 #include "linear_act.h"
 
 namespace dgcn {
 namespace {
-
-__device__ __forceinline__ float elem(const uint8_t* p, int64_t i) {
-  return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(p[i]), 0);
-}
-template <class T>
-__device__ __forceinline__ float elem(const T* p, int64_t i) { return static_cast<float>(p[i]); }
-
-// Products whose operands the tiled kernel does not take: 64 x 64 tiles, fp32 operands in LDS, 4 x 4 sums a thread.
-template <class T, class O>
-__global__ __launch_bounds__(256) void mat_simple_kernel(const MatParams P, int ta, int tb) {
-  constexpr int BM = 64, BN = 64, BK = 16;
-  __shared__ float As[BK][BM + 4], Bs[BK][BN + 4];
-  const T* A = static_cast<const T*>(P.a);
-  const T* B = static_cast<const T*>(P.b);
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x) * BM, n0 = static_cast<int64_t>(blockIdx.y) * BN;
-  const int tm = threadIdx.x & 15, tn = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < P.K; k0 += BK) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int idx = threadIdx.x + i * 256;
-      // consecutive threads along the axis that is contiguous
-      const int ka = ta ? idx / BM : idx % BK, ma = ta ? idx % BM : idx / BK;
-      const int kb = tb ? idx / BN : idx % BK, nb = tb ? idx % BN : idx / BK;
-      const int64_t m = m0 + ma, n = n0 + nb;
-      As[ka][ma] = (m < P.M && k0 + ka < P.K) ? elem(A, ta ? (k0 + ka) * P.lda + m : m * P.lda + k0 + ka) : 0.f;
-      Bs[kb][nb] = (n < P.N && k0 + kb < P.K) ? elem(B, tb ? (k0 + kb) * P.ldb + n : n * P.ldb + k0 + kb) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < BK; ++k) {
-      float a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { a[i] = As[k][tm * 4 + i]; b[i] = Bs[k][tn * 4 + i]; }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-      }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + tm * 4 + i, n = n0 + tn * 4;
-    if (m >= P.M || n >= P.N) continue;
-    if (P.a_scale) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] *= P.a_scale[m] * (n + j < P.N ? P.b_scale[n + j] : 0.f);
-    }
-    mat_epilogue<O, 4>(P, m, n, acc[i]);
-  }
-}
 
 // the epilogue of a product whose reduction was split: the partial sums are added in split order
 template <class O>
@@ -88,15 +35,8 @@ __global__ __launch_bounds__(256) void split_join_kernel(const MatParams P) {
   }
 }
 
-template <class T, class O>
-int mat_simple(const MatParams& P, int ta, int tb, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>((P.M + 63) / 64), static_cast<unsigned>((P.N + 63) / 64));
-  hipLaunchKernelGGL((mat_simple_kernel<T, O>), grid, dim3(256), 0, s, P, ta, tb);
-  return launch_status();
-}
-
 struct MatPlan {
-  int tile;             // tile size, or -1: the simple kernel
+  int tile;
   int splits;
 };
 
@@ -104,15 +44,14 @@ struct MatPlan {
 // traffic take (`work`, times the workgroups a CU holds), and at least the latency of the copies behind it; a split
 // writes and reads fp32 partial sums and launches once more.
 inline MatPlan mat_plan(int64_t M, int64_t N, int64_t K, int type, int ta) {
-  if (type == DGCN_T_F32) return {-1, 1};
   struct { int bm, bn, held; double work; } tiles[3] = {{256, 256, 1, 3000.}, {128, 128, 2, 900.}, {64, 128, 3, 600.}};
-  const int64_t steps = (K + (type == DGCN_T_E4M3 ? 127 : 63)) / (type == DGCN_T_E4M3 ? 128 : 64);
+  const int64_t bk = type == DGCN_T_E4M3 ? 128 : type == DGCN_T_F32 ? 32 : 64, steps = (K + bk - 1) / bk;
   const double cus = num_cus();
   MatPlan best = {0, 1};
   double least = 1e300;
   for (int t = 0; t < (ta ? 2 : 3); ++t) {
     const double wgs1 = static_cast<double>((M + tiles[t].bm - 1) / tiles[t].bm) * ((N + tiles[t].bn - 1) / tiles[t].bn);
-    for (int sp = 1; sp <= 64 && sp <= steps; sp *= 2) {
+    for (int sp = 1; sp <= 512 && sp <= steps; sp *= 2) {
       const double wgs = wgs1 * sp, per_cu = ceil(wgs / cus);
       const double held = per_cu < tiles[t].held ? per_cu : tiles[t].held;
       const double step = held * tiles[t].work > 2000. ? held * tiles[t].work : 2000.;
@@ -139,27 +78,26 @@ int split_join(const MatParams& P, hipStream_t s) {
 inline bool aligned16(const void* p, int64_t ld, int es) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * es % 16 == 0; }
 
 int mat_run(MatParams P, int ta, int tb, int in_type, int out_type, void* ws, size_t ws_bytes, hipStream_t s) {
-  MatPlan plan = mat_plan(P.M, P.N, P.K, in_type, ta);
-  const int es = in_type == DGCN_T_E4M3 ? 1 : 2;
-  const int64_t ca = ta ? P.M : P.K, cb = tb ? P.N : P.K;
-  if (!aligned16(P.a, P.lda, es) || !aligned16(P.b, P.ldb, es) || ca * es % 16 || cb * es % 16) plan = {-1, 1};
+  if (ta == 0 && tb == 0 && P.M <= kSmallRows) {
+    switch (in_type) {
+      case DGCN_T_F32: return mat_small_f32(P, s);
+      case DGCN_T_BF16: return mat_small_bf16(P, s);
+      case DGCN_T_F16: return mat_small_f16(P, s);
+      default: return mat_small_e4m3(P, out_type, s);
+    }
+  }
+  const MatPlan plan = mat_plan(P.M, P.N, P.K, in_type, ta);
+  const int es = in_type == DGCN_T_E4M3 ? 1 : in_type == DGCN_T_F32 ? 4 : 2;
+  if (!aligned16(P.a, P.lda, es) || !aligned16(P.b, P.ldb, es)) return DGCN_E_ALIGN;
   if (plan.splits > 1 && (ws_bytes < plan_bytes(plan, P.M, P.N) || !ws)) return DGCN_E_WORKSPACE;
   P.splits = plan.splits;
   P.part = static_cast<float*>(ws);
   int rc = DGCN_E_MODE;
   switch (in_type) {
-    case DGCN_T_F32: return mat_simple<float, float>(P, ta, tb, s);
-    case DGCN_T_BF16: rc = plan.tile < 0 ? mat_simple<__bf16, __bf16>(P, ta, tb, s) : mat_tile_bf16(P, ta, tb, plan.tile, s); break;
-    case DGCN_T_F16: rc = plan.tile < 0 ? mat_simple<_Float16, _Float16>(P, ta, tb, s) : mat_tile_f16(P, ta, tb, plan.tile, s); break;
-    case DGCN_T_E4M3:
-      if (plan.tile >= 0) {
-        rc = mat_tile_e4m3(P, out_type, plan.tile, s);
-      } else {
-        rc = out_type == DGCN_T_F32 ? mat_simple<uint8_t, float>(P, 0, 0, s)
-             : out_type == DGCN_T_BF16 ? mat_simple<uint8_t, __bf16>(P, 0, 0, s)
-             : out_type == DGCN_T_F16 ? mat_simple<uint8_t, _Float16>(P, 0, 0, s) : DGCN_E_MODE;
-      }
-      break;
+    case DGCN_T_F32: rc = mat_tile_f32(P, ta, tb, plan.tile, s); break;
+    case DGCN_T_BF16: rc = mat_tile_bf16(P, ta, tb, plan.tile, s); break;
+    case DGCN_T_F16: rc = mat_tile_f16(P, ta, tb, plan.tile, s); break;
+    case DGCN_T_E4M3: rc = mat_tile_e4m3(P, out_type, plan.tile, s); break;
     default: break;
   }
   if (rc != DGCN_OK || plan.splits == 1) return rc;
@@ -173,8 +111,8 @@ int mat_run(MatParams P, int ta, int tb, int in_type, int out_type, void* ws, si
 // dz = g act'(z), and the column sums of dz over a slab of rows: CL lanes (eight channels each) across, 256 / CL rows at
 // a time; a workgroup takes the rows blockIdx.y * slab .. and leaves one partial sum per channel
 template <class T>
-__global__ __launch_bounds__(256) void gate_kernel(const T* __restrict__ g, int64_t ldg, const T* __restrict__ z, int act,
-                                                   float slope, T* __restrict__ dz, float* __restrict__ part,
+__global__ __launch_bounds__(256) void gate_kernel(const T* __restrict__ g, int64_t ldg, const void* __restrict__ z, int act,
+                                                   float slope, T* __restrict__ dz, int64_t lddz, float* __restrict__ part,
                                                    int64_t rows, int N, int cl, int64_t slab) {
   __shared__ float red[256 * 8];
   const int lane = threadIdx.x % cl, slot = threadIdx.x / cl, slots = 256 / cl;
@@ -186,12 +124,14 @@ __global__ __launch_bounds__(256) void gate_kernel(const T* __restrict__ g, int6
     for (int64_t r = r0 + slot; r < r1; r += slots) {
       float d[8];
       load_chunk(g + r * ldg, at, N, d);
-      if (act != DGCN_ACT_NONE) {
-        float zz[8];
-        load_chunk(z + r * N, at, N, zz);
+      if (dz) {
+        if (act != DGCN_ACT_NONE) {
+          float sl[8];
+          load_slopes<T>(z, r * N, at, N, act, slope, sl);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] *= act_slope<sizeof(T) == 4>(zz[e], act, slope);
-        store_chunk(dz + r * N, at, N, d);
+          for (int e = 0; e < 8; ++e) d[e] *= sl[e];
+        }
+        store_chunk(dz + r * lddz, at, static_cast<int>(lddz), d);     // (d is 0 behind N)
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum[e] += d[e];
@@ -233,6 +173,27 @@ inline GateShape gate_shape(int64_t rows, int N) {
   return S;
 }
 
+// rows of C bytes -> rows of ldo bytes (ldo a multiple of 16, less than 16 more than C), zeros behind; 16 bytes a thread
+__global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* __restrict__ x, int64_t ldx, uint8_t* __restrict__ out,
+                                                       int64_t ldo, int64_t rows, int64_t C) {
+  typedef u4v u4v_any1 __attribute__((aligned(1)));
+  const int64_t per = ldo / 16, total = rows * per;
+  for (int64_t it = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; it < total; it += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t r = it / per, at = (it - r * per) * 16;
+    const uint8_t* p = x + r * ldx + at;
+    u4v v = {0, 0, 0, 0};
+    if (at + 16 <= C) {
+      v = *reinterpret_cast<const u4v_any1*>(p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (at + e < C) v[e >> 2] |= static_cast<uint32_t>(p[e]) << (8 * (e & 3));
+      }
+    }
+    *reinterpret_cast<u4v*>(out + r * ldo + at) = v;
+  }
+}
+
 inline bool known_act(int act) { return act >= DGCN_ACT_NONE && act <= DGCN_ACT_SILU; }
 inline bool sizes_ok(int64_t rows, int32_t K, int32_t N) {
   return rows >= 0 && rows < (int64_t{1} << 36) && K >= 1 && N >= 1 && K <= (1 << 20) && N <= (1 << 20);
@@ -243,10 +204,12 @@ inline bool sizes_ok(int64_t rows, int32_t K, int32_t N) {
 
 using namespace dgcn;
 
+extern "C" int32_t dgcn_linear_small_rows(void) { return kSmallRows; }
+
 extern "C" size_t dgcn_linear_workspace(int32_t product, int64_t rows, int32_t K, int32_t N, int32_t in_type) {
   if (rows <= 0 || K < 1 || N < 1) return 0;
   switch (product) {
-    case 0: return plan_bytes(mat_plan(rows, N, K, in_type, 0), rows, N);
+    case 0: return rows <= kSmallRows ? 0 : plan_bytes(mat_plan(rows, N, K, in_type, 0), rows, N);
     case 1: return plan_bytes(mat_plan(rows, K, N, in_type, 0), rows, K);
     case 2: return plan_bytes(mat_plan(N, K, rows, in_type, 1), N, K);
     default: return 0;
@@ -273,9 +236,9 @@ extern "C" int32_t dgcn_linear_gate_num_partials(int64_t rows, int32_t N) {
 }
 
 extern "C" int dgcn_linear_gate(const void* g, int64_t ldg, const void* z, int32_t act, float slope, int32_t dtype,
-                                void* dz, float* db_part, int64_t rows, int32_t N, void* stream) {
+                                void* dz, int64_t lddz, float* db_part, int64_t rows, int32_t N, void* stream) {
   if (!g || (act != DGCN_ACT_NONE && (!z || !dz))) return DGCN_E_NULL;
-  if (!sizes_ok(rows, 1, N) || ldg < 0) return DGCN_E_SHAPE;
+  if (!sizes_ok(rows, 1, N) || ldg < 0 || (dz && (lddz < N || lddz > (N + 7) / 8 * 8))) return DGCN_E_SHAPE;
   if (!known_act(act)) return DGCN_E_MODE;
   if (rows == 0) return DGCN_OK;
   const GateShape S = gate_shape(rows, N);
@@ -284,15 +247,15 @@ extern "C" int dgcn_linear_gate(const void* g, int64_t ldg, const void* z, int32
   switch (dtype) {
     case DGCN_T_F32:
       hipLaunchKernelGGL(gate_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(g), ldg,
-                         static_cast<const float*>(z), act, slope, static_cast<float*>(dz), db_part, rows, N, S.cl, S.slab);
+                         z, act, slope, static_cast<float*>(dz), lddz, db_part, rows, N, S.cl, S.slab);
       break;
     case DGCN_T_BF16:
       hipLaunchKernelGGL(gate_kernel<__bf16>, grid, dim3(256), 0, s, static_cast<const __bf16*>(g), ldg,
-                         static_cast<const __bf16*>(z), act, slope, static_cast<__bf16*>(dz), db_part, rows, N, S.cl, S.slab);
+                         z, act, slope, static_cast<__bf16*>(dz), lddz, db_part, rows, N, S.cl, S.slab);
       break;
     case DGCN_T_F16:
       hipLaunchKernelGGL(gate_kernel<_Float16>, grid, dim3(256), 0, s, static_cast<const _Float16*>(g), ldg,
-                         static_cast<const _Float16*>(z), act, slope, static_cast<_Float16*>(dz), db_part, rows, N, S.cl, S.slab);
+                         z, act, slope, static_cast<_Float16*>(dz), lddz, db_part, rows, N, S.cl, S.slab);
       break;
     default: return DGCN_E_MODE;
   }
@@ -316,4 +279,16 @@ extern "C" int dgcn_linear_dw(const void* dz, int64_t lddz, const void* x, int64
   if (dtype < DGCN_T_F32 || dtype > DGCN_T_F16) return DGCN_E_MODE;
   const MatParams P = {dz, lddz, x, ldx, nullptr, nullptr, nullptr, 0, DGCN_ACT_NONE, 0.f, 1, nullptr, nullptr, 0, nullptr, dw, N, K, rows};
   return mat_run(P, 1, 1, dtype, dtype, ws, ws_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int dgcn_pad_rows(const void* x, int64_t ldx, void* out, int64_t ldo, int64_t rows, int64_t bytes, void* stream) {
+  if (!x || !out) return DGCN_E_NULL;
+  if (rows < 0 || bytes < 1 || ldx < 0 || ldo != (bytes + 15) / 16 * 16) return DGCN_E_SHAPE;
+  if (reinterpret_cast<uintptr_t>(out) & 15) return DGCN_E_ALIGN;
+  if (rows == 0) return DGCN_OK;
+  int64_t wgs = (rows * (ldo / 16) + 255) / 256;
+  if (wgs > 32 * num_cus()) wgs = 32 * num_cus();
+  hipLaunchKernelGGL(pad_rows_kernel, dim3(static_cast<unsigned>(wgs)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const uint8_t*>(x), ldx, static_cast<uint8_t*>(out), ldo, rows, bytes);
+  return launch_status();
 }

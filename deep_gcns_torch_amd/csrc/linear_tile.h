@@ -4,6 +4,7 @@
 
 #include <type_traits>
 
+#include "bf16x6.h"
 #include "linear_act.h"
 
 namespace dgcn {
@@ -14,51 +15,108 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s4v lds_s4;
 
+// What a wave does with the fragments of one step (128 bytes of the reduction): a raw fragment is two 16-byte units of an
+// operand row; prep() makes of it what the matrix instructions take, mul() adds four channel fragments' products.
 template <class T> struct MatIn;
-template <> struct MatIn<__bf16> {
+
+template <class T>
+struct MatIn16 {
   static constexpr int ES = 2;
-  static __device__ __forceinline__ f32x4 mul(const u4v (&a)[2], const u4v (&b)[2], f32x4 c) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[0]), __builtin_bit_cast(bf16x8, b[0]), c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[1]), __builtin_bit_cast(bf16x8, b[1]), c, 0, 0, 0);
+  struct Frag { u4v r[2]; };
+  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) { return Frag{{r[0], r[1]}}; }
+  static __device__ __forceinline__ f32x4 one(u4v a, u4v b, f32x4 c) {
+    if constexpr (__is_same(T, __bf16)) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+  }
+  static __device__ __forceinline__ void mul(const Frag (&b)[4], const Frag& a, f32x4 (&c)[4]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) c[t] = one(b[t].r[s], a.r[s], c[t]);
+    }
+  }
+  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
+    c = one(b.r[1], a.r[1], one(b.r[0], a.r[0], c));
   }
 };
-template <> struct MatIn<_Float16> {
-  static constexpr int ES = 2;
-  static __device__ __forceinline__ f32x4 mul(const u4v (&a)[2], const u4v (&b)[2], f32x4 c) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[0]), __builtin_bit_cast(f16x8, b[0]), c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[1]), __builtin_bit_cast(f16x8, b[1]), c, 0, 0, 0);
+template <> struct MatIn<__bf16> : MatIn16<__bf16> {};
+template <> struct MatIn<_Float16> : MatIn16<_Float16> {};
+
+// fp32: three bf16 parts that add up to the value bit for bit, and the six products of parts down to 2^-16 of the largest
+// (bf16x6.h: off by at most 3 2^-24 |a b|), at six times the cost of a bf16 product and a sixteenth of an fp32 one's
+template <> struct MatIn<float> {
+  static constexpr int ES = 4;
+  struct Frag { i4v h, m, l; };
+  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) {
+    Frag f;
+    eg_split3(__builtin_bit_cast(f4v, r[0]), __builtin_bit_cast(f4v, r[1]), f.h, f.m, f.l);
+    return f;
+  }
+  static __device__ __forceinline__ void mul(const Frag (&b)[4], const Frag& a, f32x4 (&c)[4]) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].m, a.m, c[t]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].l, a.h, c[t]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].h, a.l, c[t]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].m, a.h, c[t]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].h, a.m, c[t]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].h, a.h, c[t]);
+  }
+  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
+    c = eg_mfma_bf16(b.h, a.l, eg_mfma_bf16(b.l, a.h, eg_mfma_bf16(b.m, a.m, c)));
+    c = eg_mfma_bf16(b.h, a.h, eg_mfma_bf16(b.h, a.m, eg_mfma_bf16(b.m, a.h, c)));
   }
 };
+
 // e4m3 for a 16-bit result: one instruction of K = 128 at twice the 16-bit rate, its block scales held at 2^0.  It aligns
 // the products of eight neighbouring k to the largest one's exponent and drops what lies more than 13 bits below it
 // (measured, bit by bit), so a sum is off by up to 7 2^-13 of the largest product of each eight: 6e-5 of the result's
 // root mean square over normal rows, an order below a bf16 half step and under half of an fp16 one.
 template <> struct MatIn<uint8_t> {
   static constexpr int ES = 1;
-  static __device__ __forceinline__ f32x4 mul(const u4v (&a)[2], const u4v (&b)[2], f32x4 c) {
-    const i8v aa = __builtin_bit_cast(i8v, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
-    const i8v bb = __builtin_bit_cast(i8v, __builtin_shufflevector(b[0], b[1], 0, 1, 2, 3, 4, 5, 6, 7));
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(aa, bb, c, 0, 0, 0, 127, 0, 127);
+  typedef i8v Frag;
+  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) {
+    return __builtin_bit_cast(i8v, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  static __device__ __forceinline__ void mul(const Frag (&b)[4], const Frag& a, f32x4 (&c)[4]) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[t], a, c[t], 0, 0, 0, 127, 0, 127);
+  }
+  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
+    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, 127, 0, 127);
   }
 };
 // e4m3 for an fp32 result: every e4m3 value is an fp16 value; their products are exact and their sum is fp32
 struct WideE4m3 {};
 template <> struct MatIn<WideE4m3> {
   static constexpr int ES = 1;
-  static __device__ __forceinline__ f16x8 widen(uint32_t lo, uint32_t hi) {
-    const u4v r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true))};
-    return __builtin_bit_cast(f16x8, r);
+  struct Frag { u4v r[4]; };
+  static __device__ __forceinline__ u4v widen(uint32_t lo, uint32_t hi) {
+    return u4v{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true))};
   }
-  static __device__ __forceinline__ f32x4 mul(const u4v (&a)[2], const u4v (&b)[2], f32x4 c) {
+  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) {
+    return Frag{{widen(r[0][0], r[0][1]), widen(r[0][2], r[0][3]), widen(r[1][0], r[1][1]), widen(r[1][2], r[1][3])}};
+  }
+  static __device__ __forceinline__ void mul(const Frag (&b)[4], const Frag& a, f32x4 (&c)[4]) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(a[s][0], a[s][1]), widen(b[s][0], b[s][1]), c, 0, 0, 0);
-      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(a[s][2], a[s][3]), widen(b[s][2], b[s][3]), c, 0, 0, 0);
+    for (int s = 0; s < 4; ++s) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) c[t] = MatIn16<_Float16>::one(b[t].r[s], a.r[s], c[t]);
     }
-    return c;
+  }
+  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = MatIn16<_Float16>::one(b.r[s], a.r[s], c);
   }
 };
 
@@ -66,21 +124,20 @@ constexpr unsigned kRsrcFlags = 0x00027000;               // raw 32-bit buffer; 
 constexpr unsigned kBehind = 0x80000000u;                 // an offset behind any buffer here (at most 2^31 bytes)
 
 // Which rows / columns of an operand tile a 16-byte unit of LDS holds.
-//   K-contiguous, R rows of 128 bytes: unit u of row r holds the row's chunk u ^ f(r)
-//     (f = r & 7 for A; for B, whose fragments take rows 16 (i >> 2) + 4 t + (i & 3), f = (r & 3) | bit 4 of r << 2)
-//   K-strided, 64 k-rows of 2 R bytes: unit u of k-row k holds chunk u ^ 2 f(k), f = (k & 3) | bit 3 of k << 2
-// In both, lanes that read together fall on different banks.
-template <int T, int R, bool IS_B>
-__device__ __forceinline__ unsigned tile_offset(int inst, int lane, int64_t ld, int es) {
+//   K-contiguous, R rows of 128 bytes: unit u of row r holds the row's chunk u ^ (r & 7)
+//   K-strided, k-rows of R values: unit u of k-row k holds chunk u ^ 2 ((k & 3) | bit 3 of k << 2) in 16 bits,
+//     u ^ 4 (bits 4, 3 of k) in 32
+// In all, lanes that read together fall on different banks.
+template <int T, int R, int ES>
+__device__ __forceinline__ unsigned tile_offset(int inst, int lane, int64_t ld) {
   if constexpr (T == 0) {
     const int row = inst * 8 + (lane >> 3);
-    const int f = IS_B ? ((row & 3) | ((row >> 4) & 1) << 2) : (row & 7);
-    return static_cast<unsigned>(row * ld * es) + (((lane & 7) ^ f) << 4);
+    return static_cast<unsigned>(row * ld * ES) + (((lane & 7) ^ (row & 7)) << 4);
   } else {
-    constexpr int UNITS = R / 8;
+    constexpr int UNITS = R * ES / 16;
     const int k = inst * (64 / UNITS) + lane / UNITS;
-    const int f = (k & 3) | ((k >> 3) & 1) << 2;
-    return static_cast<unsigned>(k * ld * es) + (((lane % UNITS) ^ (2 * f)) << 4);
+    const int f = ES == 2 ? 2 * ((k & 3) | ((k >> 3) & 1) << 2) : 4 * ((k >> 3) & 3);
+    return static_cast<unsigned>(k * ld * ES) + (((lane % UNITS) ^ f) << 4);
   }
 }
 
@@ -117,14 +174,15 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
 
   unsigned offa[IA], offb[IB];
 #pragma unroll
-  for (int c = 0; c < IA; ++c) offa[c] = tile_offset<TA, BM, false>(wave * IA + c, lane, P.lda, ES);
+  for (int c = 0; c < IA; ++c) offa[c] = tile_offset<TA, BM, ES>(wave * IA + c, lane, P.lda);
 #pragma unroll
-  for (int c = 0; c < IB; ++c) offb[c] = tile_offset<TB, BN, true>(wave * IB + c, lane, P.ldb, ES);
+  for (int c = 0; c < IB; ++c) offb[c] = tile_offset<TB, BN, ES>(wave * IB + c, lane, P.ldb);
   const int64_t rows_a = P.M - m0 < BM ? P.M - m0 : BM, rows_b = P.N - n0 < BN ? P.N - n0 : BN;
 
   // Rows and k-rows behind the matrix lie behind the buffer's end and read as zeros; so do, by an offset of kBehind, the
-  // chunks of a K-contiguous row behind K.  Columns of a K-strided operand behind M or N read what is there: their sums
-  // are not stored.
+  // chunks of a K-contiguous row behind K (a chunk that K ends in is the operand's zero padding from there).  Columns of a
+  // K-strided operand behind M or N read what is there: their sums are not stored.
+  constexpr int CH = 16 / ES;                                           // values in 16 bytes
   auto copy = [&](int step, int buf) {
     const int64_t k0 = static_cast<int64_t>(step) * BK;
     const int64_t left = P.K - k0 < BK ? P.K - k0 : BK;
@@ -132,7 +190,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
     auto one = [&](auto layout, auto count, const void* base, int64_t ld, int64_t line0, int64_t lines, const unsigned* off, char* to) {
       constexpr int L = decltype(layout)::value, n = decltype(count)::value;
       const char* p = static_cast<const char*>(base) + (L == 0 ? line0 * ld + k0 : k0 * ld + line0) * ES;
-      const int64_t bytes = (L == 0 ? (lines - 1) * ld + left : (left - 1) * ld + lines) * ES;
+      const int64_t bytes = (L == 0 ? (lines - 1) * ld + (left + CH - 1) / CH * CH : (left - 1) * ld + (lines + CH - 1) / CH * CH) * ES;
       const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, static_cast<int>(bytes), kRsrcFlags);
       if (L == 0 && left < BK) {
 #pragma unroll
@@ -157,17 +215,18 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
     for (int t = 0; t < 4; ++t) acc[tm][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // fragment: element e of half s is k = 32 s + 8 q + e of operand row i (16-bit types; bytes likewise in e4m3)
-  const int rot = (q ^ (i & 7)) << 4;                                  // half 0; half 1 is the unit 4 further: ^ 64
-  const int kk = i >> 2, pc = i & 3, f2 = (kk | (q & 1) << 2) << 5;     // K-strided: this lane fetches 4 columns of k-row 8 q + kk
+  // Raw fragment of 16 operand rows (or columns), row i on lane (i, q).  One byte a value: chunks q and q + 4 of the row's
+  // eight; two: likewise, k = 8 q .. of each half; four: chunks 2 q and 2 q + 1, k = 8 q .. 8 q + 7.
+  const int at0 = ((ES == 4 ? 2 * q : q) ^ (i & 7)) << 4, at1 = at0 ^ (ES == 4 ? 16 : 64);
+  const int kk = i >> 2, pc = i & 3;                                    // K-strided, 16 bits: the lane fetches four columns of k-row 8 q + kk
+  const int f2 = (kk | (q & 1) << 2) << 5;
   auto read = [&](auto layout, const char* base, int line, int rows, u4v (&out)[2]) {
     constexpr int L = decltype(layout)::value;
     if constexpr (L == 0) {
-      const char* p = base + line * 128;
-      out[0] = *reinterpret_cast<const u4v*>(p + rot);
-      out[1] = *reinterpret_cast<const u4v*>(p + (rot ^ 64));
-    } else {
-      // line: first of 16 columns; a row is rows * 2 bytes; h: k-rows 4 further
+      const char* p = base + (line + i) * 128;
+      out[0] = *reinterpret_cast<const u4v*>(p + at0);
+      out[1] = *reinterpret_cast<const u4v*>(p + at1);
+    } else if constexpr (ES == 2) {
       const char* p = base + (8 * q + kk) * rows * 2 + ((line * 2 + ((pc >> 1) << 4)) ^ f2) + (pc & 1) * 8;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -175,11 +234,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
         const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (32 * s + 4) * rows * 2));
         out[s] = __builtin_bit_cast(u4v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       }
+    } else {
+      const char* p = base + 8 * q * rows * 4 + (((line + i) * 4) ^ (q << 6));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e >> 2][e & 3] = *reinterpret_cast<const uint32_t*>(p + e * rows * 4);
     }
   };
-  // B's fragment t: with K-contiguous rows, matrix row r is channel 16 (r >> 2) + 4 t + (r & 3), so that a lane ends up with
-  // 16 consecutive channels; K-strided, channel 16 t + r
-  const int bline = TB == 0 ? wn * 64 + 16 * (i >> 2) + (i & 3) : wn * 64;
 
   if (s0 < s1) copy(s0, 0);
   for (int step = s0; step < s1; ++step) {
@@ -189,16 +249,18 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
     if (step + 1 < s1) copy(step + 1, buf ^ 1);
     const char* sa = lds + buf * STAGE;
     const char* sb = sa + A_BYTES;
-    u4v fb[4][2];
+    typename MatIn<T>::Frag fb[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) read(std::integral_constant<int, TB>{}, sb, bline + (TB == 0 ? 4 : 16) * t, BN, fb[t]);
+    for (int t = 0; t < 4; ++t) {
+      u4v raw[2];
+      read(std::integral_constant<int, TB>{}, sb, wn * 64 + 16 * t, BN, raw);
+      fb[t] = MatIn<T>::prep(raw);
+    }
 #pragma unroll
     for (int tm = 0; tm < TM; ++tm) {
-      u4v fa[2];
-      const int line = wm * TM * 16 + tm * 16 + (TA == 0 ? i : 0);
-      read(std::integral_constant<int, TA>{}, sa, line, BM, fa);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) acc[tm][t] = MatIn<T>::mul(fb[t], fa, acc[tm][t]);
+      u4v raw[2];
+      read(std::integral_constant<int, TA>{}, sa, wm * TM * 16 + tm * 16, BM, raw);
+      MatIn<T>::mul(fb, MatIn<T>::prep(raw), acc[tm]);
     }
   }
 
@@ -219,8 +281,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
     for (int tm = 0; tm < PASS; ++tm) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int unit = TB == 0 ? 4 * q + t : 4 * t + q;
-        *reinterpret_cast<f32x4*>(mine + (tm * 16 + i) * 256 + ((unit ^ i) << 4)) = acc[p * PASS + tm][t];
+        *reinterpret_cast<f32x4*>(mine + (tm * 16 + i) * 256 + (((4 * t + q) ^ i) << 4)) = acc[p * PASS + tm][t];
       }
     }
 #pragma unroll 1
@@ -253,7 +314,7 @@ int tile_launch(const MatParams& P, hipStream_t s) {
   constexpr int LDS = 2 * (BM + BN) * 128;
   const int64_t tiles = ((P.M + BM - 1) / BM) * ((P.N + BN - 1) / BN);
   // 32-bit offsets inside a tile's lines, 31-bit tile count
-  const int64_t far = MatIn<T>::ES * 256 * (P.lda > P.ldb ? P.lda : P.ldb);
+  const int64_t far = 4 * 256 * (P.lda > P.ldb ? P.lda : P.ldb);
   if (tiles > 0x7fffffff || far + 2 * 128 * 256 > 0x7fffffff || P.splits < 1 || P.splits > 65535) return DGCN_E_SHAPE;
   const void* fn = reinterpret_cast<const void*>(tile_kernel<T, O, TA, TB, TM, WM, WN>);
   const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);

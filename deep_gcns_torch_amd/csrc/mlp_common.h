@@ -213,4 +213,70 @@ __device__ __forceinline__ float act_slope(float z, int act, float slope) {
   }
 }
 
+// ---- what the backward of an activation in 16 bits keeps: act'(z) in fixed point, code = (act' + 1/4) 2^15 ----
+// gelu's and silu's slopes lie in (-0.13, 1.13); they come back within 2^-16, an eighth of a bf16 half step and less of
+// anything that is averaged.  (z in 16 bits would be off by half a step of z in act': measured, 1.5 times the error of the
+// bias gradient.)  relu and leakyrelu keep z > 0 as a slope of 1 or 0.  65535 is NaN.
+constexpr uint32_t kGateNaN = 65535u;
+
+__device__ __forceinline__ uint32_t gate_encode(float z, int act) {
+  float d = z > 0.f ? 1.f : 0.f;
+  if (act == DGCN_ACT_GELU || act == DGCN_ACT_SILU) d = act_slope<false>(z, act, 0.f);
+  const float c = fminf(fmaxf(fmaf(d, 32768.f, 8192.5f), 0.f), 65534.f);
+  return (z != z || d != d) ? kGateNaN : static_cast<uint32_t>(c);
+}
+
+__device__ __forceinline__ float gate_decode(uint32_t code, int act, float slope) {
+  const float d = fmaf(static_cast<float>(code), 1.f / 32768.f, -0.25f);
+  if (code == kGateNaN) return __builtin_nanf("");
+  return act == DGCN_ACT_LEAKY_RELU && code == 8192u ? slope : d;
+}
+
+template <int CNT>
+__device__ __forceinline__ void store_gates(uint16_t* row, int start, int n, const float (&z)[CNT], int act) {
+  uint32_t c[CNT];
+  if (act == DGCN_ACT_GELU) {
+#pragma unroll
+    for (int e = 0; e < CNT; ++e) c[e] = gate_encode(z[e], DGCN_ACT_GELU);
+  } else if (act == DGCN_ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < CNT; ++e) c[e] = gate_encode(z[e], DGCN_ACT_SILU);
+  } else {
+#pragma unroll
+    for (int e = 0; e < CNT; ++e) c[e] = gate_encode(z[e], DGCN_ACT_RELU);
+  }
+  if (start + CNT <= n) {
+    if constexpr (CNT == 8) {
+      *reinterpret_cast<u4v_any2*>(row + start) = u4v{c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16};
+    } else {
+      *reinterpret_cast<u2v_any2*>(row + start) = u2v{c[0] | c[1] << 16, c[2] | c[3] << 16};
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < CNT; ++e) {
+      if (start + e < n) row[start + e] = static_cast<uint16_t>(c[e]);
+    }
+  }
+}
+
+// act'(z) of eight values of a row, from what the forward kept
+template <class T>
+__device__ __forceinline__ void load_slopes(const void* kept, int64_t row_at, int start, int n, int act, float slope, float (&d)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    load_chunk(static_cast<const float*>(kept) + row_at, start, n, d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e] = act_slope<true>(d[e], act, slope);
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(kept) + row_at;
+    if (start + 8 <= n) {
+      const u4v v = *reinterpret_cast<const u4v_any2*>(p + start);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = gate_decode((v[e >> 1] >> (16 * (e & 1))) & 0xffffu, act, slope);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = start + e < n ? gate_decode(p[start + e], act, slope) : 0.f;
+    }
+  }
+}
+
 }  // namespace dgcn

@@ -45,6 +45,16 @@ class RowsE4M3(NamedTuple):
         return (self.data.to(torch.float32) * self.scale.unsqueeze(-1)).to(dtype)
 
 
+# The calls below are made once per layer and token: checks and launches are written to touch each argument once.
+def _device(what: str, *tensors) -> int:
+    """Index of the device that all of the tensors (None apart) are on."""
+    d = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (d < 0 or t.get_device() != d):
+            _lib.require_device(*tensors)        # raises: a CPU tensor, or two devices
+    return d
+
+
 def _row_type(x: torch.Tensor, what: str) -> int:
     t = _TYPES.get(x.dtype)
     if t is None:
@@ -58,20 +68,22 @@ def _rows2d(x: torch.Tensor):
     """``x`` as (rows, C) with unit stride in a row, and its row stride.  Rows that repeat (stride 0) are taken as they are."""
     C = x.size(-1)
     x2 = x if x.dim() == 2 else x.reshape(-1, C)
-    if C > 1 and x2.stride(1) != 1 or x2.stride(0) < 0:
+    ld, inner = x2.stride()
+    if (inner != 1 and C > 1) or ld < 0:
         x2 = x2.contiguous()
-    return x2, x2.stride(0) if x2.size(0) > 1 else C
+        ld = C
+    return x2, ld if x2.size(0) > 1 else C
 
 
-def _param(p, n: int, like: torch.Tensor, what: str):
+def _param(p, n: int, dtype, what: str):
     """A (n,) parameter in the rows' type or fp32 -> (contiguous tensor, is it fp32)."""
     if p is None:
         return None, 0
     if p.dim() != 1 or p.size(0) != n:
         raise ValueError(f"{what} must have shape ({n},), got {tuple(p.shape)}")
-    if p.dtype != like.dtype and p.dtype != torch.float32:
-        raise TypeError(f"{what} must be {like.dtype} or float32, got {p.dtype}")
-    return p.detach().contiguous(), 1 if p.dtype == torch.float32 else 0
+    if p.dtype != dtype and p.dtype != torch.float32:
+        raise TypeError(f"{what} must be {dtype} or float32, got {p.dtype}")
+    return p if p.is_contiguous() else p.detach().contiguous(), 1 if p.dtype == torch.float32 else 0
 
 
 def _same_rows(r, x: torch.Tensor, n: int, dtype, what: str) -> None:
@@ -82,36 +94,59 @@ def _same_rows(r, x: torch.Tensor, n: int, dtype, what: str) -> None:
         raise TypeError(f"{what} must be {dtype}, got {r.dtype}")
 
 
-def _param_sum(parts: torch.Tensor, dtype) -> torch.Tensor:
+def _param_sum(parts: torch.Tensor, dtype, stream: int) -> torch.Tensor:
     out = torch.empty(parts.size(1), device=parts.device, dtype=dtype)
     _lib.check(_lib.load().dgcn_param_sum(parts.data_ptr(), parts.size(0), parts.size(1), _TYPES[dtype], out.data_ptr(),
-                                          _lib.current_stream_handle(parts.device)), "dgcn_param_sum")
+                                          stream), "dgcn_param_sum")
     return out
 
 
+def _needs_grad(*tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _no_grad_only(what, *tensors):
+    if _needs_grad(*tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or on tensors that require none")
+
+
 # ---- root-mean-square norm ------------------------------------------------------------------------------------------
-def _rms_launch(x, weight, eps, residual, e4m3: bool, want_rstd: bool):
-    """-> (y or (q, scale), h or None, rstd or None), contiguous, h and y of x's shape."""
-    lib = _lib.load()
-    dev = _lib.require_device(x, weight, residual)
+def _rms(what, x, weight, eps, residual, e4m3: bool, want_rstd: bool):
+    """Checks and launch -> (y or RowsE4M3, h or None, rstd or None), contiguous, of x's shape."""
+    t = _row_type(x, what)
+    C = x.size(-1)
+    if C > _MAX_NORM_C:
+        raise ValueError(f"{what}: rows of at most {_MAX_NORM_C} channels, got {C}")
+    w, w_f32 = _param(weight, C, x.dtype, "weight")
+    shape = x.shape
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != x.dtype:
+            _same_rows(residual, x, C, x.dtype, "residual")
+    d = _device(what, x, weight, residual)
     x2, ldx = _rows2d(x)
-    r2, ldr = _rows2d(residual) if residual is not None else (None, 0)
-    rows, C = x2.shape
-    w, w_f32 = _param(weight, C, x, "weight")
-    h = torch.empty(x.shape, device=dev, dtype=x.dtype) if residual is not None else None
-    rstd = torch.empty(rows, device=dev, dtype=torch.float32) if want_rstd else None
-    y = q = scale = None
+    rows = x2.size(0)
+    h = rstd = y = q = scale = None
+    r2, ldr = (None, 0) if residual is None else _rows2d(residual)
+    if residual is not None:
+        h = x.new_empty(shape)
+    if want_rstd:
+        rstd = x.new_empty(rows, dtype=torch.float32)
     if e4m3:
-        q = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
-        scale = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32)
+        q = x.new_empty(shape, dtype=torch.float8_e4m3fn)
+        scale = x.new_empty(shape[:-1], dtype=torch.float32)
     else:
-        y = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    if rows == 0:
-        return (RowsE4M3(q, scale) if e4m3 else y), h, rstd
-    with _lib.device_ctx(dev):
-        _lib.check(lib.dgcn_rms_norm_fwd(x2.data_ptr(), ldx, _lib.ptr(r2), ldr, _lib.ptr(w), w_f32, eps, _TYPES[x.dtype],
-                                         _lib.ptr(y), _lib.ptr(h), _lib.ptr(q), _lib.ptr(scale), _lib.ptr(rstd), rows, C,
-                                         _lib.current_stream_handle(dev)), "dgcn_rms_norm_fwd")
+        y = x.new_empty(shape)
+    if rows:
+        ptr = _lib.ptr
+        with _lib.device_ctx(d):
+            rc = _lib.load().dgcn_rms_norm_fwd(x2.data_ptr(), ldx, ptr(r2), ldr, ptr(w), w_f32, eps, t, ptr(y), ptr(h), ptr(q),
+                                               ptr(scale), ptr(rstd), rows, C, _lib.current_stream_handle(d))
+        if rc:
+            _lib.check(rc, "dgcn_rms_norm_fwd")
     return (RowsE4M3(q, scale) if e4m3 else y), h, rstd
 
 
@@ -119,7 +154,7 @@ class _RMSNormRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps: float):
         ctx.set_materialize_grads(False)
-        y, h, rstd = _rms_launch(x, weight, eps, residual, False, True)
+        y, h, rstd = _rms("rms_norm_rows", x, weight, eps, residual, False, True)
         ctx.save_for_backward(x if h is None else h, weight, rstd)
         return y if h is None else (y, h)
 
@@ -134,40 +169,25 @@ class _RMSNormRows(torch.autograd.Function):
             gw = torch.zeros_like(weight) if need_w else None
             return (gh if ctx.needs_input_grad[0] else None), gw, (gh if ctx.needs_input_grad[2] else None), None
         lib = _lib.load()
-        dev = h.device
+        d = h.get_device()
         h2, ldh = _rows2d(h)
         g2, ldg = _rows2d(g)
         gh2, ldgh = _rows2d(gh) if gh is not None else (None, 0)
         rows, C = h2.shape
-        w, w_f32 = _param(weight, C, h, "weight")
-        dx = torch.empty(h.shape, device=dev, dtype=h.dtype) if need_x else None
-        gw = None
-        with _lib.device_ctx(dev):
-            parts = None
+        w, w_f32 = _param(weight, C, h.dtype, "weight")
+        dx = h.new_empty(h.shape) if need_x else None
+        gw = parts = None
+        with _lib.device_ctx(d):
+            stream = _lib.current_stream_handle(d)
             if need_w:
-                parts = torch.empty(lib.dgcn_rms_norm_num_partials(rows, C), C, device=dev, dtype=torch.float32)
+                parts = h.new_empty((lib.dgcn_rms_norm_num_partials(rows, C), C), dtype=torch.float32)
             if need_x or need_w:
                 _lib.check(lib.dgcn_rms_norm_bwd(g2.data_ptr(), ldg, _lib.ptr(gh2), ldgh, h2.data_ptr(), ldh, _lib.ptr(w),
                                                  w_f32, rstd.data_ptr(), _TYPES[h.dtype], _lib.ptr(dx), _lib.ptr(parts),
-                                                 rows, C, _lib.current_stream_handle(dev)), "dgcn_rms_norm_bwd")
+                                                 rows, C, stream), "dgcn_rms_norm_bwd")
             if need_w:
-                gw = _param_sum(parts, weight.dtype)
+                gw = _param_sum(parts, weight.dtype, stream)
         return (dx if ctx.needs_input_grad[0] else None), gw, (dx if ctx.needs_input_grad[2] else None), None
-
-
-def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _rms_checks(what, x, weight, residual):
-    _row_type(x, what)
-    C = x.size(-1)
-    if C > _MAX_NORM_C:
-        raise ValueError(f"{what}: rows of at most {_MAX_NORM_C} channels, got {C}")
-    _param(weight, C, x, "weight")
-    if residual is not None:
-        _same_rows(residual, x, C, x.dtype, "residual")
-    _lib.require_device(x, weight, residual)
 
 
 def rms_norm_rows(x, weight=None, eps: float = 1e-6, residual=None):
@@ -176,24 +196,17 @@ def rms_norm_rows(x, weight=None, eps: float = 1e-6, residual=None):
     Returns ``y``, or ``(y, h)`` with a residual: ``h`` is the stream that the next layer adds to.  ``x`` (..., C) fp32,
     bf16 or fp16, C <= 32768; ``residual`` of the same shape and type; ``weight`` (C,) in the rows' type or fp32.  ``y`` is
     computed from the fp32 sum; its gradient (of x, weight and residual) from the stored ``h``."""
-    _rms_checks("rms_norm_rows", x, weight, residual)
     if _needs_grad(x, weight, residual):
-        return _RMSNormRows.apply(x, weight, residual, float(eps))
-    y, h, _ = _rms_launch(x, weight, float(eps), residual, False, False)
+        return _RMSNormRows.apply(x, weight, residual, eps)
+    y, h, _ = _rms("rms_norm_rows", x, weight, eps, residual, False, False)
     return y if residual is None else (y, h)
-
-
-def _no_grad_only(what, *tensors):
-    if _needs_grad(*tensors):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or on tensors that require none")
 
 
 def rms_norm_rows_e4m3(x, weight=None, eps: float = 1e-6, residual=None):
     """``rms_norm_rows`` whose ``y`` leaves as :class:`RowsE4M3`: ``scale = max|y| / 448`` per row (1 for a row of zeros).
     Returns the rows, or ``(rows, h)`` with a residual.  A NaN or an infinity becomes NaN in its own place.  No gradient."""
-    _rms_checks("rms_norm_rows_e4m3", x, weight, residual)
     _no_grad_only("rms_norm_rows_e4m3", x, weight, residual)
-    y, h, _ = _rms_launch(x, weight, float(eps), residual, True, False)
+    y, h, _ = _rms("rms_norm_rows_e4m3", x, weight, eps, residual, True, False)
     return y if residual is None else (y, h)
 
 
@@ -203,17 +216,18 @@ def quantize_rows(x) -> RowsE4M3:
     t = _row_type(x, "quantize_rows")
     if x.size(-1) > _MAX_NORM_C:
         raise ValueError(f"quantize_rows: rows of at most {_MAX_NORM_C} channels, got {x.size(-1)}")
-    dev = _lib.require_device(x)
+    d = _device("quantize_rows", x)
     _no_grad_only("quantize_rows", x)
     x2, ldx = _rows2d(x)
-    q = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
-    scale = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32)
-    if x.numel() == 0:
-        return RowsE4M3(q, scale)
-    with _lib.device_ctx(dev):
-        _lib.check(_lib.load().dgcn_quantize_rows_e4m3(x2.data_ptr(), ldx, t, q.data_ptr(), scale.data_ptr(), x2.size(0),
-                                                       x2.size(1), _lib.current_stream_handle(dev)),
-                   "dgcn_quantize_rows_e4m3")
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rows, C = x2.shape
+    if rows:
+        with _lib.device_ctx(d):
+            rc = _lib.load().dgcn_quantize_rows_e4m3(x2.data_ptr(), ldx, t, q.data_ptr(), scale.data_ptr(), rows, C,
+                                                     _lib.current_stream_handle(d))
+        if rc:
+            _lib.check(rc, "dgcn_quantize_rows_e4m3")
     return RowsE4M3(q, scale)
 
 
@@ -237,41 +251,75 @@ class RMSNorm(nn.Module):
 
 
 # ---- product with epilogue ------------------------------------------------------------------------------------------
-def _workspace(product: int, rows: int, K: int, N: int, in_type: int, dev):
+_FAR = 1 << 20          # row strides from here on leave the kernels' 32-bit offsets
+_SMALL = None           # rows up to which linear_act takes its operands at any byte (dgcn_linear_small_rows)
+
+
+def _workspace(product: int, rows: int, K: int, N: int, in_type: int, like: torch.Tensor):
     """(workspace or None, its bytes) of one product call: memory of that call alone, also inside a captured graph."""
     n = _lib.load().dgcn_linear_workspace(product, rows, K, N, in_type)
-    return (torch.empty(n, device=dev, dtype=torch.uint8), n) if n else (None, 0)
+    return (like.new_empty(n, dtype=torch.uint8), n) if n else (None, 0)
 
 
-def _linear_launch(x2, ldx, w2, ldw, sx, sw, bias, bias_f32, r2, ldr, act, slope, in_type, out_type, z, y, K, N):
-    dev = y.device
+def _operand(x: torch.Tensor):
+    """A product operand as (rows on 16-byte starts, zeros up to 16 bytes behind each row; row stride in values).  Rows that
+    are so already are taken in place."""
+    x2, ld = _rows2d(x)
+    es = x2.element_size()
+    C = x2.size(1)
+    if x2.data_ptr() % 16 == 0 and ld * es % 16 == 0 and C * es % 16 == 0 and ld <= _FAR:
+        return x2, ld
+    ldo = -(-C * es // 16) * 16
+    out = x2.new_empty((x2.size(0), ldo // es))
+    if x2.size(0):
+        d = x2.get_device()
+        with _lib.device_ctx(d):
+            _lib.check(_lib.load().dgcn_pad_rows(x2.data_ptr(), ld * es, out.data_ptr(), ldo, x2.size(0), C * es,
+                                                 _lib.current_stream_handle(d)), "dgcn_pad_rows")
+    return out, ldo // es
+
+
+def _linear(x, weight, sx, sw, bias, residual, act: int, slope: float, in_type: int, out_dtype, keep: bool):
+    """One launch of checked arguments -> (y, what the backward keeps of the activation or None)."""
+    global _SMALL
+    lib = _lib.load()
+    if _SMALL is None:
+        _SMALL = lib.dgcn_linear_small_rows()
+    N, K = weight.shape
+    lead = x.shape[:-1]
+    y = x.new_empty((*lead, N), dtype=out_dtype)
+    z = y.new_empty(y.shape) if keep and act != 0 else None
     if y.numel() == 0:
-        return
-    ws, ws_bytes = _workspace(0, x2.size(0), K, N, in_type, dev)
-    with _lib.device_ctx(dev):
-        _lib.check(_lib.load().dgcn_linear_act(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _lib.ptr(sx), _lib.ptr(sw),
-                                               _lib.ptr(bias), bias_f32, _lib.ptr(r2), ldr, act, slope, in_type, out_type,
-                                               _lib.ptr(z), y.data_ptr(), x2.size(0), K, N, _lib.ptr(ws), ws_bytes,
-                                               _lib.current_stream_handle(dev)), "dgcn_linear_act")
-
-
-def _linear_forward(x, weight, bias, residual, act, slope, keep_z: bool):
+        return y, z
     x2, ldx = _rows2d(x)
-    w2, ldw = _rows2d(weight)
-    N, K = w2.shape
-    b, b_f32 = _param(bias, N, x, "bias")
-    r2, ldr = _rows2d(residual) if residual is not None else (None, 0)
-    t = _TYPES[x.dtype]
-    y = torch.empty((*x.shape[:-1], N), device=x.device, dtype=x.dtype)
-    z = torch.empty_like(y) if keep_z and act != 0 else None
-    _linear_launch(x2, ldx, w2, ldw, None, None, b, b_f32, r2, ldr, act, slope, t, t, z, y, K, N)
+    rows = x2.size(0)
+    ws, ws_bytes = None, 0
+    if rows <= _SMALL:
+        w2, ldw = _rows2d(weight)
+    else:
+        x2, ldx = _operand(x2)
+        w2, ldw = _operand(weight)
+        ws, ws_bytes = _workspace(0, rows, K, N, in_type, y)
+    r2, ldr = (None, 0) if residual is None else _rows2d(residual)
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.detach().contiguous()
+    ptr = _lib.ptr
+    d = y.get_device()
+    with _lib.device_ctx(d):
+        rc = lib.dgcn_linear_act(x2.data_ptr(), ldx, w2.data_ptr(), ldw, ptr(sx), ptr(sw), ptr(bias),
+                                 1 if bias is not None and bias.dtype == torch.float32 else 0, ptr(r2), ldr, act, slope, in_type,
+                                 _TYPES[out_dtype], ptr(z), y.data_ptr(), rows, K, N, ptr(ws), ws_bytes,
+                                 _lib.current_stream_handle(d))
+    if rc:
+        _lib.check(rc, "dgcn_linear_act")
     return y, z
 
 
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act: int, slope: float):
-        y, z = _linear_forward(x, weight, bias, residual, act, slope, any(ctx.needs_input_grad[:3]))
+        y, z = _linear(x, weight, None, None, bias, residual, act, slope, _TYPES[x.dtype], x.dtype,
+                       any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, weight, z)
         ctx.cfg = (act, slope, None if bias is None else bias.dtype)
         return y
@@ -290,33 +338,36 @@ class _LinearAct(torch.autograd.Function):
         elif need_x or need_w or need_b:
             lib = _lib.load()
             dev, t = x.device, _TYPES[x.dtype]
-            x2, ldx = _rows2d(x)
-            w2, ldw = _rows2d(weight)
+            N, K = weight.shape
             g2, ldg = _rows2d(g)
-            rows, K = x2.shape
-            N = w2.size(0)
+            rows = g2.size(0)
             with _lib.device_ctx(dev):
                 stream = _lib.current_stream_handle(dev)
                 d2, ldd = g2, ldg
                 if act != 0 or need_b:
                     parts = None
                     if act != 0:
-                        d2, ldd = torch.empty(rows, N, device=dev, dtype=x.dtype), N
+                        ldd = -(-N // 8) * 8     # whole 16 bytes: the products below take dz as it is
+                        d2 = torch.empty(rows, ldd, device=dev, dtype=x.dtype)
                     if need_b:
                         parts = torch.empty(lib.dgcn_linear_gate_num_partials(rows, N), N, device=dev, dtype=torch.float32)
                     _lib.check(lib.dgcn_linear_gate(g2.data_ptr(), ldg, _lib.ptr(z), act, slope, t,
-                                                    d2.data_ptr() if act != 0 else None, _lib.ptr(parts), rows, N, stream),
-                               "dgcn_linear_gate")
+                                                    d2.data_ptr() if act != 0 else None, ldd if act != 0 else 0,
+                                                    _lib.ptr(parts), rows, N, stream), "dgcn_linear_gate")
                     if need_b:
-                        gb = _param_sum(parts, bias_type)
+                        gb = _param_sum(parts, bias_type, stream)
+                if act == 0 and (need_x or need_w):
+                    d2, ldd = _operand(g2)
                 if need_x:
+                    w2, ldw = _operand(weight)
                     gx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-                    ws, ws_bytes = _workspace(1, rows, K, N, t, dev)
+                    ws, ws_bytes = _workspace(1, rows, K, N, t, gx)
                     _lib.check(lib.dgcn_linear_dx(d2.data_ptr(), ldd, w2.data_ptr(), ldw, t, gx.data_ptr(), rows, K, N,
                                                   _lib.ptr(ws), ws_bytes, stream), "dgcn_linear_dx")
                 if need_w:
+                    x2, ldx = _operand(x)
                     gw = torch.empty(N, K, device=dev, dtype=weight.dtype)
-                    ws, ws_bytes = _workspace(2, rows, K, N, t, dev)
+                    ws, ws_bytes = _workspace(2, rows, K, N, t, gw)
                     _lib.check(lib.dgcn_linear_dw(d2.data_ptr(), ldd, x2.data_ptr(), ldx, t, gw.data_ptr(), rows, K, N,
                                                   _lib.ptr(ws), ws_bytes, stream), "dgcn_linear_dw")
         return gx, gw, gb, (g if need_r else None), None, None
@@ -329,14 +380,10 @@ def _linear_checks(what, x, weight, bias, residual, act, out_dtype):
     if weight.dim() != 2 or x.dim() < 1 or weight.size(1) != x.size(-1) or weight.size(0) < 1 or weight.size(1) < 1:
         raise ValueError(f"{what}: rows (..., K) and a weight (N, K) with K, N >= 1, got {tuple(x.shape)} and "
                          f"{tuple(weight.shape)}")
-    if max(weight.shape) > _MAX_K:
+    N, K = weight.shape
+    if max(N, K) > _MAX_K:
         raise ValueError(f"{what}: at most {_MAX_K} channels, got {tuple(weight.shape)}")
-    N = weight.size(0)
-    if bias is not None:
-        if bias.dim() != 1 or bias.size(0) != N:
-            raise ValueError(f"bias must have shape ({N},), got {tuple(bias.shape)}")
-        if bias.dtype != out_dtype and bias.dtype != torch.float32:
-            raise TypeError(f"bias must be {out_dtype} or float32, got {bias.dtype}")
+    _param(bias, N, out_dtype, "bias")
     if residual is not None:
         _same_rows(residual, x, N, out_dtype, "residual")
     return code
@@ -347,43 +394,36 @@ def linear_act(x, weight, bias=None, act: str = "none", residual=None, neg_slope
 
     ``x`` (..., K) and ``weight`` (N, K) in one of fp32, bf16, fp16; ``bias`` (N,) in that type or fp32; ``residual``
     (..., N) in that type; ``act`` one of :data:`ACTIVATIONS` (``neg_slope``: of leakyrelu, gelu: ``z Phi(z)``).  Gradients
-    of all four; the pre-activation is kept in the rows' type for them where there is an activation."""
-    _row_type(x, "linear_act")
+    of all four; for them the forward keeps, where there is an activation, one value per result: the pre-activation of fp32
+    rows, the activation's slope in 16-bit fixed point of 16-bit ones."""
+    t = _row_type(x, "linear_act")
     if weight.dtype != x.dtype:
         raise TypeError(f"linear_act: weight must be {x.dtype} as the rows are, got {weight.dtype}")
     code = _linear_checks("linear_act", x, weight, bias, residual, act, x.dtype)
-    _lib.require_device(x, weight, bias, residual)
+    _device("linear_act", x, weight, bias, residual)
     if _needs_grad(x, weight, bias, residual):
-        return _LinearAct.apply(x, weight, bias, residual, code, float(neg_slope))
-    return _linear_forward(x, weight, bias, residual, code, float(neg_slope), False)[0]
+        return _LinearAct.apply(x, weight, bias, residual, code, neg_slope)
+    return _linear(x, weight, None, None, bias, residual, code, neg_slope, t, x.dtype, False)[0]
 
 
 def linear_act_e4m3(x: RowsE4M3, weight: RowsE4M3, bias=None, act: str = "none", residual=None,
                     out_dtype=torch.bfloat16, neg_slope: float = 0.2):
-    """``act((x.data * x.scale) @ (weight.data * weight.scale).T + bias) + residual``: the products of e4m3 values are
-    exact, their sum is fp32, the scales join behind it.  ``x`` rows (..., K), ``weight`` rows (N, K) (``quantize_rows`` of
-    an nn.Linear weight, once); the result, ``residual`` and ``bias`` (or an fp32 bias) in ``out_dtype``.  No gradient."""
+    """``act((x.data * x.scale) @ (weight.data * weight.scale).T + bias) + residual``: ``x`` rows (..., K), ``weight`` rows
+    (N, K) (``quantize_rows`` of an nn.Linear weight, once); the result, ``residual`` and ``bias`` (or an fp32 bias) in
+    ``out_dtype``; the scales join behind the sum.  For an fp32 result the products are summed in fp32; for a 16-bit one on
+    the 8-bit matrix pipe at twice the rate, which cuts products that lie more than 2^13 below the largest of eight
+    neighbouring ones (about 6e-5 of the result's root mean square over normal rows).  No gradient."""
     what = "linear_act_e4m3"
-    t = _TYPES.get(out_dtype)
-    if t is None:
+    if out_dtype not in _TYPES:
         raise TypeError(f"{what}: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
-    for name, r in (("x", x), ("weight", weight)):
-        if r.data.dtype != torch.float8_e4m3fn or r.scale.dtype != torch.float32:
-            raise TypeError(f"{what}: {name} must be float8_e4m3fn rows with float32 scales, got {r.data.dtype} and "
-                            f"{r.scale.dtype}")
-        if r.scale.shape != r.data.shape[:-1]:
-            raise ValueError(f"{what}: {name} of shape {tuple(r.data.shape)} needs scales of shape "
-                             f"{tuple(r.data.shape[:-1])}, got {tuple(r.scale.shape)}")
-    code = _linear_checks(what, x.data, weight.data, bias, residual, act, out_dtype)
-    dev = _lib.require_device(x.data, x.scale, weight.data, weight.scale, bias, residual)
-    _no_grad_only(what, bias, residual, x.scale, weight.scale)
-    x2, ldx = _rows2d(x.data)
-    w2, ldw = _rows2d(weight.data)
-    N, K = w2.shape
-    b = None if bias is None else bias.contiguous()
-    r2, ldr = _rows2d(residual) if residual is not None else (None, 0)
-    y = torch.empty((*x.data.shape[:-1], N), device=dev, dtype=out_dtype)
-    _linear_launch(x2, ldx, w2, ldw, x.scale.contiguous(), weight.scale.contiguous(), b,
-                   1 if b is not None and b.dtype == torch.float32 else 0, r2, ldr, code, float(neg_slope), _E4M3, t, None, y,
-                   K, N)
-    return y
+    (xd, sx), (wd, sw) = x, weight
+    for name, r, s in (("x", xd, sx), ("weight", wd, sw)):
+        if r.dtype != torch.float8_e4m3fn or s.dtype != torch.float32:
+            raise TypeError(f"{what}: {name} must be float8_e4m3fn rows with float32 scales, got {r.dtype} and {s.dtype}")
+        if s.shape != r.shape[:-1]:
+            raise ValueError(f"{what}: {name} of shape {tuple(r.shape)} needs scales of shape {tuple(r.shape[:-1])}, got "
+                             f"{tuple(s.shape)}")
+    code = _linear_checks(what, xd, wd, bias, residual, act, out_dtype)
+    _device(what, xd, sx, wd, sw, bias, residual)
+    _no_grad_only(what, bias, residual, sx, sw)
+    return _linear(xd, wd, sx.contiguous(), sw.contiguous(), bias, residual, code, neg_slope, _E4M3, out_dtype, False)[0]

@@ -745,13 +745,20 @@ int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width, int32_t dt
  *   x (rows, K) row stride ldx, w (N, K) row stride ldw, both in in_type; K, N <= 2^20
  *   in_type DGCN_T_E4M3: x_scale (rows) and w_scale (N) are required and out_type is free; otherwise out_type = in_type
  *   bias (N) in out_type or, with bias_f32, fp32, or NULL; res (rows, N) out_type, row stride ldr, or NULL
- *   z (rows, N) out_type contiguous, or NULL: kept for dgcn_linear_gate; y (rows, N) out_type contiguous
+ *   z (rows, N) contiguous, or NULL: kept for dgcn_linear_gate -- z in fp32, or in the 16-bit types act'(z) in 16-bit fixed
+ *     point (code 2^-15 - 1/4; 65535 is NaN; relu and leakyrelu: z > 0 as 1 or 0); y (rows, N) out_type contiguous
  * Backward, all in one dtype:
- *   dgcn_linear_gate: dz = g act'(z) contiguous (neither z nor dz with DGCN_ACT_NONE: dz is g), and db_part
+ *   dgcn_linear_gate: dz = g act'(z), row stride lddz, N <= lddz <= N rounded up to 8, zeros behind N (dz may be NULL with
+ *     DGCN_ACT_NONE: dz is g), and db_part
  *     [dgcn_linear_gate_num_partials(rows, N)][N], whose sum is the bias gradient, or NULL
  *   dgcn_linear_dx: dx (rows, K) = dz w        dgcn_linear_dw: dw (N, K) = dz^T x
+ * Operands of the three products (x, w, dz; not those of dgcn_linear_act with at most dgcn_linear_small_rows() rows) start on 16 bytes and their row strides are multiples of 16 bytes (DGCN_E_ALIGN
+ *   otherwise); where a row's K or N values are not, the values up to the next 16 bytes are there and are zeros:
+ *   dgcn_pad_rows copies rows of `bytes` bytes, row stride ldx bytes, to such rows of ldo = bytes rounded up to 16.
  * ws: dgcn_linear_workspace(product, rows, K, N, in_type) bytes, 16-byte aligned, of this call's own (fp32 partial sums of a
  *   split reduction; may be 0 and NULL); product 0: dgcn_linear_act, 1: dgcn_linear_dx, 2: dgcn_linear_dw. */
+int32_t dgcn_linear_small_rows(void);
+int dgcn_pad_rows(const void* x, int64_t ldx, void* out, int64_t ldo, int64_t rows, int64_t bytes, void* stream);
 size_t dgcn_linear_workspace(int32_t product, int64_t rows, int32_t K, int32_t N, int32_t in_type);
 int dgcn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* x_scale, const float* w_scale,
                     const void* bias, int32_t bias_f32, const void* res, int64_t ldr, int32_t act, float slope,
@@ -759,7 +766,7 @@ int dgcn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
                     size_t ws_bytes, void* stream);
 int32_t dgcn_linear_gate_num_partials(int64_t rows, int32_t N);
 int dgcn_linear_gate(const void* g, int64_t ldg, const void* z, int32_t act, float slope, int32_t dtype, void* dz,
-                     float* db_part, int64_t rows, int32_t N, void* stream);
+                     int64_t lddz, float* db_part, int64_t rows, int32_t N, void* stream);
 int dgcn_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, int32_t dtype, void* dx, int64_t rows,
                    int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream);
 int dgcn_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, int32_t dtype, void* dw, int64_t rows,

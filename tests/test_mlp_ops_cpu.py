@@ -67,8 +67,19 @@ def test_c_entry_argument_errors_do_not_launch():
     assert lib.dgcn_param_sum(None, 1, 4, 0, p, None) == -1
     assert lib.dgcn_rms_norm_num_partials(0, 8) == 0 and lib.dgcn_linear_gate_num_partials(0, 8) == 0
     gate = lib.dgcn_linear_gate
-    assert gate(p, 8, None, 1, 0.2, 0, p, None, 1, 8, None) == -1                              # an activation needs z
-    assert gate(p, 8, p, 9, 0.2, 0, p, None, 1, 8, None) == -4
+    assert gate(p, 8, None, 1, 0.2, 0, p, 8, None, 1, 8, None) == -1                              # an activation needs z
+    assert gate(p, 8, p, 9, 0.2, 0, p, 8, None, 1, 8, None) == -4
+    assert gate(p, 8, p, 1, 0.2, 0, p, 7, None, 1, 8, None) == -2 and gate(p, 8, p, 1, 0.2, 0, p, 16, None, 1, 8, None) == -2
+    act = lib.dgcn_linear_act
+    assert act(p, 8, p, 8, None, None, None, 0, None, 0, 0, 0.0, 3, 1, None, p, 1, 8, 8, None, 0, None) == -1   # e4m3 without scales
+    assert act(p, 8, p, 8, None, None, None, 0, None, 0, 0, 0.0, 1, 2, None, p, 1, 8, 8, None, 0, None) == -4   # bf16 rows, fp16 result
+    assert act(p, 8, p, 8, None, None, None, 0, None, 0, 9, 0.0, 1, 1, None, p, 1, 8, 8, None, 0, None) == -4   # no such activation
+    assert act(p + 2, 8, p, 8, None, None, None, 0, None, 0, 0, 0.0, 1, 1, None, p, 99, 8, 8, None, 0, None) == -3
+    assert act(p, 9, p, 8, None, None, None, 0, None, 0, 0, 0.0, 1, 1, None, p, 99, 8, 8, None, 0, None) == -3
+    n = lib.dgcn_linear_workspace(2, 100000, 64, 64, 1)
+    assert n > 0 and lib.dgcn_linear_dw(p, 64, p, 64, 1, p, 100000, 64, 64, p, n - 1, None) == -5               # workspace too small
+    assert lib.dgcn_linear_dw(p, 64, p, 64, 1, p, 0, 64, 64, None, 0, None) == -2                               # a sum over no rows is the caller's
+    assert lib.dgcn_pad_rows(p, 5, p, 32, 1, 5, None) == -2 and lib.dgcn_pad_rows(p, 5, p + 4, 16, 1, 5, None) == -3
 
 
 def test_norm_layer_offers_rms():

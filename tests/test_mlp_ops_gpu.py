@@ -218,7 +218,9 @@ LINEAR_SHAPES = [(1, 8, 8), (1, 1, 1), (1, 4096, 512), (2, 17, 5), (16, 256, 409
                  (65, 1000, 72), (128, 128, 128), (100, 2048, 40), (257, 520, 264), (300, 96, 1025), (1500, 112, 224),
                  (5000, 128, 256), (1025, 13, 7), (0, 16, 24),
                  # whole and ragged tiles of each size, long and split reductions
-                 (4096, 72, 4104), (2049, 1096, 2056), (60, 8192, 512), (700, 4096, 264), (129, 6152, 136), (9000, 264, 520)]
+                 (4096, 72, 4104), (2049, 1096, 2056), (60, 8192, 512), (700, 4096, 264), (129, 6152, 136), (9000, 264, 520),
+                 # few rows: one to four tiles of 16, rows that end inside a step, channels that end inside 16
+                 (15, 4095, 33), (32, 1030, 100), (47, 777, 1000), (64, 2048, 130), (5, 70, 4100)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
