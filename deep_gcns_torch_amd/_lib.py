@@ -204,23 +204,21 @@ _SIGNATURES = {
                                     C.c_void_p]),
     "dgcn_rms_norm_num_partials": (C.c_int32, [C.c_int64, C.c_int32]),
     "dgcn_rms_norm_bwd": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32,
-                                    C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
+                                    C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
+                                    C.c_void_p]),
     "dgcn_quantize_rows_e4m3": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
                                           C.c_void_p]),
     "dgcn_param_sum": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]),
     "dgcn_linear_act": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                                   C.c_void_p, C.c_int64, C.c_int32, C.c_float, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
                                   C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]),
-    "dgcn_linear_workspace": (C.c_size_t, [C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
-    "dgcn_linear_gate_num_partials": (C.c_int32, [C.c_int64, C.c_int32]),
-    "dgcn_linear_gate": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_float, C.c_int32, C.c_void_p, C.c_int64,
-                                   C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
-    "dgcn_linear_small_rows": (C.c_int32, []),
-    "dgcn_pad_rows": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p]),
-    "dgcn_linear_dx": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_int32,
-                                 C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]),
-    "dgcn_linear_dw": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_int32,
-                                 C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "dgcn_linear_workspace": (C.c_size_t, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_int64, C.c_int32,
+                                           C.c_int32]),
+    "dgcn_linear_bwd_workspace": (C.c_size_t, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32,
+                                               C.c_int32, C.c_int32, C.c_int64, C.c_int32, C.c_int32]),
+    "dgcn_linear_bwd": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32,
+                                  C.c_float, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32,
+                                  C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]),
 }
 
 _lib = None

@@ -63,49 +63,12 @@ inline MatPlan mat_plan(int64_t M, int64_t N, int64_t K, int type, int ta) {
   return best;
 }
 
-inline size_t plan_bytes(const MatPlan& p, int64_t M, int64_t N) {
-  return p.splits > 1 ? static_cast<size_t>(p.splits) * M * N * sizeof(float) : 0;
-}
-
 template <class O>
 int split_join(const MatParams& P, hipStream_t s) {
   int64_t wgs = (P.M * ((P.N + 3) / 4) + 255) / 256;
   if (wgs > 16 * num_cus()) wgs = 16 * num_cus();
   hipLaunchKernelGGL((split_join_kernel<O>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, P);
   return launch_status();
-}
-
-inline bool aligned16(const void* p, int64_t ld, int es) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * es % 16 == 0; }
-
-int mat_run(MatParams P, int ta, int tb, int in_type, int out_type, void* ws, size_t ws_bytes, hipStream_t s) {
-  if (ta == 0 && tb == 0 && P.M <= kSmallRows) {
-    switch (in_type) {
-      case DGCN_T_F32: return mat_small_f32(P, s);
-      case DGCN_T_BF16: return mat_small_bf16(P, s);
-      case DGCN_T_F16: return mat_small_f16(P, s);
-      default: return mat_small_e4m3(P, out_type, s);
-    }
-  }
-  const MatPlan plan = mat_plan(P.M, P.N, P.K, in_type, ta);
-  const int es = in_type == DGCN_T_E4M3 ? 1 : in_type == DGCN_T_F32 ? 4 : 2;
-  if (!aligned16(P.a, P.lda, es) || !aligned16(P.b, P.ldb, es)) return DGCN_E_ALIGN;
-  if (plan.splits > 1 && (ws_bytes < plan_bytes(plan, P.M, P.N) || !ws)) return DGCN_E_WORKSPACE;
-  P.splits = plan.splits;
-  P.part = static_cast<float*>(ws);
-  int rc = DGCN_E_MODE;
-  switch (in_type) {
-    case DGCN_T_F32: rc = mat_tile_f32(P, ta, tb, plan.tile, s); break;
-    case DGCN_T_BF16: rc = mat_tile_bf16(P, ta, tb, plan.tile, s); break;
-    case DGCN_T_F16: rc = mat_tile_f16(P, ta, tb, plan.tile, s); break;
-    case DGCN_T_E4M3: rc = mat_tile_e4m3(P, out_type, plan.tile, s); break;
-    default: break;
-  }
-  if (rc != DGCN_OK || plan.splits == 1) return rc;
-  switch (out_type) {
-    case DGCN_T_F32: return split_join<float>(P, s);
-    case DGCN_T_BF16: return split_join<__bf16>(P, s);
-    default: return split_join<_Float16>(P, s);
-  }
 }
 
 // dz = g act'(z), and the column sums of dz over a slab of rows: CL lanes (eight channels each) across, 256 / CL rows at
@@ -199,21 +162,177 @@ inline bool sizes_ok(int64_t rows, int32_t K, int32_t N) {
   return rows >= 0 && rows < (int64_t{1} << 36) && K >= 1 && N >= 1 && K <= (1 << 20) && N <= (1 << 20);
 }
 
+inline int type_bytes(int type) { return type == DGCN_T_F32 ? 4 : type == DGCN_T_E4M3 ? 1 : 2; }
+inline int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+// Memory of one call, handed out front to back in 256-byte steps (base null: only counted)
+struct Arena {
+  char* base;
+  size_t used, size;
+  void* take(size_t bytes) {
+    char* p = base ? base + used : nullptr;
+    used += (bytes + 255) / 256 * 256;
+    return p;
+  }
+  bool full() const { return used > size; }
+};
+
+// An operand as the tiled kernel takes it: 16-byte starts and strides, nothing but the row in its last 16 bytes
+struct Operand {
+  const void* p;
+  int64_t ld;
+};
+
+constexpr int64_t kFarStride = int64_t{1} << 20;           // strides from here on leave the tile's 32-bit offsets
+
+inline bool operand_ready(const void* p, int64_t ld, int64_t C, int es) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * es % 16 == 0 && C * es % 16 == 0 && ld <= kFarStride;
+}
+
+int operand(const void* p, int64_t ld, int64_t rows, int64_t C, int es, Arena& ws, bool launch, hipStream_t s, Operand* out) {
+  *out = {p, ld};
+  if (operand_ready(p, ld, C, es)) return DGCN_OK;
+  const int64_t ldo = round16(C * es);
+  uint8_t* to = static_cast<uint8_t*>(ws.take(rows * ldo));
+  *out = {to, ldo / es};
+  if (!launch) return DGCN_OK;
+  if (ws.full()) return DGCN_E_WORKSPACE;
+  int64_t wgs = (rows * (ldo / 16) + 255) / 256;
+  if (wgs > 32 * num_cus()) wgs = 32 * num_cus();
+  hipLaunchKernelGGL(pad_rows_kernel, dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, static_cast<const uint8_t*>(p), ld * es,
+                     to, ldo, rows, C * es);
+  return launch_status();
+}
+
+// One product; launch false: only its workspace is counted
+int mat_run(MatParams P, int ta, int tb, int in_type, int out_type, Arena& ws, bool launch, hipStream_t s) {
+  const MatPlan plan = mat_plan(P.M, P.N, P.K, in_type, ta);
+  P.splits = plan.splits;
+  if (plan.splits > 1) P.part = static_cast<float*>(ws.take(static_cast<size_t>(plan.splits) * P.M * P.N * sizeof(float)));
+  if (!launch) return DGCN_OK;
+  if (ws.full()) return DGCN_E_WORKSPACE;
+  int rc = DGCN_E_MODE;
+  switch (in_type) {
+    case DGCN_T_F32: rc = mat_tile_f32(P, ta, tb, plan.tile, s); break;
+    case DGCN_T_BF16: rc = mat_tile_bf16(P, ta, tb, plan.tile, s); break;
+    case DGCN_T_F16: rc = mat_tile_f16(P, ta, tb, plan.tile, s); break;
+    case DGCN_T_E4M3: rc = mat_tile_e4m3(P, out_type, plan.tile, s); break;
+    default: break;
+  }
+  if (rc != DGCN_OK || plan.splits == 1) return rc;
+  switch (out_type) {
+    case DGCN_T_F32: return split_join<float>(P, s);
+    case DGCN_T_BF16: return split_join<__bf16>(P, s);
+    default: return split_join<_Float16>(P, s);
+  }
+}
+
+int small_run(const MatParams& P, int in_type, int out_type, hipStream_t s) {
+  switch (in_type) {
+    case DGCN_T_F32: return mat_small_f32(P, s);
+    case DGCN_T_BF16: return mat_small_bf16(P, s);
+    case DGCN_T_F16: return mat_small_f16(P, s);
+    default: return mat_small_e4m3(P, out_type, s);
+  }
+}
+
+int linear_forward(MatParams P, int in_type, int out_type, Arena& ws, bool launch, hipStream_t s) {
+  if (P.M <= kSmallRows) return launch ? small_run(P, in_type, out_type, s) : DGCN_OK;
+  const int es = type_bytes(in_type);
+  Operand a, b;
+  int rc = operand(P.a, P.lda, P.M, P.K, es, ws, launch, s, &a);
+  if (rc == DGCN_OK) rc = operand(P.b, P.ldb, P.N, P.K, es, ws, launch, s, &b);
+  if (rc != DGCN_OK) return rc;
+  P.a = a.p; P.lda = a.ld; P.b = b.p; P.ldb = b.ld;
+  return mat_run(P, 0, 0, in_type, out_type, ws, launch, s);
+}
+
+struct BwdArgs {
+  const void* g;
+  int64_t ldg;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const void* z;
+  int act;
+  float slope;
+  int type;
+  void *dx, *dw, *db;
+  int db_f32;
+  int64_t rows;
+  int K, N;
+};
+
+inline MatParams plain_product(Operand a, Operand b, void* y, int64_t M, int64_t N, int64_t K) {
+  MatParams P = {};
+  P.a = a.p; P.lda = a.ld; P.b = b.p; P.ldb = b.ld;
+  P.act = DGCN_ACT_NONE; P.splits = 1; P.y = y; P.M = M; P.N = N; P.K = K;
+  return P;
+}
+
+template <class T>
+int gate_launch(const BwdArgs& A, const GateShape& S, void* dz, int64_t lddz, float* part, hipStream_t s) {
+  hipLaunchKernelGGL(gate_kernel<T>, dim3(S.gx, S.gy), dim3(256), 0, s, static_cast<const T*>(A.g), A.ldg, A.z, A.act, A.slope,
+                     static_cast<T*>(dz), lddz, part, A.rows, A.N, S.cl, S.slab);
+  return launch_status();
+}
+
+int linear_backward(const BwdArgs& A, Arena& ws, bool launch, hipStream_t s) {
+  const int es = type_bytes(A.type);
+  Operand dz = {A.g, A.ldg};
+  const bool products = A.dx || A.dw;
+  int rc = DGCN_OK;
+  if (A.act != DGCN_ACT_NONE || A.db) {
+    const GateShape S = gate_shape(A.rows, A.N);
+    void* to = nullptr;
+    if (A.act != DGCN_ACT_NONE || (products && !operand_ready(A.g, A.ldg, A.N, es))) {
+      const int64_t ld = round16(static_cast<int64_t>(A.N) * es) / es;
+      to = ws.take(A.rows * ld * es);
+      dz = {to, ld};
+    }
+    float* part = A.db ? static_cast<float*>(ws.take(static_cast<size_t>(S.gy) * A.N * sizeof(float))) : nullptr;
+    if (launch) {
+      if (ws.full()) return DGCN_E_WORKSPACE;
+      switch (A.type) {
+        case DGCN_T_F32: rc = gate_launch<float>(A, S, to, dz.ld, part, s); break;
+        case DGCN_T_BF16: rc = gate_launch<__bf16>(A, S, to, dz.ld, part, s); break;
+        default: rc = gate_launch<_Float16>(A, S, to, dz.ld, part, s); break;
+      }
+      if (rc == DGCN_OK && A.db) rc = dgcn_param_sum(part, S.gy, A.N, A.db_f32 ? DGCN_T_F32 : A.type, A.db, s);
+      if (rc != DGCN_OK) return rc;
+    }
+  } else if (products) {
+    rc = operand(A.g, A.ldg, A.rows, A.N, es, ws, launch, s, &dz);
+    if (rc != DGCN_OK) return rc;
+  }
+  if (A.dx) {
+    Operand w;
+    rc = operand(A.w, A.ldw, A.N, A.K, es, ws, launch, s, &w);
+    if (rc == DGCN_OK) rc = mat_run(plain_product(dz, w, A.dx, A.rows, A.K, A.N), 0, 1, A.type, A.type, ws, launch, s);
+    if (rc != DGCN_OK) return rc;
+  }
+  if (A.dw) {
+    Operand x;
+    rc = operand(A.x, A.ldx, A.rows, A.K, es, ws, launch, s, &x);
+    if (rc == DGCN_OK) rc = mat_run(plain_product(dz, x, A.dw, A.N, A.K, A.rows), 1, 1, A.type, A.type, ws, launch, s);
+  }
+  return rc;
+}
+
 }  // namespace
 }  // namespace dgcn
 
 using namespace dgcn;
 
-extern "C" int32_t dgcn_linear_small_rows(void) { return kSmallRows; }
-
-extern "C" size_t dgcn_linear_workspace(int32_t product, int64_t rows, int32_t K, int32_t N, int32_t in_type) {
-  if (rows <= 0 || K < 1 || N < 1) return 0;
-  switch (product) {
-    case 0: return rows <= kSmallRows ? 0 : plan_bytes(mat_plan(rows, N, K, in_type, 0), rows, N);
-    case 1: return plan_bytes(mat_plan(rows, K, N, in_type, 0), rows, K);
-    case 2: return plan_bytes(mat_plan(N, K, rows, in_type, 1), N, K);
-    default: return 0;
-  }
+extern "C" size_t dgcn_linear_workspace(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t in_type, int64_t rows,
+                                        int32_t K, int32_t N) {
+  if (!sizes_ok(rows, K, N) || rows == 0 || in_type < DGCN_T_F32 || in_type > DGCN_T_E4M3) return 0;
+  MatParams P = {};
+  P.a = x; P.lda = ldx; P.b = w; P.ldb = ldw; P.M = rows; P.N = N; P.K = K;
+  Arena ws = {nullptr, 0, 0};
+  linear_forward(P, in_type, in_type, ws, false, nullptr);
+  return ws.used;
 }
 
 extern "C" int dgcn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* x_scale,
@@ -223,72 +342,35 @@ extern "C" int dgcn_linear_act(const void* x, int64_t ldx, const void* w, int64_
   if (!x || !w || !y || (in_type == DGCN_T_E4M3 && (!x_scale || !w_scale))) return DGCN_E_NULL;
   if (!sizes_ok(rows, K, N) || ldx < 0 || ldw < 0 || (res && ldr < 0)) return DGCN_E_SHAPE;
   if (!known_act(act) || out_type < DGCN_T_F32 || out_type > DGCN_T_F16 || (in_type != DGCN_T_E4M3 && in_type != out_type)) return DGCN_E_MODE;
+  if (reinterpret_cast<uintptr_t>(ws) & 15) return DGCN_E_ALIGN;
   if (rows == 0) return DGCN_OK;
   const bool scaled = in_type == DGCN_T_E4M3;
   const MatParams P = {x, ldx, w, ldw, scaled ? x_scale : nullptr, scaled ? w_scale : nullptr, bias, bias_f32, act, slope, 1,
                        nullptr, res, ldr, z, y, rows, N, K};
-  return mat_run(P, 0, 0, in_type, out_type, ws, ws_bytes, static_cast<hipStream_t>(stream));
+  Arena arena = {static_cast<char*>(ws), 0, ws ? ws_bytes : 0};
+  return linear_forward(P, in_type, out_type, arena, true, static_cast<hipStream_t>(stream));
 }
 
-extern "C" int32_t dgcn_linear_gate_num_partials(int64_t rows, int32_t N) {
-  if (rows <= 0 || N < 1) return 0;
-  return static_cast<int32_t>(gate_shape(rows, N).gy);
+extern "C" size_t dgcn_linear_bwd_workspace(const void* g, int64_t ldg, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                            int32_t act, int32_t dtype, int32_t want, int64_t rows, int32_t K, int32_t N) {
+  if (!sizes_ok(rows, K, N) || rows == 0 || dtype < DGCN_T_F32 || dtype > DGCN_T_F16) return 0;
+  char any;
+  const BwdArgs A = {g, ldg, x, ldx, w, ldw, nullptr, act, 0.f, dtype, want & 1 ? &any : nullptr, want & 2 ? &any : nullptr,
+                     want & 4 ? &any : nullptr, 0, rows, K, N};
+  Arena ws = {nullptr, 0, 0};
+  linear_backward(A, ws, false, nullptr);
+  return ws.used;
 }
 
-extern "C" int dgcn_linear_gate(const void* g, int64_t ldg, const void* z, int32_t act, float slope, int32_t dtype,
-                                void* dz, int64_t lddz, float* db_part, int64_t rows, int32_t N, void* stream) {
-  if (!g || (act != DGCN_ACT_NONE && (!z || !dz))) return DGCN_E_NULL;
-  if (!sizes_ok(rows, 1, N) || ldg < 0 || (dz && (lddz < N || lddz > (N + 7) / 8 * 8))) return DGCN_E_SHAPE;
-  if (!known_act(act)) return DGCN_E_MODE;
-  if (rows == 0) return DGCN_OK;
-  const GateShape S = gate_shape(rows, N);
-  const dim3 grid(S.gx, S.gy);
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case DGCN_T_F32:
-      hipLaunchKernelGGL(gate_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(g), ldg,
-                         z, act, slope, static_cast<float*>(dz), lddz, db_part, rows, N, S.cl, S.slab);
-      break;
-    case DGCN_T_BF16:
-      hipLaunchKernelGGL(gate_kernel<__bf16>, grid, dim3(256), 0, s, static_cast<const __bf16*>(g), ldg,
-                         z, act, slope, static_cast<__bf16*>(dz), lddz, db_part, rows, N, S.cl, S.slab);
-      break;
-    case DGCN_T_F16:
-      hipLaunchKernelGGL(gate_kernel<_Float16>, grid, dim3(256), 0, s, static_cast<const _Float16*>(g), ldg,
-                         z, act, slope, static_cast<_Float16*>(dz), lddz, db_part, rows, N, S.cl, S.slab);
-      break;
-    default: return DGCN_E_MODE;
-  }
-  return launch_status();
-}
-
-extern "C" int dgcn_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, int32_t dtype, void* dx,
-                              int64_t rows, int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream) {
-  if (!dz || !w || !dx) return DGCN_E_NULL;
-  if (!sizes_ok(rows, K, N) || lddz < 0 || ldw < 0) return DGCN_E_SHAPE;
-  if (dtype < DGCN_T_F32 || dtype > DGCN_T_F16) return DGCN_E_MODE;
-  if (rows == 0) return DGCN_OK;
-  const MatParams P = {dz, lddz, w, ldw, nullptr, nullptr, nullptr, 0, DGCN_ACT_NONE, 0.f, 1, nullptr, nullptr, 0, nullptr, dx, rows, K, N};
-  return mat_run(P, 0, 1, dtype, dtype, ws, ws_bytes, static_cast<hipStream_t>(stream));
-}
-
-extern "C" int dgcn_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, int32_t dtype, void* dw,
-                              int64_t rows, int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream) {
-  if (!dz || !x || !dw) return DGCN_E_NULL;
-  if (!sizes_ok(rows, K, N) || rows == 0 || lddz < 0 || ldx < 0) return DGCN_E_SHAPE;
-  if (dtype < DGCN_T_F32 || dtype > DGCN_T_F16) return DGCN_E_MODE;
-  const MatParams P = {dz, lddz, x, ldx, nullptr, nullptr, nullptr, 0, DGCN_ACT_NONE, 0.f, 1, nullptr, nullptr, 0, nullptr, dw, N, K, rows};
-  return mat_run(P, 1, 1, dtype, dtype, ws, ws_bytes, static_cast<hipStream_t>(stream));
-}
-
-extern "C" int dgcn_pad_rows(const void* x, int64_t ldx, void* out, int64_t ldo, int64_t rows, int64_t bytes, void* stream) {
-  if (!x || !out) return DGCN_E_NULL;
-  if (rows < 0 || bytes < 1 || ldx < 0 || ldo != (bytes + 15) / 16 * 16) return DGCN_E_SHAPE;
-  if (reinterpret_cast<uintptr_t>(out) & 15) return DGCN_E_ALIGN;
-  if (rows == 0) return DGCN_OK;
-  int64_t wgs = (rows * (ldo / 16) + 255) / 256;
-  if (wgs > 32 * num_cus()) wgs = 32 * num_cus();
-  hipLaunchKernelGGL(pad_rows_kernel, dim3(static_cast<unsigned>(wgs)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                     static_cast<const uint8_t*>(x), ldx, static_cast<uint8_t*>(out), ldo, rows, bytes);
-  return launch_status();
+extern "C" int dgcn_linear_bwd(const void* g, int64_t ldg, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z,
+                               int32_t act, float slope, int32_t dtype, void* dx, void* dw, void* db, int32_t db_f32,
+                               int64_t rows, int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream) {
+  if (!g || (dw && !x) || (dx && !w) || (act != DGCN_ACT_NONE && !z)) return DGCN_E_NULL;
+  if (!sizes_ok(rows, K, N) || rows == 0 || ldg < 0 || ldx < 0 || ldw < 0) return DGCN_E_SHAPE;
+  if (!known_act(act) || dtype < DGCN_T_F32 || dtype > DGCN_T_F16) return DGCN_E_MODE;
+  if (reinterpret_cast<uintptr_t>(ws) & 15) return DGCN_E_ALIGN;
+  if (!dx && !dw && !db) return DGCN_OK;
+  const BwdArgs A = {g, ldg, x, ldx, w, ldw, z, act, slope, dtype, dx, dw, db, db_f32, rows, K, N};
+  Arena arena = {static_cast<char*>(ws), 0, ws ? ws_bytes : 0};
+  return linear_backward(A, arena, true, static_cast<hipStream_t>(stream));
 }

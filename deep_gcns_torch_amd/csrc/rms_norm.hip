@@ -403,22 +403,6 @@ extern "C" int32_t dgcn_rms_norm_num_partials(int64_t rows, int32_t C) {
   return static_cast<int32_t>(rms_bwd_grid(rows, C));
 }
 
-extern "C" int dgcn_rms_norm_bwd(const void* g, int64_t ldg, const void* gh, int64_t ldgh, const void* h, int64_t ldh,
-                                 const void* w, int32_t w_f32, const float* rstd, int32_t dtype, void* dx, float* dw_part,
-                                 int64_t rows, int32_t C, void* stream) {
-  if (!g || !h || !rstd || (!dx && !dw_part)) return DGCN_E_NULL;
-  if (rows < 0 || C < 1 || C > kRmsMaxC || ldg < 0 || ldh < 0 || (gh && ldgh < 0)) return DGCN_E_SHAPE;
-  if (rows == 0) return DGCN_OK;
-  const RmsBwdParams P = {g, ldg, gh, ldgh, h, ldh, w, w_f32, C, rstd, rows, dx, dw_part};
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case DGCN_T_F32: return rms_bwd<float>(P, s);
-    case DGCN_T_BF16: return rms_bwd<__bf16>(P, s);
-    case DGCN_T_F16: return rms_bwd<_Float16>(P, s);
-    default: return DGCN_E_MODE;
-  }
-}
-
 extern "C" int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width, int32_t dtype, void* out, void* stream) {
   if (!out || (!parts && nparts > 0)) return DGCN_E_NULL;
   if (nparts < 0 || width < 0) return DGCN_E_SHAPE;
@@ -432,4 +416,22 @@ extern "C" int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width,
     default: return DGCN_E_MODE;
   }
   return launch_status();
+}
+
+extern "C" int dgcn_rms_norm_bwd(const void* g, int64_t ldg, const void* gh, int64_t ldgh, const void* h, int64_t ldh,
+                                 const void* w, int32_t w_f32, const float* rstd, int32_t dtype, void* dx, void* dw,
+                                 float* dw_part, int64_t rows, int32_t C, void* stream) {
+  if (!g || !h || !rstd || (!dx && !dw) || (dw && !dw_part)) return DGCN_E_NULL;
+  if (rows < 1 || C < 1 || C > kRmsMaxC || ldg < 0 || ldh < 0 || (gh && ldgh < 0)) return DGCN_E_SHAPE;
+  const RmsBwdParams P = {g, ldg, gh, ldgh, h, ldh, w, w_f32, C, rstd, rows, dx, dw ? dw_part : nullptr};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  int rc = DGCN_E_MODE;
+  switch (dtype) {
+    case DGCN_T_F32: rc = rms_bwd<float>(P, s); break;
+    case DGCN_T_BF16: rc = rms_bwd<__bf16>(P, s); break;
+    case DGCN_T_F16: rc = rms_bwd<_Float16>(P, s); break;
+    default: break;
+  }
+  if (rc != DGCN_OK || !dw) return rc;
+  return dgcn_param_sum(dw_part, static_cast<int32_t>(rms_bwd_grid(rows, C)), C, w_f32 ? DGCN_T_F32 : dtype, dw, stream);
 }

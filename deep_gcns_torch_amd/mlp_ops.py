@@ -94,13 +94,6 @@ def _same_rows(r, x: torch.Tensor, n: int, dtype, what: str) -> None:
         raise TypeError(f"{what} must be {dtype}, got {r.dtype}")
 
 
-def _param_sum(parts: torch.Tensor, dtype, stream: int) -> torch.Tensor:
-    out = torch.empty(parts.size(1), device=parts.device, dtype=dtype)
-    _lib.check(_lib.load().dgcn_param_sum(parts.data_ptr(), parts.size(0), parts.size(1), _TYPES[dtype], out.data_ptr(),
-                                          stream), "dgcn_param_sum")
-    return out
-
-
 def _needs_grad(*tensors) -> bool:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -172,21 +165,22 @@ class _RMSNormRows(torch.autograd.Function):
         d = h.get_device()
         h2, ldh = _rows2d(h)
         g2, ldg = _rows2d(g)
-        gh2, ldgh = _rows2d(gh) if gh is not None else (None, 0)
+        gh2, ldgh = (None, 0) if gh is None else _rows2d(gh)
         rows, C = h2.shape
         w, w_f32 = _param(weight, C, h.dtype, "weight")
         dx = h.new_empty(h.shape) if need_x else None
         gw = parts = None
-        with _lib.device_ctx(d):
-            stream = _lib.current_stream_handle(d)
-            if need_w:
-                parts = h.new_empty((lib.dgcn_rms_norm_num_partials(rows, C), C), dtype=torch.float32)
-            if need_x or need_w:
-                _lib.check(lib.dgcn_rms_norm_bwd(g2.data_ptr(), ldg, _lib.ptr(gh2), ldgh, h2.data_ptr(), ldh, _lib.ptr(w),
-                                                 w_f32, rstd.data_ptr(), _TYPES[h.dtype], _lib.ptr(dx), _lib.ptr(parts),
-                                                 rows, C, stream), "dgcn_rms_norm_bwd")
-            if need_w:
-                gw = _param_sum(parts, weight.dtype, stream)
+        if need_w:
+            gw = weight.new_empty(C)
+            parts = h.new_empty((lib.dgcn_rms_norm_num_partials(rows, C), C), dtype=torch.float32)
+        if need_x or need_w:
+            ptr = _lib.ptr
+            with _lib.device_ctx(d):
+                rc = lib.dgcn_rms_norm_bwd(g2.data_ptr(), ldg, ptr(gh2), ldgh, h2.data_ptr(), ldh, ptr(w), w_f32,
+                                           rstd.data_ptr(), _TYPES[h.dtype], ptr(dx), ptr(gw), ptr(parts), rows, C,
+                                           _lib.current_stream_handle(d))
+            if rc:
+                _lib.check(rc, "dgcn_rms_norm_bwd")
         return (dx if ctx.needs_input_grad[0] else None), gw, (dx if ctx.needs_input_grad[2] else None), None
 
 
@@ -251,62 +245,28 @@ class RMSNorm(nn.Module):
 
 
 # ---- product with epilogue ------------------------------------------------------------------------------------------
-_FAR = 1 << 20          # row strides from here on leave the kernels' 32-bit offsets
-_SMALL = None           # rows up to which linear_act takes its operands at any byte (dgcn_linear_small_rows)
-
-
-def _workspace(product: int, rows: int, K: int, N: int, in_type: int, like: torch.Tensor):
-    """(workspace or None, its bytes) of one product call: memory of that call alone, also inside a captured graph."""
-    n = _lib.load().dgcn_linear_workspace(product, rows, K, N, in_type)
-    return (like.new_empty(n, dtype=torch.uint8), n) if n else (None, 0)
-
-
-def _operand(x: torch.Tensor):
-    """A product operand as (rows on 16-byte starts, zeros up to 16 bytes behind each row; row stride in values).  Rows that
-    are so already are taken in place."""
-    x2, ld = _rows2d(x)
-    es = x2.element_size()
-    C = x2.size(1)
-    if x2.data_ptr() % 16 == 0 and ld * es % 16 == 0 and C * es % 16 == 0 and ld <= _FAR:
-        return x2, ld
-    ldo = -(-C * es // 16) * 16
-    out = x2.new_empty((x2.size(0), ldo // es))
-    if x2.size(0):
-        d = x2.get_device()
-        with _lib.device_ctx(d):
-            _lib.check(_lib.load().dgcn_pad_rows(x2.data_ptr(), ld * es, out.data_ptr(), ldo, x2.size(0), C * es,
-                                                 _lib.current_stream_handle(d)), "dgcn_pad_rows")
-    return out, ldo // es
-
-
 def _linear(x, weight, sx, sw, bias, residual, act: int, slope: float, in_type: int, out_dtype, keep: bool):
-    """One launch of checked arguments -> (y, what the backward keeps of the activation or None)."""
-    global _SMALL
+    """One call of checked arguments -> (y, what the backward keeps of the activation or None)."""
     lib = _lib.load()
-    if _SMALL is None:
-        _SMALL = lib.dgcn_linear_small_rows()
     N, K = weight.shape
-    lead = x.shape[:-1]
-    y = x.new_empty((*lead, N), dtype=out_dtype)
+    y = x.new_empty((*x.shape[:-1], N), dtype=out_dtype)
     z = y.new_empty(y.shape) if keep and act != 0 else None
     if y.numel() == 0:
         return y, z
     x2, ldx = _rows2d(x)
+    w2, ldw = _rows2d(weight)
     rows = x2.size(0)
-    ws, ws_bytes = None, 0
-    if rows <= _SMALL:
-        w2, ldw = _rows2d(weight)
-    else:
-        x2, ldx = _operand(x2)
-        w2, ldw = _operand(weight)
-        ws, ws_bytes = _workspace(0, rows, K, N, in_type, y)
     r2, ldr = (None, 0) if residual is None else _rows2d(residual)
     if bias is not None and not bias.is_contiguous():
         bias = bias.detach().contiguous()
     ptr = _lib.ptr
+    px, pw = x2.data_ptr(), w2.data_ptr()
+    # memory of this call alone, also inside a captured graph
+    ws_bytes = lib.dgcn_linear_workspace(px, ldx, pw, ldw, in_type, rows, K, N)
+    ws = y.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     d = y.get_device()
     with _lib.device_ctx(d):
-        rc = lib.dgcn_linear_act(x2.data_ptr(), ldx, w2.data_ptr(), ldw, ptr(sx), ptr(sw), ptr(bias),
+        rc = lib.dgcn_linear_act(px, ldx, pw, ldw, ptr(sx), ptr(sw), ptr(bias),
                                  1 if bias is not None and bias.dtype == torch.float32 else 0, ptr(r2), ldr, act, slope, in_type,
                                  _TYPES[out_dtype], ptr(z), y.data_ptr(), rows, K, N, ptr(ws), ws_bytes,
                                  _lib.current_stream_handle(d))
@@ -330,46 +290,30 @@ class _LinearAct(torch.autograd.Function):
         x, weight, z = ctx.saved_tensors
         act, slope, bias_type = ctx.cfg
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        gx = gw = gb = None
+        gx = torch.zeros_like(x) if need_x and g.numel() == 0 else x.new_empty(x.shape) if need_x else None
+        N, K = weight.shape
         if g.numel() == 0:                       # no rows: sums over nothing
-            gx = torch.zeros_like(x) if need_x else None
-            gw = torch.zeros_like(weight) if need_w else None
-            gb = torch.zeros(weight.size(0), device=g.device, dtype=bias_type) if need_b else None
-        elif need_x or need_w or need_b:
+            gw = weight.new_zeros((N, K)) if need_w else None
+            gb = weight.new_zeros(N, dtype=bias_type) if need_b else None
+            return gx, gw, gb, (g if need_r else None), None, None
+        gw = weight.new_empty((N, K)) if need_w else None
+        gb = weight.new_empty(N, dtype=bias_type) if need_b else None
+        if need_x or need_w or need_b:
             lib = _lib.load()
-            dev, t = x.device, _TYPES[x.dtype]
-            N, K = weight.shape
-            g2, ldg = _rows2d(g)
+            t = _TYPES[x.dtype]
+            (x2, ldx), (w2, ldw), (g2, ldg) = _rows2d(x), _rows2d(weight), _rows2d(g)
             rows = g2.size(0)
-            with _lib.device_ctx(dev):
-                stream = _lib.current_stream_handle(dev)
-                d2, ldd = g2, ldg
-                if act != 0 or need_b:
-                    parts = None
-                    if act != 0:
-                        ldd = -(-N // 8) * 8     # whole 16 bytes: the products below take dz as it is
-                        d2 = torch.empty(rows, ldd, device=dev, dtype=x.dtype)
-                    if need_b:
-                        parts = torch.empty(lib.dgcn_linear_gate_num_partials(rows, N), N, device=dev, dtype=torch.float32)
-                    _lib.check(lib.dgcn_linear_gate(g2.data_ptr(), ldg, _lib.ptr(z), act, slope, t,
-                                                    d2.data_ptr() if act != 0 else None, ldd if act != 0 else 0,
-                                                    _lib.ptr(parts), rows, N, stream), "dgcn_linear_gate")
-                    if need_b:
-                        gb = _param_sum(parts, bias_type, stream)
-                if act == 0 and (need_x or need_w):
-                    d2, ldd = _operand(g2)
-                if need_x:
-                    w2, ldw = _operand(weight)
-                    gx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-                    ws, ws_bytes = _workspace(1, rows, K, N, t, gx)
-                    _lib.check(lib.dgcn_linear_dx(d2.data_ptr(), ldd, w2.data_ptr(), ldw, t, gx.data_ptr(), rows, K, N,
-                                                  _lib.ptr(ws), ws_bytes, stream), "dgcn_linear_dx")
-                if need_w:
-                    x2, ldx = _operand(x)
-                    gw = torch.empty(N, K, device=dev, dtype=weight.dtype)
-                    ws, ws_bytes = _workspace(2, rows, K, N, t, gw)
-                    _lib.check(lib.dgcn_linear_dw(d2.data_ptr(), ldd, x2.data_ptr(), ldx, t, gw.data_ptr(), rows, K, N,
-                                                  _lib.ptr(ws), ws_bytes, stream), "dgcn_linear_dw")
+            px, pw, pg, ptr = x2.data_ptr(), w2.data_ptr(), g2.data_ptr(), _lib.ptr
+            ws_bytes = lib.dgcn_linear_bwd_workspace(pg, ldg, px, ldx, pw, ldw, act, t, need_x + 2 * need_w + 4 * need_b, rows,
+                                                     K, N)
+            ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+            d = g.get_device()
+            with _lib.device_ctx(d):
+                rc = lib.dgcn_linear_bwd(pg, ldg, px, ldx, pw, ldw, ptr(z), act, slope, t, ptr(gx), ptr(gw), ptr(gb),
+                                         1 if bias_type == torch.float32 else 0, rows, K, N, ptr(ws), ws_bytes,
+                                         _lib.current_stream_handle(d))
+            if rc:
+                _lib.check(rc, "dgcn_linear_bwd")
         return gx, gw, gb, (g if need_r else None), None, None
 
 

@@ -724,8 +724,8 @@ int dgcn_rows_tn_colsum_f32(const float* g, int64_t ldg, const float* x, int64_t
  *     scale = max |y| / 448 over the finite values of the row, at least 2^-126, and 1 where that maximum is 0; a NaN or
  *     an infinity becomes NaN (0x7f) in its own place
  *   h (rows, C) dtype contiguous or NULL (y does not depend on h's rounding); rstd (rows) or NULL
- * Backward: dx = rstd (w g - xh mean(w g xh)) [+ gh], xh = h rstd, contiguous, or NULL; dw_part
- *   [dgcn_rms_norm_num_partials(rows, C)][C] whose sum over the first axis (dgcn_param_sum) is the weight's gradient, or NULL.
+ * Backward (rows >= 1): dx = rstd (w g - xh mean(w g xh)) [+ gh], xh = h rstd, contiguous, or NULL; dw (C) in the weight's
+ *   type (fp32 with w_f32) or NULL, by way of dw_part [dgcn_rms_norm_num_partials(rows, C)][C].
  * dgcn_quantize_rows_e4m3: q and scale of x itself.
  * dgcn_param_sum: out[c] = sum over p of parts[p][c], c < width, rounded to dtype; fixed order. */
 int dgcn_rms_norm_fwd(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, int32_t w_f32, float eps,
@@ -733,8 +733,8 @@ int dgcn_rms_norm_fwd(const void* x, int64_t ldx, const void* res, int64_t ldr, 
                       void* stream);
 int32_t dgcn_rms_norm_num_partials(int64_t rows, int32_t C);
 int dgcn_rms_norm_bwd(const void* g, int64_t ldg, const void* gh, int64_t ldgh, const void* h, int64_t ldh, const void* w,
-                      int32_t w_f32, const float* rstd, int32_t dtype, void* dx, float* dw_part, int64_t rows, int32_t C,
-                      void* stream);
+                      int32_t w_f32, const float* rstd, int32_t dtype, void* dx, void* dw, float* dw_part, int64_t rows,
+                      int32_t C, void* stream);
 int dgcn_quantize_rows_e4m3(const void* x, int64_t ldx, int32_t dtype, uint8_t* q, float* scale, int64_t rows, int32_t C,
                             void* stream);
 int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width, int32_t dtype, void* out, void* stream);
@@ -745,32 +745,24 @@ int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width, int32_t dt
  *   x (rows, K) row stride ldx, w (N, K) row stride ldw, both in in_type; K, N <= 2^20
  *   in_type DGCN_T_E4M3: x_scale (rows) and w_scale (N) are required and out_type is free; otherwise out_type = in_type
  *   bias (N) in out_type or, with bias_f32, fp32, or NULL; res (rows, N) out_type, row stride ldr, or NULL
- *   z (rows, N) contiguous, or NULL: kept for dgcn_linear_gate -- z in fp32, or in the 16-bit types act'(z) in 16-bit fixed
+ *   z (rows, N) contiguous, or NULL: kept for the backward -- z in fp32, or in the 16-bit types act'(z) in 16-bit fixed
  *     point (code 2^-15 - 1/4; 65535 is NaN; relu and leakyrelu: z > 0 as 1 or 0); y (rows, N) out_type contiguous
- * Backward, all in one dtype:
- *   dgcn_linear_gate: dz = g act'(z), row stride lddz, N <= lddz <= N rounded up to 8, zeros behind N (dz may be NULL with
- *     DGCN_ACT_NONE: dz is g), and db_part
- *     [dgcn_linear_gate_num_partials(rows, N)][N], whose sum is the bias gradient, or NULL
- *   dgcn_linear_dx: dx (rows, K) = dz w        dgcn_linear_dw: dw (N, K) = dz^T x
- * Operands of the three products (x, w, dz; not those of dgcn_linear_act with at most dgcn_linear_small_rows() rows) start on 16 bytes and their row strides are multiples of 16 bytes (DGCN_E_ALIGN
- *   otherwise); where a row's K or N values are not, the values up to the next 16 bytes are there and are zeros:
- *   dgcn_pad_rows copies rows of `bytes` bytes, row stride ldx bytes, to such rows of ldo = bytes rounded up to 16.
- * ws: dgcn_linear_workspace(product, rows, K, N, in_type) bytes, 16-byte aligned, of this call's own (fp32 partial sums of a
- *   split reduction; may be 0 and NULL); product 0: dgcn_linear_act, 1: dgcn_linear_dx, 2: dgcn_linear_dw. */
-int32_t dgcn_linear_small_rows(void);
-int dgcn_pad_rows(const void* x, int64_t ldx, void* out, int64_t ldo, int64_t rows, int64_t bytes, void* stream);
-size_t dgcn_linear_workspace(int32_t product, int64_t rows, int32_t K, int32_t N, int32_t in_type);
+ * Backward, all in one dtype, rows >= 1:  dz = g act'(z);  dx (rows, K) = dz w, dw (N, K) = dz^T x, db (N) = sum of dz over the
+ *   rows (dtype or, with db_f32, fp32), contiguous, each or NULL; z as above (NULL with DGCN_ACT_NONE)
+ * Operands may start and repeat at any byte; those that do not lie on 16 bytes are copied into the workspace first where the
+ * product is tiled.  ws: dgcn_linear_workspace / dgcn_linear_bwd_workspace (want: 1 dx, 2 dw, 4 db) bytes for the same
+ * pointers, strides and sizes, 16-byte aligned, of this call's own (DGCN_E_WORKSPACE if smaller; may be 0 and NULL). */
+size_t dgcn_linear_workspace(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t in_type, int64_t rows, int32_t K,
+                             int32_t N);
 int dgcn_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* x_scale, const float* w_scale,
                     const void* bias, int32_t bias_f32, const void* res, int64_t ldr, int32_t act, float slope,
                     int32_t in_type, int32_t out_type, void* z, void* y, int64_t rows, int32_t K, int32_t N, void* ws,
                     size_t ws_bytes, void* stream);
-int32_t dgcn_linear_gate_num_partials(int64_t rows, int32_t N);
-int dgcn_linear_gate(const void* g, int64_t ldg, const void* z, int32_t act, float slope, int32_t dtype, void* dz,
-                     int64_t lddz, float* db_part, int64_t rows, int32_t N, void* stream);
-int dgcn_linear_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, int32_t dtype, void* dx, int64_t rows,
-                   int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream);
-int dgcn_linear_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, int32_t dtype, void* dw, int64_t rows,
-                   int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream);
+size_t dgcn_linear_bwd_workspace(const void* g, int64_t ldg, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                 int32_t act, int32_t dtype, int32_t want, int64_t rows, int32_t K, int32_t N);
+int dgcn_linear_bwd(const void* g, int64_t ldg, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z,
+                    int32_t act, float slope, int32_t dtype, void* dx, void* dw, void* db, int32_t db_f32, int64_t rows,
+                    int32_t K, int32_t N, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

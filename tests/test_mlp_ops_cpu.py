@@ -62,24 +62,31 @@ def test_c_entry_argument_errors_do_not_launch():
     assert norm(p, 8, None, 0, None, 0, 1e-6, 3, p, None, None, None, None, 1, 8, None) == -4  # 8-bit rows have no norm
     assert norm(p, 8, None, 0, None, 0, 1e-6, 0, p, None, None, None, None, 1, 32769, None) == -2
     assert norm(p, 8, None, 0, None, 0, 1e-6, 0, p, None, None, None, None, 0, 8, None) == 0   # no rows: no launch
-    assert lib.dgcn_rms_norm_bwd(p, 8, None, 0, p, 8, None, 0, p, 0, None, None, 1, 8, None) == -1
+    bwd = lib.dgcn_rms_norm_bwd
+    assert bwd(p, 8, None, 0, p, 8, None, 0, p, 0, None, None, None, 1, 8, None) == -1          # nothing asked for
+    assert bwd(p, 8, None, 0, p, 8, None, 0, p, 0, p, p, None, 1, 8, None) == -1                # dw without its partials
+    assert bwd(p, 8, None, 0, p, 8, None, 0, p, 0, p, None, None, 0, 8, None) == -2             # a sum over no rows is the caller's
     assert lib.dgcn_quantize_rows_e4m3(p, 8, 0, p, None, 1, 8, None) == -1
     assert lib.dgcn_param_sum(None, 1, 4, 0, p, None) == -1
-    assert lib.dgcn_rms_norm_num_partials(0, 8) == 0 and lib.dgcn_linear_gate_num_partials(0, 8) == 0
-    gate = lib.dgcn_linear_gate
-    assert gate(p, 8, None, 1, 0.2, 0, p, 8, None, 1, 8, None) == -1                              # an activation needs z
-    assert gate(p, 8, p, 9, 0.2, 0, p, 8, None, 1, 8, None) == -4
-    assert gate(p, 8, p, 1, 0.2, 0, p, 7, None, 1, 8, None) == -2 and gate(p, 8, p, 1, 0.2, 0, p, 16, None, 1, 8, None) == -2
+    assert lib.dgcn_rms_norm_num_partials(0, 8) == 0
     act = lib.dgcn_linear_act
     assert act(p, 8, p, 8, None, None, None, 0, None, 0, 0, 0.0, 3, 1, None, p, 1, 8, 8, None, 0, None) == -1   # e4m3 without scales
     assert act(p, 8, p, 8, None, None, None, 0, None, 0, 0, 0.0, 1, 2, None, p, 1, 8, 8, None, 0, None) == -4   # bf16 rows, fp16 result
     assert act(p, 8, p, 8, None, None, None, 0, None, 0, 9, 0.0, 1, 1, None, p, 1, 8, 8, None, 0, None) == -4   # no such activation
-    assert act(p + 2, 8, p, 8, None, None, None, 0, None, 0, 0, 0.0, 1, 1, None, p, 99, 8, 8, None, 0, None) == -3
-    assert act(p, 9, p, 8, None, None, None, 0, None, 0, 0, 0.0, 1, 1, None, p, 99, 8, 8, None, 0, None) == -3
-    n = lib.dgcn_linear_workspace(2, 100000, 64, 64, 1)
-    assert n > 0 and lib.dgcn_linear_dw(p, 64, p, 64, 1, p, 100000, 64, 64, p, n - 1, None) == -5               # workspace too small
-    assert lib.dgcn_linear_dw(p, 64, p, 64, 1, p, 0, 64, 64, None, 0, None) == -2                               # a sum over no rows is the caller's
-    assert lib.dgcn_pad_rows(p, 5, p, 32, 1, 5, None) == -2 and lib.dgcn_pad_rows(p, 5, p + 4, 16, 1, 5, None) == -3
+    assert act(p, 8, p, 8, None, None, None, 0, None, 0, 0, 0.0, 1, 1, None, p, 1, 8, 8, p + 4, 0, None) == -3  # workspace alignment
+    assert act(p, 8, p, 8, None, None, None, 0, None, 0, 0, 0.0, 1, 1, None, p, 1, 0, 8, None, 0, None) == -2
+    back = lib.dgcn_linear_bwd
+    assert back(p, 8, p, 8, p, 8, None, 1, 0.0, 0, p, p, p, 0, 1, 8, 8, None, 0, None) == -1                    # an activation needs z
+    assert back(p, 8, p, 8, p, 8, p, 9, 0.0, 0, p, p, p, 0, 1, 8, 8, None, 0, None) == -4
+    assert back(p, 8, p, 8, p, 8, None, 0, 0.0, 0, p, p, p, 0, 0, 8, 8, None, 0, None) == -2
+    assert back(p, 8, p, 8, p, 8, None, 0, 0.0, 0, None, None, None, 0, 1, 8, 8, None, 0, None) == 0            # nothing asked for
+    # workspaces: none for few rows; partial sums for a long reduction; copies for rows off 16 bytes, and too small is refused
+    need, back_need = lib.dgcn_linear_workspace, lib.dgcn_linear_bwd_workspace
+    assert need(p, 8, p, 8, 1, 64, 8, 8) == 0 and need(p, 4096, p, 4096, 1, 65536, 4096, 4096) == 0
+    assert need(p, 9, p, 8, 1, 1000, 8, 8) >= 1000 * 16 and need(p + 2, 8, p, 8, 1, 1000, 8, 8) >= 1000 * 16
+    assert act(p + 2, 8, p, 8, None, None, None, 0, None, 0, 0, 0.0, 1, 1, None, p, 1000, 8, 8, p, 64, None) == -5
+    n = back_need(p, 64, p, 64, p, 64, 0, 1, 2, 100000, 64, 64)
+    assert n > 0 and back(p, 64, p, 64, p, 64, None, 0, 0.0, 1, None, p, None, 0, 100000, 64, 64, p, n - 256, None) == -5
 
 
 def test_norm_layer_offers_rms():
