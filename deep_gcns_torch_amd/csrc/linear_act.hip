@@ -7,6 +7,7 @@
 // Every sum is held in fp32.  For the backward the forward keeps z in fp32, or act'(z) in 16-bit fixed point where the rows
 // have 16 bits (mlp_common.h); dz is rounded to the rows' type before the two products, which take that on the matrix pipe.
 
+
 #include "linear_act.h"
 
 namespace dgcn {
@@ -44,8 +45,8 @@ struct MatPlan {
 // traffic take (`work`, times the workgroups a CU holds), and at least the latency of the copies behind it; a split
 // writes and reads fp32 partial sums and launches once more.
 inline MatPlan mat_plan(int64_t M, int64_t N, int64_t K, int type, int ta) {
-  struct { int bm, bn, held; double work; } tiles[3] = {{256, 256, 1, 3000.}, {128, 128, 2, 900.}, {64, 128, 3, 600.}};
-  const int64_t bk = type == DGCN_T_E4M3 ? 128 : type == DGCN_T_F32 ? 32 : 64, steps = (K + bk - 1) / bk;
+  struct { int bm, bn, held; double work; } tiles[3] = {{256, 256, 1, 1250.}, {128, 128, 2, 380.}, {64, 128, 3, 260.}};
+  const int64_t bk = type == DGCN_T_E4M3 ? 64 : type == DGCN_T_F32 ? 16 : 32, steps = (K + bk - 1) / bk;
   const double cus = num_cus();
   MatPlan best = {0, 1};
   double least = 1e300;
@@ -54,8 +55,8 @@ inline MatPlan mat_plan(int64_t M, int64_t N, int64_t K, int type, int ta) {
     for (int sp = 1; sp <= 512 && sp <= steps; sp *= 2) {
       const double wgs = wgs1 * sp, per_cu = ceil(wgs / cus);
       const double held = per_cu < tiles[t].held ? per_cu : tiles[t].held;
-      const double step = held * tiles[t].work > 2000. ? held * tiles[t].work : 2000.;
-      double c = ceil(per_cu / tiles[t].held) * ((steps + sp - 1) / sp * step + 4000.);
+      const double step = held * tiles[t].work > 600. ? held * tiles[t].work : 600.;
+      double c = ceil(per_cu / tiles[t].held) * ((steps + sp - 1) / sp * step + 5000.);
       if (sp > 1) c += 8. * M * N * sp / 2000. + 10000.;
       if (c < least) { least = c; best = {t, sp}; }
     }

@@ -11,6 +11,64 @@
 namespace dgcn {
 namespace {
 
+// The types' fragments of a step (128 bytes of the reduction) for 16 x 16 matrix instructions; see TileIn
+template <class T> struct MatIn;
+
+template <class T>
+struct MatIn16 {
+  static constexpr int ES = 2;
+  struct Frag { u4v r[2]; };
+  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) { return Frag{{r[0], r[1]}}; }
+  static __device__ __forceinline__ f32x4 one(u4v a, u4v b, f32x4 c) {
+    if constexpr (__is_same(T, __bf16)) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+  }
+  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
+    c = one(b.r[1], a.r[1], one(b.r[0], a.r[0], c));
+  }
+};
+template <> struct MatIn<__bf16> : MatIn16<__bf16> {};
+template <> struct MatIn<_Float16> : MatIn16<_Float16> {};
+
+template <> struct MatIn<float> {
+  static constexpr int ES = 4;
+  struct Frag { i4v h, m, l; };
+  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) {
+    Frag f;
+    eg_split3(__builtin_bit_cast(f4v, r[0]), __builtin_bit_cast(f4v, r[1]), f.h, f.m, f.l);
+    return f;
+  }
+  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
+    c = eg_mfma_bf16(b.h, a.l, eg_mfma_bf16(b.l, a.h, eg_mfma_bf16(b.m, a.m, c)));
+    c = eg_mfma_bf16(b.h, a.h, eg_mfma_bf16(b.h, a.m, eg_mfma_bf16(b.m, a.h, c)));
+  }
+};
+
+template <> struct MatIn<uint8_t> {
+  static constexpr int ES = 1;
+  typedef i8v Frag;
+  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) {
+    return __builtin_bit_cast(i8v, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
+    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, 127, 0, 127);
+  }
+};
+template <> struct MatIn<WideE4m3> {
+  static constexpr int ES = 1;
+  struct Frag { u4v r[4]; };
+  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) {
+    return Frag{{widen_e4m3(r[0][0], r[0][1]), widen_e4m3(r[0][2], r[0][3]), widen_e4m3(r[1][0], r[1][1]), widen_e4m3(r[1][2], r[1][3])}};
+  }
+  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = MatIn16<_Float16>::one(b.r[s], a.r[s], c);
+  }
+};
+
 typedef u4v u4v_any1 __attribute__((aligned(1)));
 
 // 16 bytes at `at` of a row of `bytes`; behind its end zeros

@@ -1,5 +1,9 @@
-// The tiled product on the matrix pipe: BM x BN tiles, 128 bytes of the reduction a step, operands copied straight from
-// memory into LDS (two buffers), 16 x 16 matrix instructions, fp32 sums.
+// The tiled product on the matrix pipe: BM x BN tiles, fp32 sums in 32 x 32 matrix instructions, operands copied straight
+// from memory into a ring of four LDS stages of 64 bytes of the reduction.
+//
+// Bound by the matrix pipe (large products) or by HBM (long thin ones).  An iteration computes on fragments that lie in
+// registers already, while the next stage's fragments are read from LDS and the stage after the ring's last is requested from
+// memory: the matrix instructions wait for neither, and a barrier costs them the time it takes to meet.
 #pragma once
 
 #include <type_traits>
@@ -12,147 +16,177 @@ namespace {
 
 typedef int i8v __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u8v __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s4v lds_s4;
 
-// What a wave does with the fragments of one step (128 bytes of the reduction): a raw fragment is two 16-byte units of an
-// operand row; prep() makes of it what the matrix instructions take, mul() adds four channel fragments' products.
-template <class T> struct MatIn;
+__device__ __forceinline__ u4v half0(u8v r) { return __builtin_shufflevector(r, r, 0, 1, 2, 3); }
+__device__ __forceinline__ u4v half1(u8v r) { return __builtin_shufflevector(r, r, 4, 5, 6, 7); }
+
+// What a wave does with the fragments of a stage: a raw fragment is two 16-byte units of an operand row (lane l: row l & 31,
+// h = l >> 5), prep() makes of it what the matrix instructions take, mul() adds one tile's products.
+template <class T> struct TileIn;
 
 template <class T>
-struct MatIn16 {
+struct TileIn16 {                                          // units h and 2 + h: k = 8 h .. of each half of the stage's 32
   static constexpr int ES = 2;
   struct Frag { u4v r[2]; };
-  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) { return Frag{{r[0], r[1]}}; }
-  static __device__ __forceinline__ f32x4 one(u4v a, u4v b, f32x4 c) {
+  static __device__ __forceinline__ Frag prep(u8v r) { return Frag{{half0(r), half1(r)}}; }
+  static __device__ __forceinline__ f32x16 one(u4v a, u4v b, f32x16 c) {
     if constexpr (__is_same(T, __bf16)) {
-      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     } else {
-      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
   }
-  static __device__ __forceinline__ void mul(const Frag (&b)[4], const Frag& a, f32x4 (&c)[4]) {
+  static __device__ __forceinline__ void mul(const Frag (&b)[2], const Frag& a, f32x16 (&c)[2]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) c[t] = one(b[t].r[s], a.r[s], c[t]);
+      for (int t = 0; t < 2; ++t) c[t] = one(b[t].r[s], a.r[s], c[t]);
     }
   }
-  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
-    c = one(b.r[1], a.r[1], one(b.r[0], a.r[0], c));
-  }
 };
-template <> struct MatIn<__bf16> : MatIn16<__bf16> {};
-template <> struct MatIn<_Float16> : MatIn16<_Float16> {};
+template <> struct TileIn<__bf16> : TileIn16<__bf16> {};
+template <> struct TileIn<_Float16> : TileIn16<_Float16> {};
 
-// fp32: three bf16 parts that add up to the value bit for bit, and the six products of parts down to 2^-16 of the largest
-// (bf16x6.h: off by at most 3 2^-24 |a b|), at six times the cost of a bf16 product and a sixteenth of an fp32 one's
-template <> struct MatIn<float> {
+// fp32 (units 2 h and 2 h + 1: k = 8 h .. 8 h + 7 of the stage's 16): three bf16 parts that add up to the value bit for bit,
+// and the six products of parts down to 2^-16 of the largest (bf16x6.h: off by at most 3 2^-24 |a b|)
+template <> struct TileIn<float> {
   static constexpr int ES = 4;
-  struct Frag { i4v h, m, l; };
-  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) {
-    Frag f;
-    eg_split3(__builtin_bit_cast(f4v, r[0]), __builtin_bit_cast(f4v, r[1]), f.h, f.m, f.l);
-    return f;
+  struct Frag { u4v h, m, l; };
+  static __device__ __forceinline__ Frag prep(u8v r) {
+    i4v h, m, l;
+    eg_split3(__builtin_bit_cast(f4v, half0(r)), __builtin_bit_cast(f4v, half1(r)), h, m, l);
+    return Frag{__builtin_bit_cast(u4v, h), __builtin_bit_cast(u4v, m), __builtin_bit_cast(u4v, l)};
   }
-  static __device__ __forceinline__ void mul(const Frag (&b)[4], const Frag& a, f32x4 (&c)[4]) {
+  static __device__ __forceinline__ void mul(const Frag (&b)[2], const Frag& a, f32x16 (&c)[2]) {
+    typedef TileIn16<__bf16> P;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].m, a.m, c[t]);
+    for (int t = 0; t < 2; ++t) c[t] = P::one(b[t].m, a.m, c[t]);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].l, a.h, c[t]);
+    for (int t = 0; t < 2; ++t) c[t] = P::one(b[t].l, a.h, c[t]);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].h, a.l, c[t]);
+    for (int t = 0; t < 2; ++t) c[t] = P::one(b[t].h, a.l, c[t]);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].m, a.h, c[t]);
+    for (int t = 0; t < 2; ++t) c[t] = P::one(b[t].m, a.h, c[t]);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].h, a.m, c[t]);
+    for (int t = 0; t < 2; ++t) c[t] = P::one(b[t].h, a.m, c[t]);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) c[t] = eg_mfma_bf16(b[t].h, a.h, c[t]);
-  }
-  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
-    c = eg_mfma_bf16(b.h, a.l, eg_mfma_bf16(b.l, a.h, eg_mfma_bf16(b.m, a.m, c)));
-    c = eg_mfma_bf16(b.h, a.h, eg_mfma_bf16(b.h, a.m, eg_mfma_bf16(b.m, a.h, c)));
+    for (int t = 0; t < 2; ++t) c[t] = P::one(b[t].h, a.h, c[t]);
   }
 };
 
-// e4m3 for a 16-bit result: one instruction of K = 128 at twice the 16-bit rate, its block scales held at 2^0.  It aligns
-// the products of eight neighbouring k to the largest one's exponent and drops what lies more than 13 bits below it
-// (measured, bit by bit), so a sum is off by up to 7 2^-13 of the largest product of each eight: 6e-5 of the result's
-// root mean square over normal rows, an order below a bf16 half step and under half of an fp16 one.
-template <> struct MatIn<uint8_t> {
+// e4m3 for a 16-bit result (units 2 h and 2 h + 1: 32 of the stage's 64 values): one instruction at twice the 16-bit rate, its
+// block scales held at 2^0.  It aligns the products of eight neighbouring k to the largest one's exponent and drops what lies
+// more than 13 bits below it (measured, bit by bit), so a sum is off by up to 7 2^-13 of the largest product of each eight:
+// 6e-5 of the result's root mean square over normal rows, an order below a bf16 half step and under half of an fp16 one.
+template <> struct TileIn<uint8_t> {
   static constexpr int ES = 1;
   typedef i8v Frag;
-  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) {
-    return __builtin_bit_cast(i8v, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
-  }
-  static __device__ __forceinline__ void mul(const Frag (&b)[4], const Frag& a, f32x4 (&c)[4]) {
+  static __device__ __forceinline__ Frag prep(u8v r) { return __builtin_bit_cast(i8v, r); }
+  static __device__ __forceinline__ void mul(const Frag (&b)[2], const Frag& a, f32x16 (&c)[2]) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) c[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[t], a, c[t], 0, 0, 0, 127, 0, 127);
-  }
-  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
-    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, 127, 0, 127);
+    for (int t = 0; t < 2; ++t) c[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[t], a, c[t], 0, 0, 0, 127, 0, 127);
   }
 };
+
 // e4m3 for an fp32 result: every e4m3 value is an fp16 value; their products are exact and their sum is fp32
 struct WideE4m3 {};
-template <> struct MatIn<WideE4m3> {
+__device__ __forceinline__ u4v widen_e4m3(uint32_t lo, uint32_t hi) {
+  return u4v{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false)),
+             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true)),
+             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false)),
+             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true))};
+}
+template <> struct TileIn<WideE4m3> {
   static constexpr int ES = 1;
   struct Frag { u4v r[4]; };
-  static __device__ __forceinline__ u4v widen(uint32_t lo, uint32_t hi) {
-    return u4v{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true))};
+  static __device__ __forceinline__ Frag prep(u8v r) {
+    return Frag{{widen_e4m3(r[0], r[1]), widen_e4m3(r[2], r[3]), widen_e4m3(r[4], r[5]), widen_e4m3(r[6], r[7])}};
   }
-  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) {
-    return Frag{{widen(r[0][0], r[0][1]), widen(r[0][2], r[0][3]), widen(r[1][0], r[1][1]), widen(r[1][2], r[1][3])}};
-  }
-  static __device__ __forceinline__ void mul(const Frag (&b)[4], const Frag& a, f32x4 (&c)[4]) {
+  static __device__ __forceinline__ void mul(const Frag (&b)[2], const Frag& a, f32x16 (&c)[2]) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) c[t] = MatIn16<_Float16>::one(b[t].r[s], a.r[s], c[t]);
+      for (int t = 0; t < 2; ++t) c[t] = TileIn16<_Float16>::one(b[t].r[s], a.r[s], c[t]);
     }
-  }
-  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) c = MatIn16<_Float16>::one(b.r[s], a.r[s], c);
   }
 };
 
 constexpr unsigned kRsrcFlags = 0x00027000;               // raw 32-bit buffer; a load behind its end gives zeros
 constexpr unsigned kBehind = 0x80000000u;                 // an offset behind any buffer here (at most 2^31 bytes)
+constexpr int kStages = 4;
 
-// Which rows / columns of an operand tile a 16-byte unit of LDS holds.
-//   K-contiguous, R rows of 128 bytes: unit u of row r holds the row's chunk u ^ (r & 7)
-//   K-strided, k-rows of R values: unit u of k-row k holds chunk u ^ 2 ((k & 3) | bit 3 of k << 2) in 16 bits,
-//     u ^ 4 (bits 4, 3 of k) in 32
+// Which chunk (16 bytes) of an operand tile a 16-byte unit of an LDS stage holds.
+//   K-contiguous, R rows of 64 bytes: unit u of row r holds the row's chunk u ^ (bits 3, 2 of r)
+//   K-strided, k-rows of R values: unit u of k-row k holds chunk u ^ 4 (k & 3) in 16 bits, u ^ 8 (bit 3 of k) in 32
 // In all, lanes that read together fall on different banks.
 template <int T, int R, int ES>
 __device__ __forceinline__ unsigned tile_offset(int inst, int lane, int64_t ld) {
   if constexpr (T == 0) {
-    const int row = inst * 8 + (lane >> 3);
-    return static_cast<unsigned>(row * ld * ES) + (((lane & 7) ^ (row & 7)) << 4);
+    const int row = inst * 16 + (lane >> 2);
+    return static_cast<unsigned>(row * ld * ES) + (((lane & 3) ^ ((row >> 2) & 3)) << 4);
   } else {
     constexpr int UNITS = R * ES / 16;
     const int k = inst * (64 / UNITS) + lane / UNITS;
-    const int f = ES == 2 ? 2 * ((k & 3) | ((k >> 3) & 1) << 2) : 4 * ((k >> 3) & 3);
+    const int f = ES == 2 ? 4 * (k & 3) : 8 * ((k >> 3) & 1);
     return static_cast<unsigned>(k * ld * ES) + (((lane % UNITS) ^ f) << 4);
   }
 }
 
-// T: operand type, O: output type, TA / TB: layouts; a wave owns 16 TM rows x 64 channels, a workgroup WM x WN waves
+// bytes from the first to behind the last value of an operand tile whose stage holds k of the reduction
+template <int T, int ES>
+__device__ __forceinline__ int tile_bytes(int64_t ld, int64_t lines, int k) {
+  constexpr int CH = 16 / ES;                              // values in 16 bytes
+  return static_cast<int>((T == 0 ? (lines - 1) * ld + (k + CH - 1) / CH * CH : (k - 1) * ld + (lines + CH - 1) / CH * CH) * ES);
+}
+
+// 16 bytes a lane from memory to `to` + 16 lane in LDS (the host's pass of the compiler knows no copies of this width)
+__device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t r, unsigned off, char* to) {
+#ifdef __HIP_DEVICE_COMPILE__
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)to, 16, off, 0, 0, 0);
+#endif
+}
+
+template <int N>
+__device__ __forceinline__ void copy_whole(const char* p, int bytes, const unsigned (&off)[N], char* to) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, bytes, kRsrcFlags);
+#pragma unroll
+  for (int c = 0; c < N; ++c) copy16(r, off[c], to + c * 1024);
+}
+
+// any stage, k values of the reduction in it (none: zeros everywhere, and p is not read)
+template <int T, int N, int ES>
+__device__ __forceinline__ void copy_part(const char* p, int64_t ld, int64_t lines, int k, const unsigned (&off)[N], int wave,
+                                          int lane, char* to) {
+  const int bytes = k > 0 ? tile_bytes<T, ES>(ld, lines, k) : 0;
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, bytes, kRsrcFlags);
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    unsigned o = off[c];
+    if (T == 0) {
+      // byte of the row that this lane's chunk starts at
+      const unsigned at = o - static_cast<unsigned>(((wave * N + c) * 16 + (lane >> 2)) * ld * ES);
+      o = at < static_cast<unsigned>(k * ES) ? o : kBehind;
+    }
+    copy16(r, o, to + c * 1024);
+  }
+}
+
+// T: operand type, O: output type, TA / TB: layouts; a wave owns 32 TM rows x 64 channels, a workgroup WM x WN waves
 template <class T, class O, int TA, int TB, int TM, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P) {
-  constexpr int ES = MatIn<T>::ES;
-  constexpr int BM = WM * TM * 16, BN = WN * 64, BK = 128 / ES, WAVES = WM * WN;
-  constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
-  constexpr int IA = BM / 8 / WAVES, IB = BN / 8 / WAVES;               // copies a wave makes per step
-  static_assert(IA * 8 * WAVES == BM && IB * 8 * WAVES == BN, "a step's copies divide over the waves");
+  constexpr int ES = TileIn<T>::ES;
+  constexpr int BM = WM * TM * 32, BN = WN * 64, BK = 64 / ES, WAVES = WM * WN;
+  constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES;
+  constexpr int IA = BM / 16 / WAVES, IB = BN / 16 / WAVES;             // copies a wave makes per stage
+  static_assert(IA * 16 * WAVES == BM && IB * 16 * WAVES == BN, "a stage's copies divide over the waves");
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = lane_id(), wave = uni(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  const int i = lane & 15, q = lane >> 4;
+  const int i = lane & 31, h = lane >> 5;
 
   // workgroup -> tile: consecutive tiles on one XCD (hardware deals workgroups to the XCDs in turn), in groups of eight
   // tile rows, so that what an XCD works on at a time shares its operand panels in that XCD's L2
@@ -179,115 +213,143 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
   for (int c = 0; c < IB; ++c) offb[c] = tile_offset<TB, BN, ES>(wave * IB + c, lane, P.ldb);
   const int64_t rows_a = P.M - m0 < BM ? P.M - m0 : BM, rows_b = P.N - n0 < BN ? P.N - n0 : BN;
 
-  // Rows and k-rows behind the matrix lie behind the buffer's end and read as zeros; so do, by an offset of kBehind, the
-  // chunks of a K-contiguous row behind K (a chunk that K ends in is the operand's zero padding from there).  Columns of a
-  // K-strided operand behind M or N read what is there: their sums are not stored.
-  constexpr int CH = 16 / ES;                                           // values in 16 bytes
-  auto copy = [&](int step, int buf) {
-    const int64_t k0 = static_cast<int64_t>(step) * BK;
-    const int64_t left = P.K - k0 < BK ? P.K - k0 : BK;
-    char* dst = lds + buf * STAGE;
-    auto one = [&](auto layout, auto count, const void* base, int64_t ld, int64_t line0, int64_t lines, const unsigned* off, char* to) {
-      constexpr int L = decltype(layout)::value, n = decltype(count)::value;
-      const char* p = static_cast<const char*>(base) + (L == 0 ? line0 * ld + k0 : k0 * ld + line0) * ES;
-      const int64_t bytes = (L == 0 ? (lines - 1) * ld + (left + CH - 1) / CH * CH : (left - 1) * ld + (lines + CH - 1) / CH * CH) * ES;
-      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, static_cast<int>(bytes), kRsrcFlags);
-      if (L == 0 && left < BK) {
-#pragma unroll
-        for (int c = 0; c < n; ++c) {
-          // byte of the row that this lane's chunk starts at
-          const unsigned at = off[c] - static_cast<unsigned>(((wave * n + c) * 8 + (lane >> 3)) * ld * ES);
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(to + c * 1024), 16, at < left * ES ? off[c] : kBehind, 0, 0, 0);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < n; ++c) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(to + c * 1024), 16, off[c], 0, 0, 0);
-      }
-    };
-    one(std::integral_constant<int, TA>{}, std::integral_constant<int, IA>{}, P.a, P.lda, m0, rows_a, offa, dst + wave * IA * 1024);
-    one(std::integral_constant<int, TB>{}, std::integral_constant<int, IB>{}, P.b, P.ldb, n0, rows_b, offb, dst + A_BYTES + wave * IB * 1024);
+  // copy(place) requests the next stage into a place of the ring.  Rows and k-rows behind the matrix lie behind the buffer's
+  // end and read as zeros; so do, by an offset of kBehind, the chunks of a K-contiguous row behind K (a chunk that K ends in
+  // is the operand's zero padding from there), and all of a stage behind the last one, which is requested all the same so
+  // that a wave always has the same number of copies under way.  Columns of a K-strided operand behind M or N read what is
+  // there: their sums are not stored.
+  const int64_t step_a = (TA == 0 ? BK : BK * P.lda) * ES, step_b = (TB == 0 ? BK : BK * P.ldb) * ES;
+  const char* pa = static_cast<const char*>(P.a) + (TA == 0 ? m0 * P.lda : m0) * ES + s0 * step_a;
+  const char* pb = static_cast<const char*>(P.b) + (TB == 0 ? n0 * P.ldb : n0) * ES + s0 * step_b;
+  int todo = s1 - s0;                                                   // stages not yet requested, and the last one's part of BK
+  const int last_k = s1 < steps_all ? BK : static_cast<int>(P.K - static_cast<int64_t>(steps_all - 1) * BK);
+  typedef std::integral_constant<int, TA> LA;
+  typedef std::integral_constant<int, TB> LB;
+  const int whole_a = tile_bytes<TA, ES>(P.lda, rows_a, BK), whole_b = tile_bytes<TB, ES>(P.ldb, rows_b, BK);
+  auto copy = [&](auto whole, int place) {                              // whole: the stage is known to be a full one
+    char* ta = lds + place * STAGE + wave * IA * 1024;
+    char* tb = lds + place * STAGE + A_BYTES + wave * IB * 1024;
+    if constexpr (decltype(whole)::value) {
+      copy_whole<IA>(pa, whole_a, offa, ta);
+      copy_whole<IB>(pb, whole_b, offb, tb);
+    } else {
+      const int k = todo > 1 ? BK : todo == 1 ? last_k : 0;
+      copy_part<TA, IA, ES>(pa, P.lda, rows_a, k, offa, wave, lane, ta);
+      copy_part<TB, IB, ES>(pb, P.ldb, rows_b, k, offb, wave, lane, tb);
+    }
+    pa += step_a;
+    pb += step_b;
+    todo -= 1;
   };
 
-  f32x4 acc[TM][4];
-#pragma unroll
-  for (int tm = 0; tm < TM; ++tm) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) acc[tm][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  // Raw fragment of 16 operand rows (or columns), row i on lane (i, q).  One byte a value: chunks q and q + 4 of the row's
-  // eight; two: likewise, k = 8 q .. of each half; four: chunks 2 q and 2 q + 1, k = 8 q .. 8 q + 7.
-  const int at0 = ((ES == 4 ? 2 * q : q) ^ (i & 7)) << 4, at1 = at0 ^ (ES == 4 ? 16 : 64);
-  const int kk = i >> 2, pc = i & 3;                                    // K-strided, 16 bits: the lane fetches four columns of k-row 8 q + kk
-  const int f2 = (kk | (q & 1) << 2) << 5;
-  auto read = [&](auto layout, const char* base, int line, int rows, u4v (&out)[2]) {
+  // Raw fragment of 32 operand rows (or columns) from `line` on
+  const int sw = (i >> 2) & 3;
+  const int at0 = ((ES == 2 ? h : 2 * h) ^ sw) << 4, at1 = ((ES == 2 ? 2 + h : 2 * h + 1) ^ sw) << 4;
+  const int kk = (lane >> 2) & 3, pc = lane & 3, g16 = (lane >> 4) & 1;  // K-strided, 16 bits: the lane fetches four columns of k-row 8 h + kk
+  auto read = [&](auto layout, const char* base, int line, int rows) -> u8v {
     constexpr int L = decltype(layout)::value;
     if constexpr (L == 0) {
-      const char* p = base + (line + i) * 128;
-      out[0] = *reinterpret_cast<const u4v*>(p + at0);
-      out[1] = *reinterpret_cast<const u4v*>(p + at1);
+      const char* p = base + (line + i) * 64;
+      return __builtin_shufflevector(*reinterpret_cast<const u4v*>(p + at0), *reinterpret_cast<const u4v*>(p + at1), 0, 1, 2, 3, 4, 5, 6, 7);
     } else if constexpr (ES == 2) {
-      const char* p = base + (8 * q + kk) * rows * 2 + ((line * 2 + ((pc >> 1) << 4)) ^ f2) + (pc & 1) * 8;
+      const char* p = base + (8 * h + kk) * rows * 2 + ((line * 2 + g16 * 32 + pc * 8) ^ (kk << 6));
+      u4v out[2];
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (32 * s) * rows * 2));
-        const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (32 * s + 4) * rows * 2));
+        const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (16 * s) * rows * 2));
+        const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (16 * s + 4) * rows * 2));
         out[s] = __builtin_bit_cast(u4v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       }
+      return __builtin_shufflevector(out[0], out[1], 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      const char* p = base + 8 * q * rows * 4 + (((line + i) * 4) ^ (q << 6));
+      const char* p = base + 8 * h * rows * 4 + (((line + i) * 4) ^ (h << 7));
+      u8v out;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) out[e >> 2][e & 3] = *reinterpret_cast<const uint32_t*>(p + e * rows * 4);
+      for (int e = 0; e < 8; ++e) out[e] = *reinterpret_cast<const uint32_t*>(p + e * rows * 4);
+      return out;
+    }
+  };
+  auto read_a = [&](int place, int t) { return read(LA{}, lds + place * STAGE, (wm * TM + t) * 32, BM); };
+  auto read_b = [&](int place, int t) { return read(LB{}, lds + place * STAGE + A_BYTES, wn * 64 + 32 * t, BN); };
+  f32x16 acc[TM][2];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[t][0][e] = acc[t][1][e] = 0.f;
+  }
+  // All but the newest `stages` stages of this wave's copies have landed and its LDS reads are done; then everyone's.
+  auto meet = [&](auto stages) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(stages)::value * (IA + IB)) : "memory");
+  };
+  // One iteration: the stage at `place` lies in fa and b.  Each row tile's products are followed by the read of the same tile
+  // of the next stage; the stage after the ring's last is requested into `place`, which every wave has read before the
+  // barrier -- behind the first products, so that the reads before it and the barrier find the matrix pipe busy.
+  u8v fa[TM];
+  auto turn = [&](auto whole, int place, const u8v (&b)[2], u8v (&b_next)[2]) {
+    const int next = (place + 1) & (kStages - 1);
+    const typename TileIn<T>::Frag fb[2] = {TileIn<T>::prep(b[0]), TileIn<T>::prep(b[1])};
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+      TileIn<T>::mul(fb, TileIn<T>::prep(fa[t]), acc[t]);
+      if (t == 0) {
+        __builtin_amdgcn_sched_barrier(0);
+        meet(std::integral_constant<int, kStages - 2>{});
+        b_next[0] = read_b(next, 0);
+        b_next[1] = read_b(next, 1);
+      }
+      fa[t] = read_a(next, t);
+      if (t == 0) copy(whole, place);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  if (s0 < s1) copy(s0, 0);
-  for (int step = s0; step < s1; ++step) {
-    const int buf = (step - s0) & 1;
-    __builtin_amdgcn_s_waitcnt(0x0f70);                                // vmcnt(0): this wave's copies have landed
-    __syncthreads();                                                   // everyone's have; nobody still reads the other buffer
-    if (step + 1 < s1) copy(step + 1, buf ^ 1);
-    const char* sa = lds + buf * STAGE;
-    const char* sb = sa + A_BYTES;
-    typename MatIn<T>::Frag fb[4];
+  u8v even[2], odd[2];
+  for (int s = 0; s < kStages; ++s) copy(std::false_type{}, s);
+  meet(std::integral_constant<int, kStages - 1>{});
+  even[0] = read_b(0, 0);
+  even[1] = read_b(0, 1);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      u4v raw[2];
-      read(std::integral_constant<int, TB>{}, sb, wn * 64 + 16 * t, BN, raw);
-      fb[t] = MatIn<T>::prep(raw);
-    }
-#pragma unroll
-    for (int tm = 0; tm < TM; ++tm) {
-      u4v raw[2];
-      read(std::integral_constant<int, TA>{}, sa, wm * TM * 16 + tm * 16, BM, raw);
-      MatIn<T>::mul(fb, MatIn<T>::prep(raw), acc[tm]);
-    }
+  for (int t = 0; t < TM; ++t) fa[t] = read_a(0, t);
+  int place = 0, step = s0;
+  for (; todo > 2; step += 2) {                                         // full stages ahead: no branch in the loop
+    turn(std::true_type{}, place, even, odd);
+    turn(std::true_type{}, (place + 1) & (kStages - 1), odd, even);
+    place = (place + 2) & (kStages - 1);
   }
+  for (; step + 1 < s1; step += 2) {
+    turn(std::false_type{}, place, even, odd);
+    turn(std::false_type{}, (place + 1) & (kStages - 1), odd, even);
+    place = (place + 2) & (kStages - 1);
+  }
+  if (step < s1) turn(std::false_type{}, place, even, odd);
 
-  // Epilogue, through LDS (the operand buffers are free): a wave writes its sums as rows of 64 channels, up to 64 rows at a
-  // time, and takes them back eight rows by eight channels a lane, so that a store fills whole lines and the code is one
-  // rolled loop.  Lane (i, q) holds row i of each 16 and, of fragment t, matrix rows 4 q .. 4 q + 3.  16-byte unit u of row
-  // r lies at u ^ (r & 15).  A wave reads only what it wrote.
-  constexpr int PASS = TM < 4 ? TM : 4;
-  __syncthreads();
-  char* mine = lds + wave * (PASS * 16 * 256);
-  const int64_t mw = m0 + wm * TM * 16, n = n0 + wn * 64 + 8 * (lane & 7);
+  // Epilogue, through LDS (when all copies have landed and nobody reads operands any more): a wave writes its sums as rows of
+  // 64 channels, up to 64 rows at a time, and takes them back eight rows by eight channels a lane, so that a store fills
+  // whole lines and the code is one rolled loop.  Lane (i, h) holds row i of each 32 and, of a tile's 32 channels, 8 g + 4 h ..
+  // + 3 in the sums 4 g .. 4 g + 3.  16-byte unit u of row r lies at u ^ (r & 15).  A wave reads only what it wrote.
+  constexpr int PASS = TM < 2 ? TM : 2;
+  meet(std::integral_constant<int, 0>{});
+  char* mine = lds + wave * (PASS * 32 * 256);
+  const int64_t mw = m0 + wm * TM * 32, n = n0 + wn * 64 + 8 * (lane & 7);
   float bs[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) bs[e] = (ES == 1 && n + e < P.N) ? P.b_scale[n + e] : 1.f;
 #pragma unroll
   for (int p = 0; p < TM / PASS; ++p) {
 #pragma unroll
-    for (int tm = 0; tm < PASS; ++tm) {
+    for (int t = 0; t < PASS; ++t) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        *reinterpret_cast<f32x4*>(mine + (tm * 16 + i) * 256 + (((4 * t + q) ^ i) << 4)) = acc[p * PASS + tm][t];
+      for (int u = 0; u < 16; ++u) {                                    // tile u >> 3, group (u >> 1) & 3 ... unit 8 tile + 2 g + h
+        if (u & 1) continue;
+        const f32x16& c = acc[p * PASS + t][u >> 3];
+        const int g = (u >> 1) & 3;
+        *reinterpret_cast<f32x4*>(mine + (t * 32 + i) * 256 + (((u + h) ^ (i & 15)) << 4)) = f32x4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]};
       }
     }
 #pragma unroll 1
-    for (int r0 = 0; r0 < PASS * 16; r0 += 8) {
+    for (int r0 = 0; r0 < PASS * 32; r0 += 8) {
       const int r = r0 + (lane >> 3), u = 2 * (lane & 7);
-      const int64_t m = mw + p * PASS * 16 + r;
+      const int64_t m = mw + p * PASS * 32 + r;
       const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + r * 256 + ((u ^ (r & 15)) << 4));
       const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((u + 1) ^ (r & 15)) << 4));
       if (m < P.M && n < P.N) {
@@ -310,8 +372,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
 
 template <class T, class O, int TA, int TB, int TM, int WM, int WN>
 int tile_launch(const MatParams& P, hipStream_t s) {
-  constexpr int BM = WM * TM * 16, BN = WN * 64;
-  constexpr int LDS = 2 * (BM + BN) * 128;
+  constexpr int BM = WM * TM * 32, BN = WN * 64;
+  constexpr int LDS = kStages * (BM + BN) * 64;
   const int64_t tiles = ((P.M + BM - 1) / BM) * ((P.N + BN - 1) / BN);
   // 32-bit offsets inside a tile's lines, 31-bit tile count
   const int64_t far = 4 * 256 * (P.lda > P.ldb ? P.lda : P.ldb);
@@ -325,10 +387,10 @@ int tile_launch(const MatParams& P, hipStream_t s) {
 
 template <class T, class O, int TA, int TB>
 int tile_size(const MatParams& P, int tile, hipStream_t s) {
-  if (tile == 0) return tile_launch<T, O, TA, TB, 8, 2, 4>(P, s);
-  if (tile == 1) return tile_launch<T, O, TA, TB, 4, 2, 2>(P, s);
+  if (tile == 0) return tile_launch<T, O, TA, TB, 4, 2, 4>(P, s);
+  if (tile == 1) return tile_launch<T, O, TA, TB, 2, 2, 2>(P, s);
   if constexpr (TA == 0) {
-    if (tile == 2) return tile_launch<T, O, TA, TB, 2, 2, 2>(P, s);
+    if (tile == 2) return tile_launch<T, O, TA, TB, 1, 2, 2>(P, s);
   }
   return DGCN_E_MODE;
 }
