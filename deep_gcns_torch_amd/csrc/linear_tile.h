@@ -143,16 +143,23 @@ __device__ __forceinline__ int tile_bytes(int64_t ld, int64_t lines, int k) {
   return static_cast<int>((T == 0 ? (lines - 1) * ld + (k + CH - 1) / CH * CH : (k - 1) * ld + (lines + CH - 1) / CH * CH) * ES);
 }
 
-// 16 bytes a lane from memory to `to` + 16 lane in LDS (the host's pass of the compiler knows no copies of this width)
-__device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t r, unsigned off, char* to) {
-#ifdef __HIP_DEVICE_COMPILE__
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)to, 16, off, 0, 0, 0);
-#endif
+// A raw buffer of `bytes` bytes at p, as its four scalar words
+__device__ __forceinline__ i4v tile_buffer(const char* p, int bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  return i4v{static_cast<int>(at), static_cast<int>(at >> 32) & 0xffff, bytes, static_cast<int>(kRsrcFlags)};
+}
+
+// 16 bytes a lane from a buffer to LDS, `to` + 16 lane.  Written out because the compiler, which cannot tell which LDS bytes a
+// transposing read takes, waits for every copy before each of them (measured on dw of 16384 x 4096 x 8192: 1.14 ms against 0.9);
+// the kernel counts its copies itself (meet).  Nothing is returned in registers; the waits that the instruction needs behind
+// writes of m0 and of its scalar operands are in the text.
+__device__ __forceinline__ void copy16(i4v buffer, unsigned off, unsigned to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(buffer), "s"(to) : "memory", "m0");
 }
 
 template <int N>
-__device__ __forceinline__ void copy_whole(const char* p, int bytes, const unsigned (&off)[N], char* to) {
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, bytes, kRsrcFlags);
+__device__ __forceinline__ void copy_whole(const char* p, int bytes, const unsigned (&off)[N], unsigned to) {
+  const i4v r = tile_buffer(p, bytes);
 #pragma unroll
   for (int c = 0; c < N; ++c) copy16(r, off[c], to + c * 1024);
 }
@@ -160,9 +167,8 @@ __device__ __forceinline__ void copy_whole(const char* p, int bytes, const unsig
 // any stage, k values of the reduction in it (none: zeros everywhere, and p is not read)
 template <int T, int N, int ES>
 __device__ __forceinline__ void copy_part(const char* p, int64_t ld, int64_t lines, int k, const unsigned (&off)[N], int wave,
-                                          int lane, char* to) {
-  const int bytes = k > 0 ? tile_bytes<T, ES>(ld, lines, k) : 0;
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, bytes, kRsrcFlags);
+                                          int lane, unsigned to) {
+  const i4v r = tile_buffer(p, k > 0 ? tile_bytes<T, ES>(ld, lines, k) : 0);
 #pragma unroll
   for (int c = 0; c < N; ++c) {
     unsigned o = off[c];
@@ -226,9 +232,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
   typedef std::integral_constant<int, TA> LA;
   typedef std::integral_constant<int, TB> LB;
   const int whole_a = tile_bytes<TA, ES>(P.lda, rows_a, BK), whole_b = tile_bytes<TB, ES>(P.ldb, rows_b, BK);
+  const unsigned lds_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_void*)lds));
   auto copy = [&](auto whole, int place) {                              // whole: the stage is known to be a full one
-    char* ta = lds + place * STAGE + wave * IA * 1024;
-    char* tb = lds + place * STAGE + A_BYTES + wave * IB * 1024;
+    const unsigned ta = lds_at + place * STAGE + wave * IA * 1024, tb = lds_at + place * STAGE + A_BYTES + wave * IB * 1024;
     if constexpr (decltype(whole)::value) {
       copy_whole<IA>(pa, whole_a, offa, ta);
       copy_whole<IB>(pb, whole_b, offb, tb);
