@@ -45,8 +45,8 @@ struct MatPlan {
 // traffic take (`work`, times the workgroups a CU holds), and at least the latency of the copies behind it; a split
 // writes and reads fp32 partial sums and launches once more.
 inline MatPlan mat_plan(int64_t M, int64_t N, int64_t K, int type, int ta) {
-  struct { int bm, bn, held; double work; } tiles[3] = {{256, 256, 1, 1250.}, {128, 128, 2, 380.}, {64, 128, 3, 260.}};
-  const int64_t bk = type == DGCN_T_E4M3 ? 64 : type == DGCN_T_F32 ? 16 : 32, steps = (K + bk - 1) / bk;
+  struct { int bm, bn, held; double work; } tiles[3] = {{256, 256, 1, 2500.}, {128, 128, 2, 760.}, {64, 128, 3, 520.}};
+  const int64_t bk = type == DGCN_T_E4M3 ? 128 : type == DGCN_T_F32 ? 32 : 64, steps = (K + bk - 1) / bk;
   const double cus = num_cus();
   MatPlan best = {0, 1};
   double least = 1e300;
@@ -55,7 +55,7 @@ inline MatPlan mat_plan(int64_t M, int64_t N, int64_t K, int type, int ta) {
     for (int sp = 1; sp <= 512 && sp <= steps; sp *= 2) {
       const double wgs = wgs1 * sp, per_cu = ceil(wgs / cus);
       const double held = per_cu < tiles[t].held ? per_cu : tiles[t].held;
-      const double step = held * tiles[t].work > 600. ? held * tiles[t].work : 600.;
+      const double step = held * tiles[t].work > 1200. ? held * tiles[t].work : 1200.;
       double c = ceil(per_cu / tiles[t].held) * ((steps + sp - 1) / sp * step + 5000.);
       if (sp > 1) c += 8. * M * N * sp / 2000. + 10000.;
       if (c < least) { least = c; best = {t, sp}; }

@@ -1,9 +1,11 @@
 // The tiled product on the matrix pipe: BM x BN tiles, fp32 sums in 32 x 32 matrix instructions, operands copied straight
-// from memory into a ring of four LDS stages of 64 bytes of the reduction.
+// from memory into two LDS stages of 128 bytes of the reduction (whole cache lines of a K-contiguous row: with four stages of
+// 64 bytes every line was fetched twice).
 //
-// Bound by the matrix pipe (large products) or by HBM (long thin ones).  An iteration computes on fragments that lie in
-// registers already, while the next stage's fragments are read from LDS and the stage after the ring's last is requested from
-// memory: the matrix instructions wait for neither, and a barrier costs them the time it takes to meet.
+// Bound by the matrix pipe and its power (large products) or by HBM (long thin ones).  A stage is computed in two halves.
+// The fragments of a half lie in registers already while the next half's are read from LDS, and the stage after next is
+// requested as soon as every wave has read the second half of this one: the matrix instructions wait for neither, and a
+// stage costs one barrier.
 #pragma once
 
 #include <type_traits>
@@ -25,11 +27,11 @@ __device__ __forceinline__ u4v half0(u8v r) { return __builtin_shufflevector(r, 
 __device__ __forceinline__ u4v half1(u8v r) { return __builtin_shufflevector(r, r, 4, 5, 6, 7); }
 
 // What a wave does with the fragments of a stage: a raw fragment is two 16-byte units of an operand row (lane l: row l & 31,
-// h = l >> 5), prep() makes of it what the matrix instructions take, mul() adds one tile's products.
+// h = l >> 5) of a half stage's 64 bytes, prep() makes of it what the matrix instructions take, mul() adds one tile's products.
 template <class T> struct TileIn;
 
 template <class T>
-struct TileIn16 {                                          // units h and 2 + h: k = 8 h .. of each half of the stage's 32
+struct TileIn16 {                                          // units h and 2 + h: k = 8 h .. of each 16 of the 32
   static constexpr int ES = 2;
   struct Frag { u4v r[2]; };
   static __device__ __forceinline__ Frag prep(u8v r) { return Frag{{half0(r), half1(r)}}; }
@@ -51,7 +53,7 @@ struct TileIn16 {                                          // units h and 2 + h:
 template <> struct TileIn<__bf16> : TileIn16<__bf16> {};
 template <> struct TileIn<_Float16> : TileIn16<_Float16> {};
 
-// fp32 (units 2 h and 2 h + 1: k = 8 h .. 8 h + 7 of the stage's 16): three bf16 parts that add up to the value bit for bit,
+// fp32 (units 2 h and 2 h + 1: k = 8 h .. 8 h + 7 of the 16): three bf16 parts that add up to the value bit for bit,
 // and the six products of parts down to 2^-16 of the largest (bf16x6.h: off by at most 3 2^-24 |a b|)
 template <> struct TileIn<float> {
   static constexpr int ES = 4;
@@ -78,7 +80,7 @@ template <> struct TileIn<float> {
   }
 };
 
-// e4m3 for a 16-bit result (units 2 h and 2 h + 1: 32 of the stage's 64 values): one instruction at twice the 16-bit rate, its
+// e4m3 for a 16-bit result (units 2 h and 2 h + 1: 32 of the 64 values): one instruction at twice the 16-bit rate, its
 // block scales held at 2^0.  It aligns the products of eight neighbouring k to the largest one's exponent and drops what lies
 // more than 13 bits below it (measured, bit by bit), so a sum is off by up to 7 2^-13 of the largest product of each eight:
 // 6e-5 of the result's root mean square over normal rows, an order below a bf16 half step and under half of an fp16 one.
@@ -117,17 +119,16 @@ template <> struct TileIn<WideE4m3> {
 
 constexpr unsigned kRsrcFlags = 0x00027000;               // raw 32-bit buffer; a load behind its end gives zeros
 constexpr unsigned kBehind = 0x80000000u;                 // an offset behind any buffer here (at most 2^31 bytes)
-constexpr int kStages = 4;
 
 // Which chunk (16 bytes) of an operand tile a 16-byte unit of an LDS stage holds.
-//   K-contiguous, R rows of 64 bytes: unit u of row r holds the row's chunk u ^ (bits 3, 2 of r)
+//   K-contiguous, R rows of 128 bytes: unit u of row r holds the row's chunk u ^ (bits 3, 2, 1 of r)
 //   K-strided, k-rows of R values: unit u of k-row k holds chunk u ^ 4 (k & 3) in 16 bits, u ^ 8 (bit 3 of k) in 32
 // In all, lanes that read together fall on different banks.
 template <int T, int R, int ES>
 __device__ __forceinline__ unsigned tile_offset(int inst, int lane, int64_t ld) {
   if constexpr (T == 0) {
-    const int row = inst * 16 + (lane >> 2);
-    return static_cast<unsigned>(row * ld * ES) + (((lane & 3) ^ ((row >> 2) & 3)) << 4);
+    const int row = inst * 8 + (lane >> 3);
+    return static_cast<unsigned>(row * ld * ES) + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
   } else {
     constexpr int UNITS = R * ES / 16;
     const int k = inst * (64 / UNITS) + lane / UNITS;
@@ -146,15 +147,15 @@ __device__ __forceinline__ int tile_bytes(int64_t ld, int64_t lines, int k) {
 // A raw buffer of `bytes` bytes at p, as its four scalar words
 __device__ __forceinline__ i4v tile_buffer(const char* p, int bytes) {
   const uint64_t at = reinterpret_cast<uint64_t>(p);
-  return i4v{static_cast<int>(at), static_cast<int>(at >> 32) & 0xffff, bytes, static_cast<int>(kRsrcFlags)};
+  return i4v{uni(static_cast<int>(at)), uni(static_cast<int>(at >> 32) & 0xffff), uni(bytes), static_cast<int>(kRsrcFlags)};
 }
 
 // 16 bytes a lane from a buffer to LDS, `to` + 16 lane.  Written out because the compiler, which cannot tell which LDS bytes a
 // transposing read takes, waits for every copy before each of them (measured on dw of 16384 x 4096 x 8192: 1.14 ms against 0.9);
 // the kernel counts its copies itself (meet).  Nothing is returned in registers; the waits that the instruction needs behind
-// writes of m0 and of its scalar operands are in the text.
+// writes of m0 (which nothing else here uses) and of its scalar operands are in the text.
 __device__ __forceinline__ void copy16(i4v buffer, unsigned off, unsigned to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(buffer), "s"(to) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(buffer), "s"(uni(static_cast<int>(to))) : "memory");
 }
 
 template <int N>
@@ -174,7 +175,7 @@ __device__ __forceinline__ void copy_part(const char* p, int64_t ld, int64_t lin
     unsigned o = off[c];
     if (T == 0) {
       // byte of the row that this lane's chunk starts at
-      const unsigned at = o - static_cast<unsigned>(((wave * N + c) * 16 + (lane >> 2)) * ld * ES);
+      const unsigned at = o - static_cast<unsigned>(((wave * N + c) * 8 + (lane >> 3)) * ld * ES);
       o = at < static_cast<unsigned>(k * ES) ? o : kBehind;
     }
     copy16(r, o, to + c * 1024);
@@ -185,10 +186,10 @@ __device__ __forceinline__ void copy_part(const char* p, int64_t ld, int64_t lin
 template <class T, class O, int TA, int TB, int TM, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P) {
   constexpr int ES = TileIn<T>::ES;
-  constexpr int BM = WM * TM * 32, BN = WN * 64, BK = 64 / ES, WAVES = WM * WN;
-  constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES;
-  constexpr int IA = BM / 16 / WAVES, IB = BN / 16 / WAVES;             // copies a wave makes per stage
-  static_assert(IA * 16 * WAVES == BM && IB * 16 * WAVES == BN, "a stage's copies divide over the waves");
+  constexpr int BM = WM * TM * 32, BN = WN * 64, BK = 128 / ES, WAVES = WM * WN;
+  constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
+  constexpr int IA = BM / 8 / WAVES, IB = BN / 8 / WAVES;               // copies a wave makes per stage
+  static_assert(IA * 8 * WAVES == BM && IB * 8 * WAVES == BN, "a stage's copies divide over the waves");
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = lane_id(), wave = uni(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -219,10 +220,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
   for (int c = 0; c < IB; ++c) offb[c] = tile_offset<TB, BN, ES>(wave * IB + c, lane, P.ldb);
   const int64_t rows_a = P.M - m0 < BM ? P.M - m0 : BM, rows_b = P.N - n0 < BN ? P.N - n0 : BN;
 
-  // copy(place) requests the next stage into a place of the ring.  Rows and k-rows behind the matrix lie behind the buffer's
+  // copy(place) requests the next stage into one of the two places.  Rows and k-rows behind the matrix lie behind the buffer's
   // end and read as zeros; so do, by an offset of kBehind, the chunks of a K-contiguous row behind K (a chunk that K ends in
   // is the operand's zero padding from there), and all of a stage behind the last one, which is requested all the same so
-  // that a wave always has the same number of copies under way.  Columns of a K-strided operand behind M or N read what is
+  // that a wave always has the same number of copies under way.   Columns of a K-strided operand behind M or N read what is
   // there: their sums are not stored.
   const int64_t step_a = (TA == 0 ? BK : BK * P.lda) * ES, step_b = (TB == 0 ? BK : BK * P.ldb) * ES;
   const char* pa = static_cast<const char*>(P.a) + (TA == 0 ? m0 * P.lda : m0) * ES + s0 * step_a;
@@ -248,86 +249,89 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
     todo -= 1;
   };
 
-  // Raw fragment of 32 operand rows (or columns) from `line` on
-  const int sw = (i >> 2) & 3;
+  // Raw fragment of 32 operand rows (or columns) from `line` on, of one half of the stage
+  const int sw = (i >> 1) & 7;
   const int at0 = ((ES == 2 ? h : 2 * h) ^ sw) << 4, at1 = ((ES == 2 ? 2 + h : 2 * h + 1) ^ sw) << 4;
   const int kk = (lane >> 2) & 3, pc = lane & 3, g16 = (lane >> 4) & 1;  // K-strided, 16 bits: the lane fetches four columns of k-row 8 h + kk
-  auto read = [&](auto layout, const char* base, int line, int rows) -> u8v {
+  auto read = [&](auto layout, const char* base, int line, int rows, int half) -> u8v {
     constexpr int L = decltype(layout)::value;
     if constexpr (L == 0) {
-      const char* p = base + (line + i) * 64;
-      return __builtin_shufflevector(*reinterpret_cast<const u4v*>(p + at0), *reinterpret_cast<const u4v*>(p + at1), 0, 1, 2, 3, 4, 5, 6, 7);
+      const char* p = base + (line + i) * 128;
+      return __builtin_shufflevector(*reinterpret_cast<const u4v*>(p + (at0 ^ (64 * half))), *reinterpret_cast<const u4v*>(p + (at1 ^ (64 * half))),
+                                     0, 1, 2, 3, 4, 5, 6, 7);
     } else if constexpr (ES == 2) {
       const char* p = base + (8 * h + kk) * rows * 2 + ((line * 2 + g16 * 32 + pc * 8) ^ (kk << 6));
       u4v out[2];
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (16 * s) * rows * 2));
-        const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (16 * s + 4) * rows * 2));
+        const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (32 * half + 16 * s) * rows * 2));
+        const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (32 * half + 16 * s + 4) * rows * 2));
         out[s] = __builtin_bit_cast(u4v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       }
       return __builtin_shufflevector(out[0], out[1], 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      const char* p = base + 8 * h * rows * 4 + (((line + i) * 4) ^ (h << 7));
+      const char* p = base + (16 * half + 8 * h) * rows * 4 + (((line + i) * 4) ^ (h << 7));
       u8v out;
 #pragma unroll
       for (int e = 0; e < 8; ++e) out[e] = *reinterpret_cast<const uint32_t*>(p + e * rows * 4);
       return out;
     }
   };
-  auto read_a = [&](int place, int t) { return read(LA{}, lds + place * STAGE, (wm * TM + t) * 32, BM); };
-  auto read_b = [&](int place, int t) { return read(LB{}, lds + place * STAGE + A_BYTES, wn * 64 + 32 * t, BN); };
+  auto read_a = [&](int place, int half, int t) { return read(LA{}, lds + place * STAGE, (wm * TM + t) * 32, BM, half); };
+  auto read_b = [&](int place, int half, int t) { return read(LB{}, lds + place * STAGE + A_BYTES, wn * 64 + 32 * t, BN, half); };
   f32x16 acc[TM][2];
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[t][0][e] = acc[t][1][e] = 0.f;
   }
-  // All but the newest `stages` stages of this wave's copies have landed and its LDS reads are done; then everyone's.
-  auto meet = [&](auto stages) {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(stages)::value * (IA + IB)) : "memory");
+  // All but the newest `copies` of this wave's copies have landed and its LDS reads are done; then everyone's.
+  auto meet = [&](auto copies) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(copies)::value) : "memory");
   };
-  // One iteration: the stage at `place` lies in fa and b.  Each row tile's products are followed by the read of the same tile
-  // of the next stage; the stage after the ring's last is requested into `place`, which every wave has read before the
-  // barrier -- behind the first products, so that the reads before it and the barrier find the matrix pipe busy.
-  u8v fa[TM];
-  auto turn = [&](auto whole, int place, const u8v (&b)[2], u8v (&b_next)[2]) {
-    const int next = (place + 1) & (kStages - 1);
+  // A half: its fragments lie in fa and b.  Each row tile's products are followed by the read of the same tile of the next
+  // half.  Before the second half's reads, of the next stage, the waves meet -- behind the first products, so that the
+  // barrier finds the matrix pipe busy -- and behind them the stage after next is requested into the place of this one.
+  u8v fa[TM], b0[2], b1[2];
+  auto turn = [&](auto half, auto whole, int place, const u8v (&b)[2], u8v (&b_next)[2]) {
+    constexpr int H = decltype(half)::value;
+    const int from = place ^ H;
     const typename TileIn<T>::Frag fb[2] = {TileIn<T>::prep(b[0]), TileIn<T>::prep(b[1])};
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
       TileIn<T>::mul(fb, TileIn<T>::prep(fa[t]), acc[t]);
       if (t == 0) {
-        __builtin_amdgcn_sched_barrier(0);
-        meet(std::integral_constant<int, kStages - 2>{});
-        b_next[0] = read_b(next, 0);
-        b_next[1] = read_b(next, 1);
+        if constexpr (H == 1) {
+          __builtin_amdgcn_sched_barrier(0);
+          meet(std::integral_constant<int, 0>{});
+        }
+        b_next[0] = read_b(from, H ^ 1, 0);
+        b_next[1] = read_b(from, H ^ 1, 1);
       }
-      fa[t] = read_a(next, t);
-      if (t == 0) copy(whole, place);
+      fa[t] = read_a(from, H ^ 1, t);
+      if (H == 1 && t == (TM > 1 ? 1 : 0)) copy(whole, place);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  typedef std::integral_constant<int, 0> H0;
+  typedef std::integral_constant<int, 1> H1;
 
-  u8v even[2], odd[2];
-  for (int s = 0; s < kStages; ++s) copy(std::false_type{}, s);
-  meet(std::integral_constant<int, kStages - 1>{});
-  even[0] = read_b(0, 0);
-  even[1] = read_b(0, 1);
+  copy(std::false_type{}, 0);
+  copy(std::false_type{}, 1);
+  meet(std::integral_constant<int, IA + IB>{});
+  b0[0] = read_b(0, 0, 0);
+  b0[1] = read_b(0, 0, 1);
 #pragma unroll
-  for (int t = 0; t < TM; ++t) fa[t] = read_a(0, t);
+  for (int t = 0; t < TM; ++t) fa[t] = read_a(0, 0, t);
   int place = 0, step = s0;
-  for (; todo > 2; step += 2) {                                         // full stages ahead: no branch in the loop
-    turn(std::true_type{}, place, even, odd);
-    turn(std::true_type{}, (place + 1) & (kStages - 1), odd, even);
-    place = (place + 2) & (kStages - 1);
+  for (; todo > 1; ++step, place ^= 1) {                                // full stages ahead: no selection in the loop
+    turn(H0{}, std::true_type{}, place, b0, b1);
+    turn(H1{}, std::true_type{}, place, b1, b0);
   }
-  for (; step + 1 < s1; step += 2) {
-    turn(std::false_type{}, place, even, odd);
-    turn(std::false_type{}, (place + 1) & (kStages - 1), odd, even);
-    place = (place + 2) & (kStages - 1);
+  for (; step < s1; ++step, place ^= 1) {
+    turn(H0{}, std::false_type{}, place, b0, b1);
+    turn(H1{}, std::false_type{}, place, b1, b0);
   }
-  if (step < s1) turn(std::false_type{}, place, even, odd);
 
   // Epilogue, through LDS (when all copies have landed and nobody reads operands any more): a wave writes its sums as rows of
   // 64 channels, up to 64 rows at a time, and takes them back eight rows by eight channels a lane, so that a store fills
@@ -379,7 +383,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
 template <class T, class O, int TA, int TB, int TM, int WM, int WN>
 int tile_launch(const MatParams& P, hipStream_t s) {
   constexpr int BM = WM * TM * 32, BN = WN * 64;
-  constexpr int LDS = kStages * (BM + BN) * 64;
+  constexpr int LDS = 2 * (BM + BN) * 128;
   const int64_t tiles = ((P.M + BM - 1) / BM) * ((P.N + BN - 1) / BN);
   // 32-bit offsets inside a tile's lines, 31-bit tile count
   const int64_t far = 4 * 256 * (P.lda > P.ldb ? P.lda : P.ldb);
