@@ -13,25 +13,41 @@
 namespace dgcn {
 namespace {
 
-// the epilogue of a product whose reduction was split: the partial sums are added in split order
+// The epilogue of a product whose reduction was split: four channels an item, 256 / segs items a workgroup; `segs` threads of
+// an item add every segs-th partial sum and meet in LDS, in a fixed order.  (One thread an item, which a 256 x 128 result with
+// 128 partial sums was until then, took 71 us: 128 loads one behind the other on 32 workgroups.)
 template <class O>
-__global__ __launch_bounds__(256) void split_join_kernel(const MatParams P) {
-  const int64_t per = (P.N + 3) / 4, total = P.M * per;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; it < total; it += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t m = it / per, n = (it - m * per) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+__global__ __launch_bounds__(256) void split_join_kernel(const MatParams P, int segs) {
+  __shared__ f32x4 red[256];
+  const int items = 256 / segs, mine = threadIdx.x % items, seg = threadIdx.x / items;
+  const int64_t per = (P.N + 3) / 4, total = P.M * per, it = static_cast<int64_t>(blockIdx.x) * items + mine;
+  const int64_t m = it / per, n = (it - m * per) * 4, size = P.M * P.N;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (it < total) {
     const float* p = P.part + m * P.N + n;
-    for (int s = 0; s < P.splits; ++s, p += P.M * P.N) {
+    const bool whole = n + 4 <= P.N;
+    auto load = [&](int s) {
       float t[4];
-      if (n + 4 <= P.N) {
-        load4(p, t);
+      if (whole) {
+        load4(p + s * size, t);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) t[j] = n + j < P.N ? p[j] : 0.f;
+        for (int j = 0; j < 4; ++j) t[j] = n + j < P.N ? p[s * size + j] : 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += t[j];
+      return f32x4{t[0], t[1], t[2], t[3]};
+    };
+    int s = seg;
+    for (; s + 3 * segs < P.splits; s += 4 * segs) {
+      const f32x4 a = load(s), b = load(s + segs), c = load(s + 2 * segs), d = load(s + 3 * segs);
+      sum += (a + b) + (c + d);
     }
+    for (; s < P.splits; s += segs) sum += load(s);
+  }
+  red[threadIdx.x] = sum;
+  __syncthreads();
+  if (seg == 0 && it < total) {
+    for (int g = 1; g < segs; ++g) sum += red[g * items + mine];
+    float v[4] = {sum[0], sum[1], sum[2], sum[3]};
     mat_epilogue<O, 4>(P, m, n, v);
   }
 }
@@ -41,24 +57,32 @@ struct MatPlan {
   int splits;
 };
 
-// Tile and split by the cost of the alternatives, in cycles of a CU: a workgroup's step takes what its matrix instructions and LDS
-// traffic take (`work`, times the workgroups a CU holds), and at least the latency of the copies behind it; a split
-// writes and reads fp32 partial sums and launches once more.
+// Tile and split by what the alternatives cost, in us.  A CU's workgroups take `work` for each step (128 bytes of the
+// reduction) of each of them, and a step takes at least `lag` however few they are; a round of workgroups ends in an epilogue;
+// a split writes and reads fp32 partial sums (from the caches: 8 TB/s) and launches once more.  The constants are fits to
+// measured times, bf16 and fp16 | e4m3 | fp32: 4096^3 (bf16) takes 117 / 156 / 210 us by tiles of 256 / 128 / 64 rows,
+// 1024 x 4096 x 4096 55 (split by four) / 48 / 43, 66,880 x 294 x 192 41 / 30 / 29, 512 x 512 x 40,000 51 / 47 / -- split by 32 / 16.
+struct TileCost {
+  int bm, bn, held;      // rows, channels, workgroups a CU holds
+  double work, lag, end;
+};
+constexpr TileCost kCost16[3] = {{256, 256, 1, 1.55, 1.55, 8.}, {128, 128, 2, 0.55, 0.65, 4.}, {64, 128, 3, 0.30, 0.50, 3.}};
+constexpr TileCost kCost32[3] = {{256, 256, 1, 5.0, 5.0, 12.}, {128, 128, 2, 1.4, 1.6, 5.}, {64, 128, 3, 0.8, 1.0, 4.}};
+
 inline MatPlan mat_plan(int64_t M, int64_t N, int64_t K, int type, int ta) {
-  struct { int bm, bn, held; double work; } tiles[3] = {{256, 256, 1, 2500.}, {128, 128, 2, 760.}, {64, 128, 3, 520.}};
+  const TileCost* cost = type == DGCN_T_F32 ? kCost32 : kCost16;
   const int64_t bk = type == DGCN_T_E4M3 ? 128 : type == DGCN_T_F32 ? 32 : 64, steps = (K + bk - 1) / bk;
   const double cus = num_cus();
   MatPlan best = {0, 1};
   double least = 1e300;
   for (int t = 0; t < (ta ? 2 : 3); ++t) {
-    const double wgs1 = static_cast<double>((M + tiles[t].bm - 1) / tiles[t].bm) * ((N + tiles[t].bn - 1) / tiles[t].bn);
+    const double tiles = static_cast<double>((M + cost[t].bm - 1) / cost[t].bm) * ((N + cost[t].bn - 1) / cost[t].bn);
     for (int sp = 1; sp <= 512 && sp <= steps; sp *= 2) {
-      const double wgs = wgs1 * sp, per_cu = ceil(wgs / cus);
-      const double held = per_cu < tiles[t].held ? per_cu : tiles[t].held;
-      const double step = held * tiles[t].work > 1200. ? held * tiles[t].work : 1200.;
-      double c = ceil(per_cu / tiles[t].held) * ((steps + sp - 1) / sp * step + 5000.);
-      if (sp > 1) c += 8. * M * N * sp / 2000. + 10000.;
-      if (c < least) { least = c; best = {t, sp}; }
+      const double per_cu = ceil(tiles * sp / cus), rounds = ceil(per_cu / cost[t].held);
+      const double each = static_cast<double>((steps + sp - 1) / sp), busy = per_cu * cost[t].work, lag = rounds * cost[t].lag;
+      double us = each * (busy > lag ? busy : lag) + rounds * cost[t].end;
+      if (sp > 1) us += 3. + 1e-6 * M * N * sp;
+      if (us < least) { least = us; best = {t, sp}; }
     }
   }
   return best;
@@ -66,9 +90,12 @@ inline MatPlan mat_plan(int64_t M, int64_t N, int64_t K, int type, int ta) {
 
 template <class O>
 int split_join(const MatParams& P, hipStream_t s) {
-  int64_t wgs = (P.M * ((P.N + 3) / 4) + 255) / 256;
-  if (wgs > 16 * num_cus()) wgs = 16 * num_cus();
-  hipLaunchKernelGGL((split_join_kernel<O>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, P);
+  const int64_t total = P.M * ((P.N + 3) / 4);
+  int segs = 1;
+  while (segs < 32 && segs * 4 <= P.splits && total * segs < 128 * static_cast<int64_t>(num_cus())) segs *= 2;
+  const int64_t wgs = (total + 256 / segs - 1) / (256 / segs);
+  if (wgs > 0x7fffffff) return DGCN_E_SHAPE;
+  hipLaunchKernelGGL((split_join_kernel<O>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, P, segs);
   return launch_status();
 }
 
@@ -127,8 +154,8 @@ inline GateShape gate_shape(int64_t rows, int N) {
   S.cl = 1;
   while (S.cl < 64 && S.cl < chunks) S.cl <<= 1;
   S.gx = static_cast<unsigned>((chunks + S.cl - 1) / S.cl);
-  // about eight workgroups a CU, at least 8 row steps each
-  int64_t want = 8 * static_cast<int64_t>(num_cus()) / S.gx;
+  // about four workgroups a CU, at least 8 row steps each
+  int64_t want = 4 * static_cast<int64_t>(num_cus()) / S.gx;
   const int64_t step = 256 / S.cl, most = (rows + 8 * step - 1) / (8 * step);
   if (want > most) want = most;
   if (want < 1) want = 1;
