@@ -64,8 +64,7 @@ int mat_tile_bf16(const MatParams& P, int ta, int tb, int tile, hipStream_t s);
 int mat_tile_f16(const MatParams& P, int ta, int tb, int tile, hipStream_t s);
 int mat_tile_e4m3(const MatParams& P, int out_type, int tile, hipStream_t s);
 
-// The product of a few K-contiguous rows, M <= kSmallRows (linear_small.h): operands at any byte
-constexpr int kSmallRows = 64;
+// The product of a few K-contiguous rows, at most 32 (linear_small.h): operands at any byte
 int mat_small_f32(const MatParams& P, hipStream_t s);
 int mat_small_bf16(const MatParams& P, hipStream_t s);
 int mat_small_f16(const MatParams& P, hipStream_t s);

@@ -265,8 +265,14 @@ int small_run(const MatParams& P, int in_type, int out_type, hipStream_t s) {
 }
 
 int linear_forward(MatParams P, int in_type, int out_type, Arena& ws, bool launch, hipStream_t s) {
-  if (P.M <= kSmallRows) return launch ? small_run(P, in_type, out_type, s) : DGCN_OK;
   const int es = type_bytes(in_type);
+  // Few rows go straight from memory.  From 17 on the tile is faster (32 rows x 16,384 x 4096 bf16: 31 us against 50, 1024 x 8192
+  // 13 against 25, 4096 x 4096 16 against 14), but not by as much as a copy of a weight that does not lie on 16 bytes costs.
+  const bool ready = operand_ready(P.a, P.lda, P.K, es) && operand_ready(P.b, P.ldb, P.K, es);
+  // Nor do few channels with a long K, whose workgroups leave most CUs idle: 256 x 16,384 bf16 takes 20 - 30 us against 9 split
+  // over the tile's workgroups, 1024 x 8192 12 - 17 against 11, 512 x 4096 7 - 9 against 8.
+  const bool narrow = P.N < 8 * static_cast<int64_t>(num_cus()) && P.K * es >= 16384;
+  if (P.M <= (ready ? 16 : 32) && !(ready && narrow)) return launch ? small_run(P, in_type, out_type, s) : DGCN_OK;
   Operand a, b;
   int rc = operand(P.a, P.lda, P.M, P.K, es, ws, launch, s, &a);
   if (rc == DGCN_OK) rc = operand(P.b, P.ldb, P.N, P.K, es, ws, launch, s, &b);

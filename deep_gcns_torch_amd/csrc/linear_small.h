@@ -1,9 +1,9 @@
-// The product of a few rows (kSmallRows at most) with a weight: what a model answers with one token or one node at a time.
+// The product of a few rows (16; 32 whose rows do not lie on 16 bytes) with a weight: what a model answers with one token or one node at a time.
 //
-// Bound by reading the weight once (2 rows flop a byte in 16 bits).  A workgroup owns 16 channels and all of K, its eight
-// waves take the 128-byte steps of the reduction in turn, straight from memory into matrix fragments (no LDS: nothing of
-// the weight is used twice), UNROLL steps requested ahead; the waves' sums meet in LDS in wave order.  Loads may start at
-// any byte, so odd strides and lengths need no copy of the weight.
+// Bound by reading the weight once (2 rows flop a byte in 16 bits).  A workgroup owns 16 channels and all of K, its eight or
+// sixteen waves take the 128-byte steps of the reduction in turn, straight from memory into matrix fragments (no LDS: nothing of
+// the weight is used twice), UNROLL steps requested ahead; the waves' sums meet in LDS in wave order.  Rows may start at any
+// byte, so odd strides and lengths need no copy of the weight.
 #pragma once
 
 #include "linear_tile.h"
@@ -69,82 +69,104 @@ template <> struct MatIn<WideE4m3> {
   }
 };
 
-typedef u4v u4v_any1 __attribute__((aligned(1)));
-
-// 16 bytes at `at` of a row of `bytes`; behind its end zeros
-__device__ __forceinline__ u4v row_unit(const char* row, int64_t at, int64_t bytes) {
-  if (at + 16 <= bytes) return *reinterpret_cast<const u4v_any1*>(row + at);
-  u4v v = {0, 0, 0, 0};
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    if (at + e < bytes) v[e >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[at + e])) << (8 * (e & 3));
+// A row that the kernel reads 16 bytes at a time.  Loads may start at any byte, but off a dword they take more than twice
+// as long (14,057 e4m3 channels, 5,121 rows of weight: 60 us against 29): SHIFT reads the five dwords that hold the 16 bytes,
+// which lie in the same allocation as the bytes do, and takes them together by a byte shift.
+template <bool SHIFT>
+struct Row {
+  const char* p;
+  uint32_t by;
+  __device__ __forceinline__ explicit Row(const char* row) : p(row), by(0) {
+    if constexpr (SHIFT) {
+      by = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 3u);
+      p = row - by;
+    }
   }
-  return v;
-}
+  __device__ __forceinline__ u4v at(int64_t a) const {
+    if constexpr (!SHIFT) return *reinterpret_cast<const u4v_any4*>(p + a);
+    const u4v v = *reinterpret_cast<const u4v_any4*>(p + a);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p + a + (by ? 16 : 12));
+    return u4v{__builtin_amdgcn_alignbyte(v[1], v[0], by), __builtin_amdgcn_alignbyte(v[2], v[1], by),
+               __builtin_amdgcn_alignbyte(v[3], v[2], by), __builtin_amdgcn_alignbyte(w, v[3], by)};
+  }
+  // at(a) of a row of `bytes`, zeros behind its end
+  __device__ __forceinline__ u4v end(int64_t a, int64_t bytes) const {
+    if (a + 16 <= bytes) return at(a);
+    u4v v = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if (a + e < bytes) v[e >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(p[a + by + e])) << (8 * (e & 3));
+    }
+    return v;
+  }
+};
 
-constexpr int kSmallWaves = 8;
-
-// MT: tiles of 16 rows
-template <class T, class O, int MT>
-__global__ __launch_bounds__(kSmallWaves * 64) void small_kernel(const MatParams P) {
-  constexpr int ES = MatIn<T>::ES, UNROLL = MT == 1 ? 4 : 2;
-  __shared__ f32x4 red[kSmallWaves][MT][64];
+// MT: tiles of 16 rows, NT: tiles of 16 channels a workgroup owns
+template <class T, class O, int MT, int NT, int WAVES, bool SHIFT>
+__global__ __launch_bounds__(WAVES * 64) void small_kernel(const MatParams P) {
+  constexpr int ES = MatIn<T>::ES, UNROLL = MT * NT == 1 ? 4 : 2;
+  __shared__ f32x4 red[WAVES][MT * NT][64];
   const int lane = lane_id(), wave = uni(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16, bytes = P.K * ES;
-  const int64_t nrow = n0 + i < P.N ? n0 + i : P.N - 1;
-  const char* wrow = static_cast<const char*>(P.b) + nrow * P.ldb * ES;
-  const char* xrow[MT];
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * NT), bytes = P.K * ES;
+  auto row_of = [&](const void* x, int64_t r, int64_t n, int64_t ld) { return static_cast<const char*>(x) + (r < n ? r : n - 1) * ld * ES; };
+  const Row<SHIFT> w0(row_of(P.b, n0 + i, P.N, P.ldb)), w1(row_of(P.b, n0 + 16 * (NT - 1) + i, P.N, P.ldb));
+  const Row<SHIFT> x0(row_of(P.a, i, P.M, P.lda)), x1(row_of(P.a, 16 * (MT - 1) + i, P.M, P.lda));
+  const int at0 = (ES == 4 ? 2 * q : q) * 16, at1 = at0 + (ES == 4 ? 16 : 64);
+  f32x4 acc[MT][NT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
-    const int64_t m = 16 * t + i < P.M ? 16 * t + i : P.M - 1;
-    xrow[t] = static_cast<const char*>(P.a) + m * P.lda * ES;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const int at0 = (ES == 4 ? 2 * q : q) * 16, at1 = at0 + (ES == 4 ? 16 : 64);
-  f32x4 acc[MT];
+  auto w_row = [&](int u) -> const Row<SHIFT>& { return u ? w1 : w0; };
+  auto x_row = [&](int t) -> const Row<SHIFT>& { return t ? x1 : x0; };
+  auto add = [&](const u4v (&rw)[NT][2], const u4v (&rx)[MT][2]) {
+    typename MatIn<T>::Frag w[NT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto add = [&](const u4v (&rw)[2], const u4v (&rx)[MT][2]) {
-    const typename MatIn<T>::Frag w = MatIn<T>::prep(rw);
+    for (int u = 0; u < NT; ++u) w[u] = MatIn<T>::prep(rw[u]);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) MatIn<T>::one_tile(w, MatIn<T>::prep(rx[t]), acc[t]);
+    for (int t = 0; t < MT; ++t) {
+      const typename MatIn<T>::Frag x = MatIn<T>::prep(rx[t]);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) MatIn<T>::one_tile(w[u], x, acc[t][u]);
+    }
   };
   const int64_t whole = bytes / 128;                       // steps that end inside every row
   int64_t s = wave;
-  for (; s + (UNROLL - 1) * kSmallWaves < whole; s += UNROLL * kSmallWaves) {
-    u4v rw[UNROLL][2], rx[UNROLL][MT][2];
+  for (; s + (UNROLL - 1) * WAVES < whole; s += UNROLL * WAVES) {
+    u4v rw[UNROLL][NT][2], rx[UNROLL][MT][2];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int64_t at = (s + u * kSmallWaves) * 128;
-      rw[u][0] = *reinterpret_cast<const u4v_any1*>(wrow + at + at0);
-      rw[u][1] = *reinterpret_cast<const u4v_any1*>(wrow + at + at1);
+    for (int k = 0; k < UNROLL; ++k) {
+      const int64_t at = (s + k * WAVES) * 128;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        rx[u][t][0] = *reinterpret_cast<const u4v_any1*>(xrow[t] + at + at0);
-        rx[u][t][1] = *reinterpret_cast<const u4v_any1*>(xrow[t] + at + at1);
-      }
+      for (int u = 0; u < NT; ++u) { rw[k][u][0] = w_row(u).at(at + at0); rw[k][u][1] = w_row(u).at(at + at1); }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) { rx[k][t][0] = x_row(t).at(at + at0); rx[k][t][1] = x_row(t).at(at + at1); }
     }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) add(rw[u], rx[u]);
+    for (int k = 0; k < UNROLL; ++k) add(rw[k], rx[k]);
   }
-  for (; s * 128 < bytes; s += kSmallWaves) {
+  for (; s * 128 < bytes; s += WAVES) {
     const int64_t at = s * 128;
-    u4v rw[2] = {row_unit(wrow, at + at0, bytes), row_unit(wrow, at + at1, bytes)}, rx[MT][2];
+    u4v rw[NT][2], rx[MT][2];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      rx[t][0] = row_unit(xrow[t], at + at0, bytes);
-      rx[t][1] = row_unit(xrow[t], at + at1, bytes);
-    }
+    for (int u = 0; u < NT; ++u) { rw[u][0] = w_row(u).end(at + at0, bytes); rw[u][1] = w_row(u).end(at + at1, bytes); }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) { rx[t][0] = x_row(t).end(at + at0, bytes); rx[t][1] = x_row(t).end(at + at1, bytes); }
     add(rw, rx);
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
+  for (int t = 0; t < MT; ++t) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) red[wave][t * NT + u][lane] = acc[t][u];
+  }
   __syncthreads();
-  // lane (i, q) of tile t: row 16 t + i, channels 4 q .. 4 q + 3
-  if (wave < MT) {
+  // lane (i, q) of tile (t, u): row 16 t + i, channels 16 u + 4 q .. + 3
+  if (wave < MT * NT) {
     f32x4 sum = red[0][wave][lane];
 #pragma unroll
-    for (int w = 1; w < kSmallWaves; ++w) sum += red[w][wave][lane];
-    const int64_t m = 16 * wave + i, n = n0 + 4 * q;
+    for (int w = 1; w < WAVES; ++w) sum += red[w][wave][lane];
+    const int64_t m = 16 * (wave / NT) + i, n = n0 + 16 * (wave % NT) + 4 * q;
     if (m < P.M && n < P.N) {
       float v[4];
 #pragma unroll
@@ -154,17 +176,34 @@ __global__ __launch_bounds__(kSmallWaves * 64) void small_kernel(const MatParams
   }
 }
 
-template <class T, class O, int MT>
-int small_go(const MatParams& P, hipStream_t s) {
-  hipLaunchKernelGGL((small_kernel<T, O, MT>), dim3(static_cast<unsigned>((P.N + 15) / 16)), dim3(kSmallWaves * 64), 0, s, P);
+template <class T, class O, int MT, int NT, int WAVES>
+int small_go(const MatParams& P, bool shift, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>((P.N + 16 * NT - 1) / (16 * NT)));
+  if constexpr (MatIn<T>::ES < 4) {
+    if (shift) {
+      hipLaunchKernelGGL((small_kernel<T, O, MT, NT, WAVES, true>), grid, dim3(WAVES * 64), 0, s, P);
+      return launch_status();
+    }
+  }
+  hipLaunchKernelGGL((small_kernel<T, O, MT, NT, WAVES, false>), grid, dim3(WAVES * 64), 0, s, P);
   return launch_status();
 }
 
+// Sixteen waves where the channels give at most one workgroup a CU and each wave still has four steps (4096 x 4096 bf16: one
+// row 7.9 us against 9.4 with eight, 16 rows 10.0 against 10.3); 32 channels a workgroup for e4m3 where they give every CU one
+// (16,384 x 4096, 16 rows: 17.2 us against 20.3; one row 16.3 against 16.9; in 16 bits it is slower, 35.5 against 34.1).
 template <class T, class O>
 int small_launch(const MatParams& P, hipStream_t s) {
-  if (P.M <= 16) return small_go<T, O, 1>(P, s);
-  if (P.M <= 32) return small_go<T, O, 2>(P, s);
-  return P.M <= 64 ? small_go<T, O, 4>(P, s) : DGCN_E_SHAPE;
+  constexpr int ES = MatIn<T>::ES;
+  const uintptr_t off = reinterpret_cast<uintptr_t>(P.a) | reinterpret_cast<uintptr_t>(P.b) | static_cast<uintptr_t>(P.lda * ES) | static_cast<uintptr_t>(P.ldb * ES);
+  const bool shift = (off & 3) != 0;
+  if (P.M > 32) return DGCN_E_SHAPE;
+  if (P.M > 16) return small_go<T, O, 2, 1, 8>(P, shift, s);
+  if constexpr (ES == 1) {
+    if (P.N >= 32 * static_cast<int64_t>(num_cus())) return small_go<T, O, 1, 2, 8>(P, shift, s);
+  }
+  if (P.N <= 16 * static_cast<int64_t>(num_cus()) && P.K * ES >= 64 * 128) return small_go<T, O, 1, 1, 16>(P, shift, s);
+  return small_go<T, O, 1, 1, 8>(P, shift, s);
 }
 
 }  // namespace
