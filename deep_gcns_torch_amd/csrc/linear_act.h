@@ -56,8 +56,7 @@ __device__ __forceinline__ void mat_epilogue(const MatParams& P, int64_t m, int6
   store_run<O, CNT>(static_cast<O*>(P.y) + at, first, N, v);
 }
 
-// The tiled product (linear_tile_*.hip), by operand type.  Operands start on 16 bytes and their row strides are multiples of
-// 16 bytes; where the contiguous extent of an operand is none, the values up to the next one are there, and are zeros along K.
+// The tiled product (linear_tile_*.hip), by operand type; the operands' rows (k-rows) start on dwords.
 // tile: 0 = 256 x 256, 1 = 128 x 128, 2 = 64 x 128 (K-contiguous A only)
 int mat_tile_f32(const MatParams& P, int ta, int tb, int tile, hipStream_t s);
 int mat_tile_bf16(const MatParams& P, int ta, int tb, int tile, hipStream_t s);

@@ -205,7 +205,7 @@ struct Arena {
   bool full() const { return used > size; }
 };
 
-// An operand as the tiled kernel takes it: 16-byte starts and strides, nothing but the row in its last 16 bytes
+// An operand as the tiled kernel takes it: rows that start on dwords
 struct Operand {
   const void* p;
   int64_t ld;
@@ -213,13 +213,13 @@ struct Operand {
 
 constexpr int64_t kFarStride = int64_t{1} << 20;           // strides from here on leave the tile's 32-bit offsets
 
-inline bool operand_ready(const void* p, int64_t ld, int64_t C, int es) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * es % 16 == 0 && C * es % 16 == 0 && ld <= kFarStride;
+inline bool operand_ready(const void* p, int64_t ld, int es) {
+  return (reinterpret_cast<uintptr_t>(p) & 3) == 0 && ld * es % 4 == 0 && ld <= kFarStride;
 }
 
 int operand(const void* p, int64_t ld, int64_t rows, int64_t C, int es, Arena& ws, bool launch, hipStream_t s, Operand* out) {
   *out = {p, ld};
-  if (operand_ready(p, ld, C, es)) return DGCN_OK;
+  if (operand_ready(p, ld, es)) return DGCN_OK;
   const int64_t ldo = round16(C * es);
   uint8_t* to = static_cast<uint8_t*>(ws.take(rows * ldo));
   *out = {to, ldo / es};
@@ -267,8 +267,8 @@ int small_run(const MatParams& P, int in_type, int out_type, hipStream_t s) {
 int linear_forward(MatParams P, int in_type, int out_type, Arena& ws, bool launch, hipStream_t s) {
   const int es = type_bytes(in_type);
   // Few rows go straight from memory.  From 17 on the tile is faster (32 rows x 16,384 x 4096 bf16: 31 us against 50, 1024 x 8192
-  // 13 against 25, 4096 x 4096 16 against 14), but not by as much as a copy of a weight that does not lie on 16 bytes costs.
-  const bool ready = operand_ready(P.a, P.lda, P.K, es) && operand_ready(P.b, P.ldb, P.K, es);
+  // 13 against 25, 4096 x 4096 16 against 14), but not by as much as a copy of a weight whose rows start off dwords costs.
+  const bool ready = operand_ready(P.a, P.lda, es) && operand_ready(P.b, P.ldb, es);
   // Nor do few channels with a long K, whose workgroups leave most CUs idle: 256 x 16,384 bf16 takes 20 - 30 us against 9 split
   // over the tile's workgroups, 1024 x 8192 12 - 17 against 11, 512 x 4096 7 - 9 against 8.
   const bool narrow = P.N < 8 * static_cast<int64_t>(num_cus()) && P.K * es >= 16384;
@@ -320,7 +320,7 @@ int linear_backward(const BwdArgs& A, Arena& ws, bool launch, hipStream_t s) {
   if (A.act != DGCN_ACT_NONE || A.db) {
     const GateShape S = gate_shape(A.rows, A.N);
     void* to = nullptr;
-    if (A.act != DGCN_ACT_NONE || (products && !operand_ready(A.g, A.ldg, A.N, es))) {
+    if (A.act != DGCN_ACT_NONE || (products && !operand_ready(A.g, A.ldg, es))) {
       const int64_t ld = round16(static_cast<int64_t>(A.N) * es) / es;
       to = ws.take(A.rows * ld * es);
       dz = {to, ld};

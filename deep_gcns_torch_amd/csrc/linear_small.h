@@ -1,4 +1,4 @@
-// The product of a few rows (16; 32 whose rows do not lie on 16 bytes) with a weight: what a model answers with one token or one node at a time.
+// The product of a few rows (16; 32 whose rows do not start on dwords) with a weight: what a model answers with one token or one node at a time.
 //
 // Bound by reading the weight once (2 rows flop a byte in 16 bits).  A workgroup owns 16 channels and all of K, its eight or
 // sixteen waves take the 128-byte steps of the reduction in turn, straight from memory into matrix fragments (no LDS: nothing of

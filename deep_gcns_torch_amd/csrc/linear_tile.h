@@ -137,11 +137,11 @@ __device__ __forceinline__ unsigned tile_offset(int inst, int lane, int64_t ld) 
   }
 }
 
-// bytes from the first to behind the last value of an operand tile whose stage holds k of the reduction
+// Bytes from the first to behind the last value of an operand tile whose stage holds k of the reduction, in whole dwords: the
+// range check of a buffer is by dword, and the dword that holds the last value is there as long as rows start on dwords.
 template <int T, int ES>
 __device__ __forceinline__ int tile_bytes(int64_t ld, int64_t lines, int k) {
-  constexpr int CH = 16 / ES;                              // values in 16 bytes
-  return static_cast<int>((T == 0 ? (lines - 1) * ld + (k + CH - 1) / CH * CH : (k - 1) * ld + (lines + CH - 1) / CH * CH) * ES);
+  return static_cast<int>((((T == 0 ? (lines - 1) * ld + k : (k - 1) * ld + lines) * ES) + 3) & ~int64_t{3});
 }
 
 // A raw buffer of `bytes` bytes at p, as its four scalar words
@@ -221,8 +221,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
   const int64_t rows_a = P.M - m0 < BM ? P.M - m0 : BM, rows_b = P.N - n0 < BN ? P.N - n0 : BN;
 
   // copy(place) requests the next stage into one of the two places.  Rows and k-rows behind the matrix lie behind the buffer's
-  // end and read as zeros; so do, by an offset of kBehind, the chunks of a K-contiguous row behind K (a chunk that K ends in
-  // is the operand's zero padding from there), and all of a stage behind the last one, which is requested all the same so
+  // end and read as zeros; so do, by an offset of kBehind, the chunks of a K-contiguous row behind K (what follows K in the
+  // chunk that it ends in is cut from the fragments, see clip), and all of a stage behind the last one, which is requested all the same so
   // that a wave always has the same number of copies under way.   Columns of a K-strided operand behind M or N read what is
   // there: their sums are not stored.
   const int64_t step_a = (TA == 0 ? BK : BK * P.lda) * ES, step_b = (TB == 0 ? BK : BK * P.ldb) * ES;
@@ -289,17 +289,32 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
   auto meet = [&](auto copies) {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(copies)::value) : "memory");
   };
+  // the values of a half's raw fragment of a K-contiguous operand that lie behind K, cleared (both operands': what is there
+  // may be infinite or NaN)
+  const int last_bytes = last_k * ES;
+  auto clip = [&](auto layout, int half, u8v r) {
+    if constexpr (decltype(layout)::value == 0) {
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const int n = last_bytes - 64 * half - (ES == 2 ? (w < 4 ? 16 * h : 32 + 16 * h) + 4 * (w & 3) : 32 * h + 4 * w);
+        r[w] &= n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+      }
+    }
+    return r;
+  };
   // A half: its fragments lie in fa and b.  Each row tile's products are followed by the read of the same tile of the next
   // half.  Before the second half's reads, of the next stage, the waves meet -- behind the first products, so that the
   // barrier finds the matrix pipe busy -- and behind them the stage after next is requested into the place of this one.
+  // whole: that stage is a full one; cut: this stage is the one that K ends in, inside a chunk.
   u8v fa[TM], b0[2], b1[2];
-  auto turn = [&](auto half, auto whole, int place, const u8v (&b)[2], u8v (&b_next)[2]) {
+  auto turn = [&](auto half, auto whole, auto cut, int place, const u8v (&b)[2], u8v (&b_next)[2]) {
     constexpr int H = decltype(half)::value;
     const int from = place ^ H;
-    const typename TileIn<T>::Frag fb[2] = {TileIn<T>::prep(b[0]), TileIn<T>::prep(b[1])};
+    constexpr bool CUT = decltype(cut)::value;
+    const typename TileIn<T>::Frag fb[2] = {TileIn<T>::prep(CUT ? clip(LB{}, H, b[0]) : b[0]), TileIn<T>::prep(CUT ? clip(LB{}, H, b[1]) : b[1])};
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
-      TileIn<T>::mul(fb, TileIn<T>::prep(fa[t]), acc[t]);
+      TileIn<T>::mul(fb, TileIn<T>::prep(CUT ? clip(LA{}, H, fa[t]) : fa[t]), acc[t]);
       if (t == 0) {
         if constexpr (H == 1) {
           __builtin_amdgcn_sched_barrier(0);
@@ -324,13 +339,20 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
 #pragma unroll
   for (int t = 0; t < TM; ++t) fa[t] = read_a(0, 0, t);
   int place = 0, step = s0;
+  const int ends = ((TA == 0 || TB == 0) && s1 == steps_all && last_bytes % 16 != 0) ? s1 - 1 : s1;
+  typedef std::true_type Yes;
+  typedef std::false_type No;
   for (; todo > 1; ++step, place ^= 1) {                                // full stages ahead: no selection in the loop
-    turn(H0{}, std::true_type{}, place, b0, b1);
-    turn(H1{}, std::true_type{}, place, b1, b0);
+    turn(H0{}, Yes{}, No{}, place, b0, b1);
+    turn(H1{}, Yes{}, No{}, place, b1, b0);
   }
-  for (; step < s1; ++step, place ^= 1) {
-    turn(H0{}, std::false_type{}, place, b0, b1);
-    turn(H1{}, std::false_type{}, place, b1, b0);
+  for (; step < ends; ++step, place ^= 1) {
+    turn(H0{}, No{}, No{}, place, b0, b1);
+    turn(H1{}, No{}, No{}, place, b1, b0);
+  }
+  if (step < s1) {
+    turn(H0{}, No{}, Yes{}, place, b0, b1);
+    turn(H1{}, No{}, Yes{}, place, b1, b0);
   }
 
   // Epilogue, through LDS (when all copies have landed and nobody reads operands any more): a wave writes its sums as rows of

@@ -80,10 +80,10 @@ def test_c_entry_argument_errors_do_not_launch():
     assert back(p, 8, p, 8, p, 8, p, 9, 0.0, 0, p, p, p, 0, 1, 8, 8, None, 0, None) == -4
     assert back(p, 8, p, 8, p, 8, None, 0, 0.0, 0, p, p, p, 0, 0, 8, 8, None, 0, None) == -2
     assert back(p, 8, p, 8, p, 8, None, 0, 0.0, 0, None, None, None, 0, 1, 8, 8, None, 0, None) == 0            # nothing asked for
-    # workspaces: none for few rows; partial sums for a long reduction; copies for rows off 16 bytes, and too small is refused
+    # workspaces: none for few rows; partial sums for a long reduction; copies for rows off dwords, and too small is refused
     need, back_need = lib.dgcn_linear_workspace, lib.dgcn_linear_bwd_workspace
     assert need(p, 8, p, 8, 1, 16, 8, 8) == 0 and need(p, 4096, p, 4096, 1, 65536, 4096, 4096) == 0
-    assert need(p, 9, p, 8, 1, 1000, 8, 8) >= 1000 * 16 and need(p + 2, 8, p, 8, 1, 1000, 8, 8) >= 1000 * 16
+    assert need(p, 10, p, 8, 1, 1000, 8, 8) == 0 and need(p, 9, p, 8, 1, 1000, 8, 8) >= 1000 * 16 and need(p + 2, 8, p, 8, 1, 1000, 8, 8) >= 1000 * 16
     assert act(p + 2, 8, p, 8, None, None, None, 0, None, 0, 0, 0.0, 1, 1, None, p, 1000, 8, 8, p, 64, None) == -5
     n = back_need(p, 64, p, 64, p, 64, 0, 1, 2, 100000, 64, 64)
     assert n > 0 and back(p, 64, p, 64, p, 64, None, 0, 0.0, 1, None, p, None, 0, 100000, 64, 64, p, n - 256, None) == -5

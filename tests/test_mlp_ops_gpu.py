@@ -304,6 +304,36 @@ def test_strides_and_leading_dimensions(dtype):
     assert torch.equal(mlp_ops.linear_act_e4m3(xs, ws, out_dtype=dtype), mlp_ops.linear_act_e4m3(xc, wc, out_dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [1, 2, 6, 30, 33, 62, 66, 90, 127, 130, 190])
+def test_rows_that_end_inside_a_chunk_see_nothing_behind(dtype, K):
+    """Rows of a wider matrix whose neighbours are NaN and infinite: nothing behind K, and nothing of another row, gets in."""
+    big = torch.full((200, 200), float("nan"), device="cuda", dtype=dtype)
+    big[:, 150:] = float("inf")
+    wide = big.clone()
+    big[:, :K] = rand(200, K, dtype=dtype, seed=1)
+    wide[:, :K] = rand(200, K, dtype=dtype, seed=2, scale=0.2)
+    x, w = big[:, :K], wide[:, :K]
+    y = mlp_ops.linear_act(x, w)
+    assert torch.isfinite(y).all() and torch.equal(y, mlp_ops.linear_act(x.contiguous(), w.contiguous()))
+    check_linear(x, w, None, None, "none", y, dtype)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    g = big[:, :200].clone()
+    g[:, K:] = 0
+    g = torch.cat([g[:, :K], torch.zeros(200, 200 - K, device="cuda", dtype=dtype)], 1)
+    g2 = torch.full((200, 260), float("nan"), device="cuda", dtype=dtype)
+    g2[:, 3:203] = g
+    for grad in (g, g2[:, 3:203]):
+        gx, gw = torch.autograd.grad(mlp_ops.linear_act(xg, wg), (xg, wg), grad)
+        z, ez, _, _ = linear_bounds(xg.detach(), wg.detach(), None, "none", dtype)
+        check_linear_grads(xg.detach(), wg.detach(), None, None, "none", g, (gx, gw), z, ez, dtype)
+    q = mlp_ops.quantize_rows(x.contiguous())
+    nan = torch.full((200, 200), 0x7f, device="cuda", dtype=torch.uint8)
+    nan[:, :K] = q.data.view(torch.uint8)
+    part = RowsE4M3(nan.view(torch.float8_e4m3fn)[:, :K], q.scale)
+    assert torch.equal(mlp_ops.linear_act_e4m3(part, part, out_dtype=dtype), mlp_ops.linear_act_e4m3(q, q, out_dtype=dtype))
+
+
 def test_gradients_of_strided_and_broadcast_inputs():
     x0 = rand(50, 40, dtype=torch.float32, seed=1).requires_grad_()
     w = rand(24, 20, dtype=torch.float32, seed=2, scale=0.2).requires_grad_()
