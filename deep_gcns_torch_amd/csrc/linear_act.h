@@ -27,33 +27,50 @@ struct MatParams {
   int64_t M, N, K;
 };
 
-// bias, z, activation, residual and store of the channels n .. n + CNT - 1 of row m (v: the scaled sums)
+// What the backward keeps, the activation, the residual r and the store of the channels n .. n + CNT - 1 of row m (v: the
+// scaled sums with their bias)
+template <class O, int CNT>
+__device__ __forceinline__ void mat_finish(const MatParams& P, int64_t m, int n, float (&v)[CNT], const float (&r)[CNT]) {
+  constexpr bool EXACT = sizeof(O) == 4;
+  const int N = static_cast<int>(P.N);
+  const int64_t at = m * P.N;
+  if constexpr (EXACT) {
+    if (P.z) store_run<O, CNT>(static_cast<O*>(P.z) + at, n, N, v);
+    act_run<EXACT, CNT>(v, P.act, P.slope);
+  } else if (P.z) {
+    uint32_t c[CNT];
+    act_gate_run<CNT>(v, c, P.act, P.slope);
+    store_gates<CNT>(static_cast<uint16_t*>(P.z) + at, n, N, c);
+  } else {
+    act_run<EXACT, CNT>(v, P.act, P.slope);
+  }
+#pragma unroll
+  for (int e = 0; e < CNT; ++e) v[e] += r[e];
+  store_run<O, CNT>(static_cast<O*>(P.y) + at, n, N, v);
+}
+
+template <class O, int CNT>
+__device__ __forceinline__ void mat_residual(const MatParams& P, int64_t m, int n, float (&r)[CNT]) {
+  if (P.res) {
+    load_run<O, CNT>(static_cast<const O*>(P.res) + m * P.ldr, n, static_cast<int>(P.N), r);
+  } else {
+#pragma unroll
+    for (int e = 0; e < CNT; ++e) r[e] = 0.f;
+  }
+}
+
+// all of an epilogue for one run of channels
 template <class O, int CNT>
 __device__ __forceinline__ void mat_epilogue(const MatParams& P, int64_t m, int64_t n, float (&v)[CNT]) {
-  constexpr bool EXACT = sizeof(O) == 4;
-  const int64_t at = m * P.N;
-  const int first = static_cast<int>(n), N = static_cast<int>(P.N);
+  float r[CNT];
+  mat_residual<O, CNT>(P, m, static_cast<int>(n), r);
   if (P.bias) {
     float b[CNT];
-    load_param_run<O, CNT>(P.bias, P.bias_f32, first, N, b);
+    load_param_run<O, CNT>(P.bias, P.bias_f32, static_cast<int>(n), static_cast<int>(P.N), b);
 #pragma unroll
     for (int e = 0; e < CNT; ++e) v[e] += b[e];
   }
-  if (P.z) {
-    if constexpr (EXACT) {
-      store_run<O, CNT>(static_cast<O*>(P.z) + at, first, N, v);
-    } else {
-      store_gates<CNT>(static_cast<uint16_t*>(P.z) + at, first, N, v, P.act);
-    }
-  }
-  act_run<EXACT, CNT>(v, P.act, P.slope);
-  if (P.res) {
-    float r[CNT];
-    load_run<O, CNT>(static_cast<const O*>(P.res) + m * P.ldr, first, N, r);
-#pragma unroll
-    for (int e = 0; e < CNT; ++e) v[e] += r[e];
-  }
-  store_run<O, CNT>(static_cast<O*>(P.y) + at, first, N, v);
+  mat_finish<O, CNT>(P, m, static_cast<int>(n), v, r);
 }
 
 // The tiled product (linear_tile_*.hip), by operand type; the operands' rows (k-rows) start on dwords.

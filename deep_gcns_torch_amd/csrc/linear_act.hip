@@ -205,7 +205,8 @@ struct Arena {
   bool full() const { return used > size; }
 };
 
-// An operand as the tiled kernel takes it: rows that start on dwords
+// An operand as the tiled kernel takes it: rows that start on dwords, and, where they are the k-rows of a K-strided operand
+// (span: their C values), that do not repeat or overlap -- the k-rows behind the last one have to lie behind the buffer's end
 struct Operand {
   const void* p;
   int64_t ld;
@@ -213,13 +214,14 @@ struct Operand {
 
 constexpr int64_t kFarStride = int64_t{1} << 20;           // strides from here on leave the tile's 32-bit offsets
 
-inline bool operand_ready(const void* p, int64_t ld, int es) {
-  return (reinterpret_cast<uintptr_t>(p) & 3) == 0 && ld * es % 4 == 0 && ld <= kFarStride;
+inline bool operand_ready(const void* p, int64_t ld, int es, int64_t span) {
+  return ld >= span && (reinterpret_cast<uintptr_t>(p) & 3) == 0 && ld * es % 4 == 0 && ld <= kFarStride;
 }
 
-int operand(const void* p, int64_t ld, int64_t rows, int64_t C, int es, Arena& ws, bool launch, hipStream_t s, Operand* out) {
+int operand(const void* p, int64_t ld, int64_t rows, int64_t C, bool strided, int es, Arena& ws, bool launch, hipStream_t s,
+            Operand* out) {
   *out = {p, ld};
-  if (operand_ready(p, ld, es)) return DGCN_OK;
+  if (operand_ready(p, ld, es, strided ? C : 0)) return DGCN_OK;
   const int64_t ldo = round16(C * es);
   uint8_t* to = static_cast<uint8_t*>(ws.take(rows * ldo));
   *out = {to, ldo / es};
@@ -268,14 +270,14 @@ int linear_forward(MatParams P, int in_type, int out_type, Arena& ws, bool launc
   const int es = type_bytes(in_type);
   // Few rows go straight from memory.  From 17 on the tile is faster (32 rows x 16,384 x 4096 bf16: 31 us against 50, 1024 x 8192
   // 13 against 25, 4096 x 4096 16 against 14), but not by as much as a copy of a weight whose rows start off dwords costs.
-  const bool ready = operand_ready(P.a, P.lda, es) && operand_ready(P.b, P.ldb, es);
+  const bool ready = operand_ready(P.a, P.lda, es, 0) && operand_ready(P.b, P.ldb, es, 0);
   // Nor do few channels with a long K, whose workgroups leave most CUs idle: 256 x 16,384 bf16 takes 20 - 30 us against 9 split
   // over the tile's workgroups, 1024 x 8192 12 - 17 against 11, 512 x 4096 7 - 9 against 8.
   const bool narrow = P.N < 8 * static_cast<int64_t>(num_cus()) && P.K * es >= 16384;
   if (P.M <= (ready ? 16 : 32) && !(ready && narrow)) return launch ? small_run(P, in_type, out_type, s) : DGCN_OK;
   Operand a, b;
-  int rc = operand(P.a, P.lda, P.M, P.K, es, ws, launch, s, &a);
-  if (rc == DGCN_OK) rc = operand(P.b, P.ldb, P.N, P.K, es, ws, launch, s, &b);
+  int rc = operand(P.a, P.lda, P.M, P.K, false, es, ws, launch, s, &a);
+  if (rc == DGCN_OK) rc = operand(P.b, P.ldb, P.N, P.K, false, es, ws, launch, s, &b);
   if (rc != DGCN_OK) return rc;
   P.a = a.p; P.lda = a.ld; P.b = b.p; P.ldb = b.ld;
   return mat_run(P, 0, 0, in_type, out_type, ws, launch, s);
@@ -320,7 +322,7 @@ int linear_backward(const BwdArgs& A, Arena& ws, bool launch, hipStream_t s) {
   if (A.act != DGCN_ACT_NONE || A.db) {
     const GateShape S = gate_shape(A.rows, A.N);
     void* to = nullptr;
-    if (A.act != DGCN_ACT_NONE || (products && !operand_ready(A.g, A.ldg, es))) {
+    if (A.act != DGCN_ACT_NONE || (products && !operand_ready(A.g, A.ldg, es, A.dw ? A.N : 0))) {
       const int64_t ld = round16(static_cast<int64_t>(A.N) * es) / es;
       to = ws.take(A.rows * ld * es);
       dz = {to, ld};
@@ -337,18 +339,18 @@ int linear_backward(const BwdArgs& A, Arena& ws, bool launch, hipStream_t s) {
       if (rc != DGCN_OK) return rc;
     }
   } else if (products) {
-    rc = operand(A.g, A.ldg, A.rows, A.N, es, ws, launch, s, &dz);
+    rc = operand(A.g, A.ldg, A.rows, A.N, A.dw != nullptr, es, ws, launch, s, &dz);
     if (rc != DGCN_OK) return rc;
   }
   if (A.dx) {
     Operand w;
-    rc = operand(A.w, A.ldw, A.N, A.K, es, ws, launch, s, &w);
+    rc = operand(A.w, A.ldw, A.N, A.K, true, es, ws, launch, s, &w);
     if (rc == DGCN_OK) rc = mat_run(plain_product(dz, w, A.dx, A.rows, A.K, A.N), 0, 1, A.type, A.type, ws, launch, s);
     if (rc != DGCN_OK) return rc;
   }
   if (A.dw) {
     Operand x;
-    rc = operand(A.x, A.ldx, A.rows, A.K, es, ws, launch, s, &x);
+    rc = operand(A.x, A.ldx, A.rows, A.K, true, es, ws, launch, s, &x);
     if (rc == DGCN_OK) rc = mat_run(plain_product(dz, x, A.dw, A.N, A.K, A.rows), 1, 1, A.type, A.type, ws, launch, s);
   }
   return rc;

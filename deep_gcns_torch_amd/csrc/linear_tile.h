@@ -363,39 +363,56 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
   meet(std::integral_constant<int, 0>{});
   char* mine = lds + wave * (PASS * 32 * 256);
   const int64_t mw = m0 + wm * TM * 32, n = n0 + wn * 64 + 8 * (lane & 7);
-  float bs[8];
+  const bool inside = n < P.N;
+  float scale[8], bias[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) bs[e] = (ES == 1 && n + e < P.N) ? P.b_scale[n + e] : 1.f;
+  for (int e = 0; e < 8; ++e) {
+    scale[e] = (ES == 1 && n + e < P.N) ? P.b_scale[n + e] : 1.f;
+    bias[e] = 0.f;
+  }
+  if (P.bias && inside) load_param_run<O, 8>(P.bias, P.bias_f32, static_cast<int>(n), static_cast<int>(P.N), bias);
+  constexpr int AHEAD = 4;                                              // residual rows requested together: their latency is a tile's epilogue otherwise
 #pragma unroll
   for (int p = 0; p < TM / PASS; ++p) {
 #pragma unroll
     for (int t = 0; t < PASS; ++t) {
 #pragma unroll
-      for (int u = 0; u < 16; ++u) {                                    // tile u >> 3, group (u >> 1) & 3 ... unit 8 tile + 2 g + h
-        if (u & 1) continue;
+      for (int u = 0; u < 16; u += 2) {                                 // unit 8 tile + 2 g + h
         const f32x16& c = acc[p * PASS + t][u >> 3];
         const int g = (u >> 1) & 3;
         *reinterpret_cast<f32x4*>(mine + (t * 32 + i) * 256 + (((u + h) ^ (i & 15)) << 4)) = f32x4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]};
       }
     }
 #pragma unroll 1
-    for (int r0 = 0; r0 < PASS * 32; r0 += 8) {
-      const int r = r0 + (lane >> 3), u = 2 * (lane & 7);
-      const int64_t m = mw + p * PASS * 32 + r;
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + r * 256 + ((u ^ (r & 15)) << 4));
-      const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((u + 1) ^ (r & 15)) << 4));
-      if (m < P.M && n < P.N) {
-        const float as = ES == 1 ? P.a_scale[m] : 1.f;
-        float v[8];
+    for (int r0 = 0; r0 < PASS * 32; r0 += 8 * AHEAD) {
+      const int64_t m_first = mw + p * PASS * 32 + r0 + (lane >> 3);
+      float res[AHEAD][8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = ES == 1 ? lo[e] * (as * bs[e]) : lo[e];
-          v[4 + e] = ES == 1 ? hi[e] * (as * bs[4 + e]) : hi[e];
-        }
-        if (P.splits > 1) {
-          store_chunk(P.part + (static_cast<int64_t>(split) * P.M + m) * P.N, n, P.N, v);
-        } else {
-          mat_epilogue<O, 8>(P, m, n, v);
+      for (int k = 0; k < AHEAD; ++k) {
+        const int64_t m = m_first + 8 * k;
+        if (P.splits == 1 && inside && m < P.M) mat_residual<O, 8>(P, m, static_cast<int>(n), res[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int r = r0 + 8 * k + (lane >> 3), u = 2 * (lane & 7);
+        const int64_t m = m_first + 8 * k;
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + r * 256 + ((u ^ (r & 15)) << 4));
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((u + 1) ^ (r & 15)) << 4));
+        if (m < P.M && inside) {
+          const float as = ES == 1 ? P.a_scale[m] : 1.f;
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = ES == 1 ? lo[e] * (as * scale[e]) : lo[e];
+            v[4 + e] = ES == 1 ? hi[e] * (as * scale[4 + e]) : hi[e];
+          }
+          if (P.splits > 1) {
+            store_chunk(P.part + (static_cast<int64_t>(split) * P.M + m) * P.N, n, P.N, v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += bias[e];
+            mat_finish<O, 8>(P, m, static_cast<int>(n), v, res[k]);
+          }
         }
       }
     }

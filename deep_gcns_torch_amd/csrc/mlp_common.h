@@ -144,48 +144,85 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
 }
 
 // ---- activations: act(z) and act'(z), in fp32 ----
-// EXACT (the fp32 type): libm's exp and erfc.  Otherwise the hardware's 2^x, off by |z| 2^-24, and the normal distribution
-// function below, off by 1e-5 of its value: both far below a 16-bit half step (bf16 2^-9, fp16 2^-12 of a value in [1, 2)).
+// EXACT (the fp32 type): libm's exp and the longer fit below.  Otherwise the hardware's 2^x, off by |z| 2^-24, its reciprocal,
+// and the shorter fit: all far below a 16-bit half step (bf16 2^-9, fp16 2^-12 of a value in [1, 2)).
 template <bool EXACT>
 __device__ __forceinline__ float act_exp(float x) { return EXACT ? expf(x) : fast_exp(x); }
+template <bool EXACT>
+__device__ __forceinline__ float act_inv(float x) { return EXACT ? 1.f / x : __builtin_amdgcn_rcpf(x); }
 
 // Phi(z) and, in `bell`, exp(-z^2 / 2).  Both sides come from erfc(|z| / sqrt 2), so that nothing cancels for z < 0:
-// erfc(x) = exp(-x^2) t P(t), t = 1 / (1 + 0.45 x), P of degree five fitted to the least relative error over 0 <= x <= 14
-// (9.6e-6); libm's erfc is some five times as many instructions, and a 256 x 256 tile evaluates 65,536 of them.
+// erfc(x) = exp(-x^2) t P(t), t = 1 / (1 + p x), P fitted to the least relative error over 0 <= x <= 10 (degree eight, p = 0.5:
+// 4e-8, with fp32's own rounding 7e-8 on average) or 14 (degree five, p = 0.45: 1e-5).  libm's erfc is several times as many
+// instructions, and a 256 x 256 tile evaluates 65,536 of them.
 template <bool EXACT>
 __device__ __forceinline__ float normal_cdf(float z, float& bell) {
+  constexpr float kFit[9] = {0.282086422f, 0.282375231f, 0.243104417f, 0.202683901f, -0.0266177002f, 0.278054163f, -0.487187249f, 0.284568217f, -0.0590674445f};
+  constexpr float kShort[6] = {0.25396813f, 0.251702589f, 0.248475618f, 0.0894637792f, 0.292237032f, -0.135856623f};
   bell = act_exp<EXACT>(-0.5f * z * z);
-  if constexpr (EXACT) return 0.5f * erfcf(z * -0.70710678118654752f);
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.45f * 0.70710678118654752f, fabsf(z), 1.f));
-  float p = -0.135856623f;
-  p = fmaf(p, t, 0.292237032f);
-  p = fmaf(p, t, 0.0894637792f);
-  p = fmaf(p, t, 0.248475618f);
-  p = fmaf(p, t, 0.251702589f);
-  p = fmaf(p, t, 0.25396813f);
-  const float tail = 0.5f * p * t * bell;                              // Phi(-|z|)
+  const float t = act_inv<EXACT>(fmaf((EXACT ? 0.5f : 0.45f) * 0.70710678118654752f, fabsf(z), 1.f));
+  float p = EXACT ? kFit[8] : kShort[5];
+#pragma unroll
+  for (int k = EXACT ? 7 : 4; k >= 0; --k) p = fmaf(p, t, EXACT ? kFit[k] : kShort[k < 6 ? k : 5]);
+  const float tail = (0.5f * p * t) * bell;                            // Phi(-|z|)
   return z < 0.f ? tail : 1.f - tail;
 }
 
+// act(z), and act'(z) in `d` (unused: dropped by the compiler)
 template <bool EXACT>
-__device__ __forceinline__ float act_fwd(float z, int act, float slope) {
+__device__ __forceinline__ float act_both(float z, int act, float slope, float& d) {
   switch (act) {
-    case DGCN_ACT_RELU: return z < 0.f ? 0.f : z;                       // (NaN stays NaN)
-    case DGCN_ACT_LEAKY_RELU: return z > 0.f ? z : slope * z;
+    case DGCN_ACT_RELU:                                                 // (NaN stays NaN)
+      d = z > 0.f ? 1.f : z != z ? z : 0.f;
+      return z < 0.f ? 0.f : z;
+    case DGCN_ACT_LEAKY_RELU:
+      d = z > 0.f ? 1.f : slope;
+      return z > 0.f ? z : slope * z;
     case DGCN_ACT_GELU: {
       float bell;
-      return z * normal_cdf<EXACT>(z, bell);
+      const float cdf = normal_cdf<EXACT>(z, bell);
+      d = fmaf(z * 0.39894228040143268f, bell, cdf);
+      return z * cdf;
     }
-    case DGCN_ACT_SILU: return EXACT ? z / (1.f + act_exp<EXACT>(-z)) : z * __builtin_amdgcn_rcpf(1.f + act_exp<EXACT>(-z));
-    default: return z;
+    case DGCN_ACT_SILU: {
+      const float s = act_inv<EXACT>(1.f + act_exp<EXACT>(-z));
+      const float y = z * s;
+      d = fmaf(y, 1.f - s, s);
+      return y;
+    }
+    default: d = 1.f; return z;
   }
+}
+
+template <bool EXACT>
+__device__ __forceinline__ float act_slope(float z, int act, float slope) {
+  float d;
+  act_both<EXACT>(z, act, slope, d);
+  return d;
+}
+
+// ---- what the backward of an activation in 16 bits keeps: act'(z) in fixed point, code = (act' + 1/4) 2^15 ----
+// gelu's and silu's slopes lie in (-0.13, 1.13); they come back within 2^-16, an eighth of a bf16 half step and less of
+// anything that is averaged.  (z in 16 bits would be off by half a step of z in act': measured, 1.5 times the error of the
+// bias gradient.)  relu and leakyrelu keep z > 0 as a slope of 1 or 0.  Code 0 is NaN (what the conversion makes of one).
+__device__ __forceinline__ uint32_t gate_encode(float d) {
+  uint32_t c;
+  asm("v_cvt_u32_f32 %0, %1" : "=v"(c) : "v"(fmaf(d, 32768.f, 8192.5f)));
+  return c;
+}
+
+__device__ __forceinline__ float gate_decode(uint32_t code, int act, float slope) {
+  const float d = fmaf(static_cast<float>(code), 1.f / 32768.f, -0.25f);
+  if (code == 0u) return __builtin_nanf("");
+  return act == DGCN_ACT_LEAKY_RELU && code == 8192u ? slope : d;
 }
 
 // a run of values under one (uniform) activation: the branch is outside the run
 template <bool EXACT, int CNT>
 __device__ __forceinline__ void act_run(float (&v)[CNT], int act, float slope) {
+  float d;
   switch (act) {
-#define DGCN_ACT_CASE(A) case A: { _Pragma("unroll") for (int e = 0; e < CNT; ++e) v[e] = act_fwd<EXACT>(v[e], A, slope); break; }
+#define DGCN_ACT_CASE(A) case A: { _Pragma("unroll") for (int e = 0; e < CNT; ++e) v[e] = act_both<EXACT>(v[e], A, slope, d); break; }
     DGCN_ACT_CASE(DGCN_ACT_RELU)
     DGCN_ACT_CASE(DGCN_ACT_LEAKY_RELU)
     DGCN_ACT_CASE(DGCN_ACT_GELU)
@@ -195,56 +232,31 @@ __device__ __forceinline__ void act_run(float (&v)[CNT], int act, float slope) {
   }
 }
 
-template <bool EXACT>
-__device__ __forceinline__ float act_slope(float z, int act, float slope) {
+// the same in 16 bits, and the gate codes
+template <int CNT>
+__device__ __forceinline__ void act_gate_run(float (&v)[CNT], uint32_t (&c)[CNT], int act, float slope) {
+  float d;
   switch (act) {
-    case DGCN_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case DGCN_ACT_LEAKY_RELU: return z > 0.f ? 1.f : slope;
-    case DGCN_ACT_GELU: {
-      float bell;
-      const float cdf = normal_cdf<EXACT>(z, bell);
-      return fmaf(z * 0.39894228040143268f, bell, cdf);
+#define DGCN_ACT_CASE(A) case A: { _Pragma("unroll") for (int e = 0; e < CNT; ++e) { v[e] = act_both<false>(v[e], A, slope, d); c[e] = gate_encode(d); } break; }
+    case DGCN_ACT_LEAKY_RELU: {
+#pragma unroll
+      for (int e = 0; e < CNT; ++e) {
+        act_both<false>(v[e], DGCN_ACT_RELU, slope, d);
+        c[e] = gate_encode(d);
+        v[e] = act_both<false>(v[e], DGCN_ACT_LEAKY_RELU, slope, d);
+      }
+      break;
     }
-    case DGCN_ACT_SILU: {
-      const float s = EXACT ? 1.f / (1.f + act_exp<EXACT>(-z)) : __builtin_amdgcn_rcpf(1.f + act_exp<EXACT>(-z));
-      return s * (1.f + z * (1.f - s));
-    }
-    default: return 1.f;
+    DGCN_ACT_CASE(DGCN_ACT_RELU)
+    DGCN_ACT_CASE(DGCN_ACT_GELU)
+    DGCN_ACT_CASE(DGCN_ACT_SILU)
+#undef DGCN_ACT_CASE
+    default: break;
   }
-}
-
-// ---- what the backward of an activation in 16 bits keeps: act'(z) in fixed point, code = (act' + 1/4) 2^15 ----
-// gelu's and silu's slopes lie in (-0.13, 1.13); they come back within 2^-16, an eighth of a bf16 half step and less of
-// anything that is averaged.  (z in 16 bits would be off by half a step of z in act': measured, 1.5 times the error of the
-// bias gradient.)  relu and leakyrelu keep z > 0 as a slope of 1 or 0.  65535 is NaN.
-constexpr uint32_t kGateNaN = 65535u;
-
-__device__ __forceinline__ uint32_t gate_encode(float z, int act) {
-  float d = z > 0.f ? 1.f : 0.f;
-  if (act == DGCN_ACT_GELU || act == DGCN_ACT_SILU) d = act_slope<false>(z, act, 0.f);
-  const float c = fminf(fmaxf(fmaf(d, 32768.f, 8192.5f), 0.f), 65534.f);
-  return (z != z || d != d) ? kGateNaN : static_cast<uint32_t>(c);
-}
-
-__device__ __forceinline__ float gate_decode(uint32_t code, int act, float slope) {
-  const float d = fmaf(static_cast<float>(code), 1.f / 32768.f, -0.25f);
-  if (code == kGateNaN) return __builtin_nanf("");
-  return act == DGCN_ACT_LEAKY_RELU && code == 8192u ? slope : d;
 }
 
 template <int CNT>
-__device__ __forceinline__ void store_gates(uint16_t* row, int start, int n, const float (&z)[CNT], int act) {
-  uint32_t c[CNT];
-  if (act == DGCN_ACT_GELU) {
-#pragma unroll
-    for (int e = 0; e < CNT; ++e) c[e] = gate_encode(z[e], DGCN_ACT_GELU);
-  } else if (act == DGCN_ACT_SILU) {
-#pragma unroll
-    for (int e = 0; e < CNT; ++e) c[e] = gate_encode(z[e], DGCN_ACT_SILU);
-  } else {
-#pragma unroll
-    for (int e = 0; e < CNT; ++e) c[e] = gate_encode(z[e], DGCN_ACT_RELU);
-  }
+__device__ __forceinline__ void store_gates(uint16_t* row, int start, int n, const uint32_t (&c)[CNT]) {
   if (start + CNT <= n) {
     if constexpr (CNT == 8) {
       *reinterpret_cast<u4v_any2*>(row + start) = u4v{c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16};

@@ -746,11 +746,11 @@ int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width, int32_t dt
  *   in_type DGCN_T_E4M3: x_scale (rows) and w_scale (N) are required and out_type is free; otherwise out_type = in_type
  *   bias (N) in out_type or, with bias_f32, fp32, or NULL; res (rows, N) out_type, row stride ldr, or NULL
  *   z (rows, N) contiguous, or NULL: kept for the backward -- z in fp32, or in the 16-bit types act'(z) in 16-bit fixed
- *     point (code 2^-15 - 1/4; 65535 is NaN; relu and leakyrelu: z > 0 as 1 or 0); y (rows, N) out_type contiguous
+ *     point (code 2^-15 - 1/4; 0 is NaN; relu and leakyrelu: z > 0 as 1 or 0); y (rows, N) out_type contiguous
  * Backward, all in one dtype, rows >= 1:  dz = g act'(z);  dx (rows, K) = dz w, dw (N, K) = dz^T x, db (N) = sum of dz over the
  *   rows (dtype or, with db_f32, fp32), contiguous, each or NULL; z as above (NULL with DGCN_ACT_NONE)
- * Operands may start and repeat at any byte; those whose rows do not start on dwords are copied into the workspace first
- * where the product is tiled.  ws: dgcn_linear_workspace / dgcn_linear_bwd_workspace (want: 1 dx, 2 dw, 4 db) bytes for the same
+ * Operands may start and repeat at any byte; those whose rows do not start on dwords, and in the backward those whose rows
+ * repeat or overlap, are copied into the workspace first where the product is tiled.  ws: dgcn_linear_workspace / dgcn_linear_bwd_workspace (want: 1 dx, 2 dw, 4 db) bytes for the same
  * pointers, strides and sizes, 16-byte aligned, of this call's own (DGCN_E_WORKSPACE if smaller; may be 0 and NULL). */
 size_t dgcn_linear_workspace(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t in_type, int64_t rows, int32_t K,
                              int32_t N);

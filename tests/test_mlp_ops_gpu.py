@@ -359,6 +359,26 @@ def test_gradients_of_strided_and_broadcast_inputs():
         mlp_ops.rms_norm_rows_e4m3(h0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [5, 70, 200])
+def test_gradients_of_rows_that_repeat_or_overlap(dtype, rows):
+    """One row expanded over all, windows of a line that overlap, a weight likewise, and a gradient that is one row expanded
+    (of y.sum(0)): sums over `rows` rows, not over a tile's."""
+    row, line = rand(36, dtype=dtype, seed=1), rand(4 * rows + 100, dtype=dtype, seed=2)
+    wline, grow = rand(400, dtype=dtype, seed=3, scale=0.2), rand(24, dtype=dtype, seed=4)
+    w = wline.as_strided((24, 36), (8, 1))
+    for x in (row.expand(rows, 36), line.as_strided((rows, 36), (4, 1))):
+        xg, wg = x.detach().requires_grad_(), w.detach().requires_grad_()
+        b = torch.zeros(24, device="cuda", dtype=dtype).requires_grad_()
+        assert xg.stride(0) in (0, 4) and wg.stride(0) == 8
+        for bias in (None, b):
+            y = mlp_ops.linear_act(xg, wg, bias)
+            g = grow.expand(rows, 24)
+            grads = torch.autograd.grad(y, [t for t in (xg, wg, bias) if t is not None], g)
+            z, ez = check_linear(x, w, None if bias is None else b.detach(), None, "none", y.detach(), dtype)
+            check_linear_grads(x, w, None if bias is None else b.detach(), None, "none", g, grads, z, ez, dtype)
+
+
 def test_gradients_against_differences():
     """<grad, v> against (f(x + s v) - f(x - s v)) / 2 s, f = <y, g> summed in 64 bits, s a power of two.  Bound: what the
     same difference of the 64-bit reference is off by (truncation), and twice the outputs' bound over 2 s."""
