@@ -1,4 +1,4 @@
-"""Build libdgcn.so (hipcc, gfx950 only) in-tree.
+"""Build libdgcn.so (hipcc, gfx950 only) and the host extension _mlp_host.so in-tree.
 
     python -m deep_gcns_torch_amd.build [--force] [--verbose]
 
@@ -20,6 +20,8 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 OBJ = CSRC / "_obj"
 LIB = CSRC / "libdgcn.so"
+HOST_SRC = CSRC / "mlp_host.cpp"
+HOST_LIB = PKG / "_mlp_host.so"
 ARCH = "gfx950"
 # no packed fp32 instructions (v_pk_fma_f32 and its like, which -O3 makes of ordinary float code): some of their forms have
 # given wrong results on this device now and then.  The host pass warns that it does not know the feature: harmless.
@@ -83,13 +85,39 @@ def _compile_one(src: Path, force: bool, verbose: bool) -> Path:
     return obj
 
 
+def _build_host(force: bool, verbose: bool) -> None:
+    """csrc/mlp_host.cpp against torch's headers: host code only, it is handed libdgcn's entry points at run time."""
+    if (not force and HOST_LIB.exists()
+            and HOST_LIB.stat().st_mtime > max(HOST_SRC.stat().st_mtime, (INCLUDE / "dgcn.h").stat().st_mtime)):
+        return
+    import sysconfig
+
+    import torch
+    t = Path(torch.__file__).resolve().parent
+    rocm = Path(hipcc_path()).resolve().parent.parent
+    system = [t / "include", t / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
+              rocm / "include"]
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-Wall", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__",
+           "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-DTORCH_EXTENSION_NAME=_mlp_host", *(x for d in system for x in ("-isystem", str(d))), f"-I{INCLUDE}",
+           str(HOST_SRC), "-o", str(HOST_LIB), f"-L{t / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+           "-ltorch"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"host compiler failed for {HOST_SRC.name}:\n{r.stdout}\n{r.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.hip"))
     if not srcs:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+        host = ex.submit(_build_host, force, verbose)
         objs = list(ex.map(lambda s: _compile_one(s, force, verbose), srcs))
+        host.result()
     stale = force or not LIB.exists() or any(o.stat().st_mtime > LIB.stat().st_mtime for o in objs)
     if stale:
         # No rpath to /opt/rocm: at run time the HIP runtime must be the one the host process

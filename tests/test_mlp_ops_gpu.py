@@ -493,6 +493,84 @@ def test_other_stream_and_repeatability():
     assert all(torch.equal(r, want) for r in runs)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_second_derivative(dtype):
+    """create_graph gives the same gradients; what differentiates them again raises instead of seeing constants."""
+    x, w = rand(7, 40, dtype=dtype, seed=1).requires_grad_(), rand(24, 40, dtype=dtype, seed=2).requires_grad_()
+    b, r = rand(24, dtype=dtype, seed=3).requires_grad_(), rand(7, 24, dtype=dtype, seed=4).requires_grad_()
+    n, s = rand(40, dtype=dtype, seed=5).requires_grad_(), rand(7, 40, dtype=dtype, seed=6).requires_grad_()
+    for out, leaves in ((mlp_ops.linear_act(x, w, b, "silu", r), (x, w, b, r)), (mlp_ops.rms_norm_rows(x, n, 1e-6, s)[0], (x, n, s))):
+        first = torch.autograd.grad(out, leaves, torch.ones_like(out), retain_graph=True)
+        again = torch.autograd.grad(out, leaves, torch.ones_like(out), create_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(first, again))
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            again[0].float().square().sum().backward()
+
+
+def test_only_some_inputs_need_gradients():
+    """Each subset of the inputs that asks for a gradient gets the one that it gets among all."""
+    dtype = torch.bfloat16
+    make = [lambda: rand(33, 64, dtype=dtype, seed=1), lambda: rand(48, 64, dtype=dtype, seed=2, scale=0.2),
+            lambda: rand(48, dtype=torch.float32, seed=3), lambda: rand(33, 48, dtype=dtype, seed=4)]
+    norm = [lambda: rand(33, 64, dtype=dtype, seed=1), lambda: rand(64, dtype=torch.float32, seed=2),
+            lambda: rand(33, 64, dtype=dtype, seed=3)]
+
+    def linear(t):
+        return mlp_ops.linear_act(t[0], t[1], t[2], "gelu", t[3])
+
+    def rms(t):
+        y, h = mlp_ops.rms_norm_rows(t[0], t[1], 1e-6, t[2])
+        return y + h
+    for inputs, op in ((make, linear), (norm, rms)):
+        for absent in (None, 2, 3)[:len(inputs) - 1]:
+            want = None
+            for mask in reversed(range(1, 1 << len(inputs))):
+                t = [f() for f in inputs]
+                if absent is not None and op is linear:
+                    if mask >> absent & 1:
+                        continue
+                    t[absent] = None
+                for k, v in enumerate(t):
+                    if mask >> k & 1:
+                        v.requires_grad_()
+                out = op(t)
+                out.backward(rand(*out.shape, dtype=dtype, seed=9))
+                got = {k: v.grad for k, v in enumerate(t) if v is not None}
+                want = want or got
+                for k, v in got.items():
+                    assert torch.equal(v, want[k]) if mask >> k & 1 else v is None
+
+
+def test_calls_from_threads_on_their_own_streams():
+    """Calls at once share no memory: each thread's forward and backward on its own stream gives what it gives alone."""
+    import threading
+    dtype = torch.bfloat16
+    w = rand(520, 264, dtype=dtype, seed=2, scale=0.1)
+    xs = [rand(300 + 8 * k, 264, dtype=dtype, seed=10 + k) for k in range(4)]
+
+    def step(x):
+        a, v = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = mlp_ops.linear_act(mlp_ops.rms_norm_rows(a), v, act="gelu")
+        return [y.detach(), *torch.autograd.grad(y, (a, v), torch.ones_like(y))]
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    got = [None] * len(xs)
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(8):
+                got[k] = step(xs[k])
+            stream.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        assert a is not None and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
 def test_norm_layer_and_pre_activation():
     from deep_gcns_torch_amd import node_ops
     from deep_gcns_torch_amd.gcn_lib.sparse.torch_nn import MLP, norm_layer
