@@ -164,24 +164,39 @@ inline GateShape gate_shape(int64_t rows, int N) {
   return S;
 }
 
-// rows of C bytes -> rows of ldo bytes (ldo a multiple of 16, less than 16 more than C), zeros behind; 16 bytes a thread
-__global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* __restrict__ x, int64_t ldx, uint8_t* __restrict__ out,
-                                                       int64_t ldo, int64_t rows, int64_t C) {
+// rows of C bytes -> rows of ldo bytes (ldo a multiple of 16, less than 16 more than C), zeros behind; 16 bytes a thread, one
+// or two matrices a launch (a launch costs as much as a copy of 2 MB: fp16 1021 x 1013 and 2047 x 1013 take 6 us, in two launches 9)
+struct PadJob {
+  const uint8_t* x;
+  int64_t ldx;
+  uint8_t* out;
+  int64_t ldo, rows, C;
+  unsigned wgs;
+};
+struct PadJobs {
+  PadJob job[2];
+  int n;
+};
+
+__global__ __launch_bounds__(256) void pad_rows_kernel(const PadJobs jobs) {
   typedef u4v u4v_any1 __attribute__((aligned(1)));
-  const int64_t per = ldo / 16, total = rows * per;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; it < total; it += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t r = it / per, at = (it - r * per) * 16;
-    const uint8_t* p = x + r * ldx + at;
+  const bool second = blockIdx.x >= jobs.job[0].wgs;
+  const PadJob& J = jobs.job[second];
+  const int64_t per = J.ldo / 16, total = J.rows * per;
+  for (int64_t it = static_cast<int64_t>(blockIdx.x - (second ? jobs.job[0].wgs : 0)) * 256 + threadIdx.x; it < total; it += static_cast<int64_t>(J.wgs) * 256) {
+    // (a 64-bit division is as long as the rest)
+    const int64_t r = total <= 0xffffffff ? static_cast<uint32_t>(it) / static_cast<uint32_t>(per) : it / per, at = (it - r * per) * 16;
+    const uint8_t* p = J.x + r * J.ldx + at;
     u4v v = {0, 0, 0, 0};
-    if (at + 16 <= C) {
+    if (at + 16 <= J.C) {
       v = *reinterpret_cast<const u4v_any1*>(p);
     } else {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        if (at + e < C) v[e >> 2] |= static_cast<uint32_t>(p[e]) << (8 * (e & 3));
+        if (at + e < J.C) v[e >> 2] |= static_cast<uint32_t>(p[e]) << (8 * (e & 3));
       }
     }
-    *reinterpret_cast<u4v*>(out + r * ldo + at) = v;
+    *reinterpret_cast<u4v*>(J.out + r * J.ldo + at) = v;
   }
 }
 
@@ -218,19 +233,21 @@ inline bool operand_ready(const void* p, int64_t ld, int es, int64_t span) {
   return ld >= span && (reinterpret_cast<uintptr_t>(p) & 3) == 0 && ld * es % 4 == 0 && ld <= kFarStride;
 }
 
-int operand(const void* p, int64_t ld, int64_t rows, int64_t C, bool strided, int es, Arena& ws, bool launch, hipStream_t s,
-            Operand* out) {
-  *out = {p, ld};
-  if (operand_ready(p, ld, es, strided ? C : 0)) return DGCN_OK;
+// p's rows as an operand; where they are not ready, the copy that makes them so is added to the jobs (at most two)
+Operand operand(const void* p, int64_t ld, int64_t rows, int64_t C, bool strided, int es, Arena& ws, PadJobs* jobs) {
+  if (operand_ready(p, ld, es, strided ? C : 0)) return {p, ld};
   const int64_t ldo = round16(C * es);
-  uint8_t* to = static_cast<uint8_t*>(ws.take(rows * ldo));
-  *out = {to, ldo / es};
-  if (!launch) return DGCN_OK;
-  if (ws.full()) return DGCN_E_WORKSPACE;
   int64_t wgs = (rows * (ldo / 16) + 255) / 256;
   if (wgs > 32 * num_cus()) wgs = 32 * num_cus();
-  hipLaunchKernelGGL(pad_rows_kernel, dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, static_cast<const uint8_t*>(p), ld * es,
-                     to, ldo, rows, C * es);
+  uint8_t* to = static_cast<uint8_t*>(ws.take(rows * ldo));
+  jobs->job[jobs->n++] = {static_cast<const uint8_t*>(p), ld * es, to, ldo, rows, C * es, static_cast<unsigned>(wgs)};
+  return {to, ldo / es};
+}
+
+int pad_launch(const PadJobs& jobs, const Arena& ws, hipStream_t s) {
+  if (ws.full()) return DGCN_E_WORKSPACE;
+  if (jobs.n == 0) return DGCN_OK;
+  hipLaunchKernelGGL(pad_rows_kernel, dim3(jobs.job[0].wgs + (jobs.n > 1 ? jobs.job[1].wgs : 0)), dim3(256), 0, s, jobs);
   return launch_status();
 }
 
@@ -275,10 +292,12 @@ int linear_forward(MatParams P, int in_type, int out_type, Arena& ws, bool launc
   // over the tile's workgroups, 1024 x 8192 12 - 17 against 11, 512 x 4096 7 - 9 against 8.
   const bool narrow = P.N < 8 * static_cast<int64_t>(num_cus()) && P.K * es >= 16384;
   if (P.M <= (ready ? 16 : 32) && !(ready && narrow)) return launch ? small_run(P, in_type, out_type, s) : DGCN_OK;
-  Operand a, b;
-  int rc = operand(P.a, P.lda, P.M, P.K, false, es, ws, launch, s, &a);
-  if (rc == DGCN_OK) rc = operand(P.b, P.ldb, P.N, P.K, false, es, ws, launch, s, &b);
-  if (rc != DGCN_OK) return rc;
+  PadJobs pads = {};
+  const Operand a = operand(P.a, P.lda, P.M, P.K, false, es, ws, &pads), b = operand(P.b, P.ldb, P.N, P.K, false, es, ws, &pads);
+  if (launch) {
+    const int rc = pad_launch(pads, ws, s);
+    if (rc != DGCN_OK) return rc;
+  }
   P.a = a.p; P.lda = a.ld; P.b = b.p; P.ldb = b.ld;
   return mat_run(P, 0, 0, in_type, out_type, ws, launch, s);
 }
@@ -316,13 +335,13 @@ int gate_launch(const BwdArgs& A, const GateShape& S, void* dz, int64_t lddz, fl
 
 int linear_backward(const BwdArgs& A, Arena& ws, bool launch, hipStream_t s) {
   const int es = type_bytes(A.type);
-  Operand dz = {A.g, A.ldg};
-  const bool products = A.dx || A.dw;
+  const bool products = A.dx || A.dw, ready = operand_ready(A.g, A.ldg, es, A.dw ? A.N : 0);
+  Operand dz = {A.g, A.ldg}, w = {}, x = {};
   int rc = DGCN_OK;
-  if (A.act != DGCN_ACT_NONE || A.db) {
+  if (A.act != DGCN_ACT_NONE || A.db || (products && !ready)) {
     const GateShape S = gate_shape(A.rows, A.N);
     void* to = nullptr;
-    if (A.act != DGCN_ACT_NONE || (products && !operand_ready(A.g, A.ldg, es, A.dw ? A.N : 0))) {
+    if (A.act != DGCN_ACT_NONE || (products && !ready)) {
       const int64_t ld = round16(static_cast<int64_t>(A.N) * es) / es;
       to = ws.take(A.rows * ld * es);
       dz = {to, ld};
@@ -338,21 +357,13 @@ int linear_backward(const BwdArgs& A, Arena& ws, bool launch, hipStream_t s) {
       if (rc == DGCN_OK && A.db) rc = dgcn_param_sum(part, S.gy, A.N, A.db_f32 ? DGCN_T_F32 : A.type, A.db, s);
       if (rc != DGCN_OK) return rc;
     }
-  } else if (products) {
-    rc = operand(A.g, A.ldg, A.rows, A.N, A.dw != nullptr, es, ws, launch, s, &dz);
-    if (rc != DGCN_OK) return rc;
   }
-  if (A.dx) {
-    Operand w;
-    rc = operand(A.w, A.ldw, A.N, A.K, true, es, ws, launch, s, &w);
-    if (rc == DGCN_OK) rc = mat_run(plain_product(dz, w, A.dx, A.rows, A.K, A.N), 0, 1, A.type, A.type, ws, launch, s);
-    if (rc != DGCN_OK) return rc;
-  }
-  if (A.dw) {
-    Operand x;
-    rc = operand(A.x, A.ldx, A.rows, A.K, true, es, ws, launch, s, &x);
-    if (rc == DGCN_OK) rc = mat_run(plain_product(dz, x, A.dw, A.N, A.K, A.rows), 1, 1, A.type, A.type, ws, launch, s);
-  }
+  PadJobs pads = {};
+  if (A.dx) w = operand(A.w, A.ldw, A.N, A.K, true, es, ws, &pads);
+  if (A.dw) x = operand(A.x, A.ldx, A.rows, A.K, true, es, ws, &pads);
+  if (launch) rc = pad_launch(pads, ws, s);
+  if (A.dx && rc == DGCN_OK) rc = mat_run(plain_product(dz, w, A.dx, A.rows, A.K, A.N), 0, 1, A.type, A.type, ws, launch, s);
+  if (A.dw && rc == DGCN_OK) rc = mat_run(plain_product(dz, x, A.dw, A.N, A.K, A.rows), 1, 1, A.type, A.type, ws, launch, s);
   return rc;
 }
 
