@@ -5,7 +5,12 @@
 // Bound by the matrix pipe and its power (large products) or by HBM (long thin ones).  A stage is computed in two halves.
 // The fragments of a half lie in registers already while the next half's are read from LDS, and the stage after next is
 // requested as soon as every wave has read the second half of this one: the matrix instructions wait for neither, and a
-// stage costs one barrier.
+// stage costs one barrier.  (Four to six stages under way, for grids of one workgroup a CU, change nothing: 1024 x 1024 x 2048
+// fp16 12.0 us with two, 12.1 with three, 12.9 with six.)
+//
+// Measured: 8192 x 4096 x 16,384 bf16 1.01 ms forward with gelu (1.09 PFLOP/s; the library's bare product 0.88), 0.88 dx and
+// 0.91 dw (1.25, 1.21); 8192^3 e4m3 0.49 ms (2.26 PFLOP/s; the library 0.36); 169,343 x 128 x 256 fp32 0.150 ms forward (2.9
+// TB/s with z), 0.090 dx, 0.073 dw.
 #pragma once
 
 #include <type_traits>

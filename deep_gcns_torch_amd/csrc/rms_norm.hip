@@ -11,6 +11,10 @@
 // h is that sum rounded to the rows' type, and the backward reads the stored one (half a step of h off in xh, as is
 // any layer that reads h).  The weight's gradient stays in registers over all rows of a workgroup and leaves as one
 // partial per workgroup, summed in a fixed order by a second launch: no atomics, the same bits every time.
+//
+// Measured (a copy of 1 GiB reaches 5.1 TB/s; what fits the 256 MB of memory-side cache goes faster): 16,384 x 4096 bf16 with
+// residual 86 us forward (6.2 TB/s over x, r, h, y) and 114 us backward (4.7 over g, g_h, h, gx); 169,343 x 128 fp32 28 and
+// 48 us (6.2 and 5.5); to e4m3 rows 8192 x 8192 bf16 with residual 114 us (4.1), the rounding alone of 8192 x 16,384 91 us (4.4).
 
 #include "mlp_common.h"
 
