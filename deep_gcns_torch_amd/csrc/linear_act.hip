@@ -99,12 +99,13 @@ int split_join(const MatParams& P, hipStream_t s) {
 }
 
 // dz = g act'(z), and the column sums of dz over a slab of rows: CL lanes (eight channels each) across, 256 / CL rows at
-// a time; a workgroup takes the rows blockIdx.y * slab .. and leaves one partial sum per channel.  HBM: 8192 x 16,384 bf16
+// a time; a workgroup takes the rows blockIdx.y * slab .. and leaves one partial sum per channel
+// (one slab: the bias gradient itself).  HBM: 8192 x 16,384 bf16
 // 167 us, 169,343 x 256 fp32 109 us, both 4.8 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void gate_kernel(const T* __restrict__ g, int64_t ldg, const void* __restrict__ z, int act,
                                                    float slope, T* __restrict__ dz, int64_t lddz, float* __restrict__ part,
-                                                   int64_t rows, int N, int cl, int64_t slab) {
+                                                   void* __restrict__ db, int db_f32, int64_t rows, int N, int cl, int64_t slab) {
   __shared__ float red[256 * 8];
   const int lane = threadIdx.x % cl, slot = threadIdx.x / cl, slots = 256 / cl;
   const int at = (blockIdx.x * cl + lane) * 8;
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(256) void gate_kernel(const T* __restrict__ g, int6
       for (int e = 0; e < 8; ++e) sum[e] += d[e];
     }
   }
-  if (!part) return;
+  if (!db) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) red[(slot * cl + lane) * 8 + e] = sum[e];
   __syncthreads();
@@ -137,7 +138,13 @@ __global__ __launch_bounds__(256) void gate_kernel(const T* __restrict__ g, int6
     if (col < N) {
       float t = 0.f;
       for (int sl = 0; sl < slots; ++sl) t += red[sl * cl * 8 + c];
-      part[static_cast<int64_t>(blockIdx.y) * N + col] = t;
+      if (gridDim.y > 1) {
+        part[static_cast<int64_t>(blockIdx.y) * N + col] = t;
+      } else if (db_f32) {
+        static_cast<float*>(db)[col] = t;
+      } else {
+        static_cast<T*>(db)[col] = static_cast<T>(t);
+      }
     }
   }
 }
@@ -329,7 +336,7 @@ inline MatParams plain_product(Operand a, Operand b, void* y, int64_t M, int64_t
 template <class T>
 int gate_launch(const BwdArgs& A, const GateShape& S, void* dz, int64_t lddz, float* part, hipStream_t s) {
   hipLaunchKernelGGL(gate_kernel<T>, dim3(S.gx, S.gy), dim3(256), 0, s, static_cast<const T*>(A.g), A.ldg, A.z, A.act, A.slope,
-                     static_cast<T*>(dz), lddz, part, A.rows, A.N, S.cl, S.slab);
+                     static_cast<T*>(dz), lddz, part, A.db, A.db_f32, A.rows, A.N, S.cl, S.slab);
   return launch_status();
 }
 
@@ -346,7 +353,7 @@ int linear_backward(const BwdArgs& A, Arena& ws, bool launch, hipStream_t s) {
       to = ws.take(A.rows * ld * es);
       dz = {to, ld};
     }
-    float* part = A.db ? static_cast<float*>(ws.take(static_cast<size_t>(S.gy) * A.N * sizeof(float))) : nullptr;
+    float* part = A.db && S.gy > 1 ? static_cast<float*>(ws.take(static_cast<size_t>(S.gy) * A.N * sizeof(float))) : nullptr;
     if (launch) {
       if (ws.full()) return DGCN_E_WORKSPACE;
       switch (A.type) {
@@ -354,7 +361,7 @@ int linear_backward(const BwdArgs& A, Arena& ws, bool launch, hipStream_t s) {
         case DGCN_T_BF16: rc = gate_launch<__bf16>(A, S, to, dz.ld, part, s); break;
         default: rc = gate_launch<_Float16>(A, S, to, dz.ld, part, s); break;
       }
-      if (rc == DGCN_OK && A.db) rc = dgcn_param_sum(part, S.gy, A.N, A.db_f32 ? DGCN_T_F32 : A.type, A.db, s);
+      if (rc == DGCN_OK && part) rc = dgcn_param_sum(part, S.gy, A.N, A.db_f32 ? DGCN_T_F32 : A.type, A.db, s);
       if (rc != DGCN_OK) return rc;
     }
   }

@@ -6,7 +6,8 @@
 // The fragments of a half lie in registers already while the next half's are read from LDS, and the stage after next is
 // requested as soon as every wave has read the second half of this one: the matrix instructions wait for neither, and a
 // stage costs one barrier.  (Four to six stages under way, for grids of one workgroup a CU, change nothing: 1024 x 1024 x 2048
-// fp16 12.0 us with two, 12.1 with three, 12.9 with six.)
+// fp16 12.0 us with two, 12.1 with three, 12.9 with six.  Nor do four waves of 128 x 128 with a third fewer LDS reads: 8192^3 e4m3
+// 463 us against 416, 8192 x 4096 x 16,384 bf16 944 against 878: one wave a SIMD leaves the pipe idle at each barrier.)
 //
 // Measured: 8192 x 4096 x 16,384 bf16 1.01 ms forward with gelu (1.09 PFLOP/s; the library's bare product 0.88), 0.88 dx and
 // 0.91 dw (1.25, 1.21); 8192^3 e4m3 0.49 ms (2.26 PFLOP/s; the library 0.36); 169,343 x 128 x 256 fp32 0.150 ms forward (2.9
@@ -432,9 +433,11 @@ int tile_launch(const MatParams& P, hipStream_t s) {
   // 32-bit offsets inside a tile's lines, 31-bit tile count
   const int64_t far = 4 * 256 * (P.lda > P.ldb ? P.lda : P.ldb);
   if (tiles > 0x7fffffff || far + 2 * 128 * 256 > 0x7fffffff || P.splits < 1 || P.splits > 65535) return DGCN_E_SHAPE;
-  const void* fn = reinterpret_cast<const void*>(tile_kernel<T, O, TA, TB, TM, WM, WN>);
-  const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-  if (e != hipSuccess) return static_cast<int>(e);
+  if constexpr (LDS > 64 * 1024) {                                      // (a call costs as much host time as a small launch)
+    const void* fn = reinterpret_cast<const void*>(tile_kernel<T, O, TA, TB, TM, WM, WN>);
+    const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) return static_cast<int>(e);
+  }
   hipLaunchKernelGGL((tile_kernel<T, O, TA, TB, TM, WM, WN>), dim3(static_cast<unsigned>(tiles), P.splits), dim3(WM * WN * 64), LDS, s, P);
   return launch_status();
 }
