@@ -227,6 +227,9 @@ struct Arena {
   bool full() const { return used > size; }
 };
 
+// Rows off dwords are copied rather than read in place: a tile that takes them through registers, dwords and byte shifts, runs
+// fp16 1021 x 1013 x 2047 in 24.7 us against 25.8, but 4096 x 4095 x 4096 in 250 against 148 (it wins where a few rows meet a large
+// weight: 33 x 8191 x 8192 40 against 91; up to 32 rows the small kernel reads in place).
 // An operand as the tiled kernel takes it: rows that start on dwords, and, where they are the k-rows of a K-strided operand
 // (span: their C values), that do not repeat or overlap -- the k-rows behind the last one have to lie behind the buffer's end
 struct Operand {

@@ -93,3 +93,13 @@ def test_norm_layer_offers_rms():
     from deep_gcns_torch_amd.gcn_lib.sparse.torch_nn import norm_layer
     m = norm_layer("rms", 12)
     assert isinstance(m, mlp_ops.RMSNorm) and list(m.state_dict()) == ["weight"] and m.weight.shape == (12,)
+
+
+def test_missing_host_extension_raises(monkeypatch):
+    import sys
+    import deep_gcns_torch_amd
+    monkeypatch.setattr(mlp_ops, "_host", None)
+    monkeypatch.delattr(deep_gcns_torch_amd, "_mlp_host", raising=False)
+    monkeypatch.setitem(sys.modules, "deep_gcns_torch_amd._mlp_host", None)
+    with pytest.raises(RuntimeError, match="python -m deep_gcns_torch_amd.build"):
+        mlp_ops.quantize_rows(torch.zeros(2, 8))
