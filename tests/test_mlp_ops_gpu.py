@@ -629,3 +629,17 @@ def test_norm_layer_and_pre_activation():
     assert skip is x
     mlp = MLP([64, 128, 32], norm="rms", last_lin=True).cuda()
     assert mlp(x).shape == (500, 32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, C", [(300, 128), (64, 1001), (40, 4096), (16, 16384), (3, 32768)])
+def test_rows_e4m3_are_divided(dtype, rows, C):
+    """The bits of the same thing in torch, ties included: scale = max|x| / 448, q = x / scale (both rounded to fp32, q then to e4m3)."""
+    x = rand(rows, C, dtype=dtype, seed=1, scale=3.0).float()
+    x[0] *= 1e-36 if dtype != torch.float16 else 1.0                # a scale among the least normal numbers
+    x = x.to(dtype)
+    q = mlp_ops.quantize_rows(x)
+    scale = x.float().abs().amax(-1) / 448.0
+    assert torch.equal(q.scale, scale.clamp_min(torch.finfo(torch.float32).tiny))
+    want = (x.float() / q.scale.unsqueeze(-1)).to(torch.float8_e4m3fn)
+    assert torch.equal(q.data.view(torch.uint8), want.view(torch.uint8))
