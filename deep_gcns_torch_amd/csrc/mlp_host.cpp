@@ -29,7 +29,7 @@ using OptTensor = std::optional<Tensor>;
 constexpr int64_t kMaxNormC = 32768, kMaxK = int64_t{1} << 20;
 
 #define ENTRY_POINTS(X) \
-  X(rms_norm_fwd) X(rms_norm_num_partials) X(rms_norm_bwd) X(quantize_rows_e4m3) X(linear_workspace) X(linear_act) \
+  X(rms_norm_fwd) X(rms_norm_num_partials) X(rms_norm_sum_bwd) X(quantize_rows_e4m3) X(linear_workspace) X(linear_act) \
   X(linear_bwd_workspace) X(linear_bwd) X(strerror)
 
 struct {
@@ -155,7 +155,7 @@ struct RmsFn : torch::autograd::Function<RmsFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps) {
     ctx->set_materialize_grads(false);
     const Rms o = rms_run(x, weight, residual, eps, false, true);
-    ctx->save_for_backward({residual.has_value() ? o.h : x, weight.has_value() ? *weight : Tensor(), o.rstd});
+    ctx->save_for_backward({x, weight.has_value() ? *weight : Tensor(), o.rstd, residual.has_value() ? *residual : Tensor()});
     ctx->saved_data["weight"] = weight.has_value();
     ctx->saved_data["residual"] = residual.has_value();
     if (residual.has_value()) return {o.y, o.h};
@@ -167,31 +167,31 @@ struct RmsFn : torch::autograd::Function<RmsFn> {
   static variable_list run(AutogradContext* ctx, const variable_list& grads) {
     const bool has_w = ctx->saved_data["weight"].toBool(), has_r = ctx->saved_data["residual"].toBool();
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &h = saved[0], &weight = saved[1], &rstd = saved[2];
+    const Tensor &x = saved[0], &weight = saved[1], &rstd = saved[2], &residual = saved[3];
     const bool need_x = ctx->needs_input_grad(0), need_w = has_w && ctx->needs_input_grad(1);
     const bool need_r = has_r && ctx->needs_input_grad(has_w ? 2 : 1);
     const Tensor g = grads[0], gh = has_r ? grads[1] : Tensor();
     Tensor dx, dw;
-    if (!g.defined() || h.numel() == 0) {                     // only the sum was used: its gradient is both inputs'
-      dx = gh.defined() ? gh : at::zeros_like(h);
+    if (!g.defined() || x.numel() == 0) {                     // only the sum was used: its gradient is both inputs'
+      dx = gh.defined() ? gh : at::zeros_like(x);
       if (need_w) dw = at::zeros_like(weight);
     } else {
-      const Rows rh(h), rg(g), rgh = gh.defined() ? Rows(gh) : Rows();
-      const int64_t rows = rh.rows();
-      const int32_t C = static_cast<int32_t>(h.size(-1));
+      const Rows rx(x), rg(g), rgh = gh.defined() ? Rows(gh) : Rows(), rr = has_r ? Rows(residual) : Rows();
+      const int64_t rows = rx.rows();
+      const int32_t C = static_cast<int32_t>(x.size(-1));
       const Tensor w = has_w ? param(weight) : Tensor();
       Tensor parts;
-      if (need_x || need_r) dx = at::empty(h.sizes(), h.options());
+      if (need_x || need_r) dx = at::empty(x.sizes(), x.options());
       if (need_w) {
         dw = at::empty({C}, weight.options());
-        parts = at::empty({lib.rms_norm_num_partials(rows, C), C}, h.options().dtype(at::kFloat));
+        parts = at::empty({lib.rms_norm_num_partials(rows, C), C}, x.options().dtype(at::kFloat));
       }
       if (dx.defined() || need_w) {
-        const Place at_(h);
-        check(lib.rms_norm_bwd(rg.p(), rg.ld, rgh.p(), rgh.ld, rh.p(), rh.ld, param_ptr(w), is_f32(w), rstd.data_ptr<float>(),
-                               row_type(h.scalar_type()), dx.defined() ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr,
-                               need_w ? parts.data_ptr<float>() : nullptr, rows, C, at_.stream),
-              "dgcn_rms_norm_bwd");
+        const Place at_(x);
+        check(lib.rms_norm_sum_bwd(rg.p(), rg.ld, rgh.p(), rgh.ld, rx.p(), rx.ld, rr.p(), rr.ld, param_ptr(w), is_f32(w), rstd.data_ptr<float>(),
+                                   row_type(x.scalar_type()), dx.defined() ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr,
+                                   need_w ? parts.data_ptr<float>() : nullptr, rows, C, at_.stream),
+              "dgcn_rms_norm_sum_bwd");
       }
     }
     return {need_x ? dx : Tensor(), need_w ? dw : Tensor(), need_r ? dx : Tensor(), Tensor()};

@@ -7,9 +7,10 @@
 //
 // What bounds it: HBM.  A row is read once into registers (eight elements a chunk, NV chunks a lane, one to sixteen
 // waves or a part of a wave a row), the sum of squares is joined by shuffles (and LDS between waves), and everything
-// that depends on the row is written from the same registers.  The statistics use the fp32 sum x + r; what is stored of
-// h is that sum rounded to the rows' type, and the backward reads the stored one (half a step of h off in xh, as is
-// any layer that reads h).  The weight's gradient stays in registers over all rows of a workgroup and leaves as one
+// that depends on the row is written from the same registers.  The statistics use the fp32 sum x + r, of which h is the
+// rounding to the rows' type; the backward adds x and r again (the stored h instead is one row less to read and to keep,
+// 16,384 x 4096 bf16 114 us against 141, but half a step of it is off in every term of the weight's gradient: bf16 2.3e-3 of its
+// norm against 1.7e-3 that its own rounding costs).  The weight's gradient stays in registers over all rows of a workgroup and leaves as one
 // partial per workgroup, summed in a fixed order by a second launch: no atomics, the same bits every time.
 //
 // Measured (a copy of 1 GiB reaches 5.1 TB/s; what fits the 256 MB of memory-side cache goes faster): 16,384 x 4096 bf16 with
@@ -174,8 +175,10 @@ struct RmsBwdParams {
   int64_t ldg;
   const void* gh;     // gradient of h, or null
   int64_t ldgh;
-  const void* h;
-  int64_t ldh;
+  const void* x;
+  int64_t ldx;
+  const void* res;    // h = x + res in fp32, or null: h = x
+  int64_t ldr;
   const void* w;
   int32_t w_f32;
   int32_t C;
@@ -211,8 +214,20 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_bwd_kernel(const Rm
 #pragma unroll
       for (int e = 0; e < 8; ++e) { g[i][e] = 0.f; h[i][e] = 0.f; }
       if (at < C) {
-        load_chunk(static_cast<const T*>(P.h) + row * P.ldh, at, C, h[i]);
+        load_chunk(static_cast<const T*>(P.x) + row * P.ldx, at, C, h[i]);
         load_chunk(static_cast<const T*>(P.g) + row * P.ldg, at, C, g[i]);
+      }
+    }
+    if (P.res) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int at = (lane + i * LPR) * 8;
+        if (at < C) {
+          float r[8];
+          load_chunk(static_cast<const T*>(P.res) + row * P.ldr, at, C, r);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[i][e] += r[e];
+        }
       }
     }
 #pragma unroll
@@ -430,12 +445,12 @@ extern "C" int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width,
   return launch_status();
 }
 
-extern "C" int dgcn_rms_norm_bwd(const void* g, int64_t ldg, const void* gh, int64_t ldgh, const void* h, int64_t ldh,
-                                 const void* w, int32_t w_f32, const float* rstd, int32_t dtype, void* dx, void* dw,
-                                 float* dw_part, int64_t rows, int32_t C, void* stream) {
-  if (!g || !h || !rstd || (!dx && !dw) || (dw && !dw_part)) return DGCN_E_NULL;
-  if (rows < 1 || C < 1 || C > kRmsMaxC || ldg < 0 || ldh < 0 || (gh && ldgh < 0)) return DGCN_E_SHAPE;
-  const RmsBwdParams P = {g, ldg, gh, ldgh, h, ldh, w, w_f32, C, rstd, rows, dx, dw ? dw_part : nullptr};
+extern "C" int dgcn_rms_norm_sum_bwd(const void* g, int64_t ldg, const void* gh, int64_t ldgh, const void* x, int64_t ldx,
+                                     const void* res, int64_t ldr, const void* w, int32_t w_f32, const float* rstd,
+                                     int32_t dtype, void* dx, void* dw, float* dw_part, int64_t rows, int32_t C, void* stream) {
+  if (!g || !x || !rstd || (!dx && !dw) || (dw && !dw_part)) return DGCN_E_NULL;
+  if (rows < 1 || C < 1 || C > kRmsMaxC || ldg < 0 || ldx < 0 || (gh && ldgh < 0) || (res && ldr < 0)) return DGCN_E_SHAPE;
+  const RmsBwdParams P = {g, ldg, gh, ldgh, x, ldx, res, ldr, w, w_f32, C, rstd, rows, dx, dw ? dw_part : nullptr};
   hipStream_t s = static_cast<hipStream_t>(stream);
   int rc = DGCN_E_MODE;
   switch (dtype) {
@@ -446,4 +461,10 @@ extern "C" int dgcn_rms_norm_bwd(const void* g, int64_t ldg, const void* gh, int
   }
   if (rc != DGCN_OK || !dw) return rc;
   return dgcn_param_sum(dw_part, static_cast<int32_t>(rms_bwd_grid(rows, C)), C, w_f32 ? DGCN_T_F32 : dtype, dw, stream);
+}
+
+extern "C" int dgcn_rms_norm_bwd(const void* g, int64_t ldg, const void* gh, int64_t ldgh, const void* h, int64_t ldh,
+                                 const void* w, int32_t w_f32, const float* rstd, int32_t dtype, void* dx, void* dw,
+                                 float* dw_part, int64_t rows, int32_t C, void* stream) {
+  return dgcn_rms_norm_sum_bwd(g, ldg, gh, ldgh, h, ldh, nullptr, 0, w, w_f32, rstd, dtype, dx, dw, dw_part, rows, C, stream);
 }

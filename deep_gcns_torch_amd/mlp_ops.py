@@ -112,8 +112,8 @@ def rms_norm_rows(x, weight=None, eps: float = 1e-6, residual=None):
     """``h = x [+ residual]``, ``y = h * rsqrt(mean(h^2) + eps) [* weight]`` over the last dimension.
 
     Returns ``y``, or ``(y, h)`` with a residual: ``h`` is the stream that the next layer adds to.  ``x`` (..., C) fp32,
-    bf16 or fp16, C <= 32768; ``residual`` of the same shape and type; ``weight`` (C,) in the rows' type or fp32.  ``y`` is
-    computed from the fp32 sum; its gradient (of x, weight and residual) from the stored ``h``."""
+    bf16 or fp16, C <= 32768; ``residual`` of the same shape and type; ``weight`` (C,) in the rows' type or fp32.  ``y`` and its
+    gradient (of x, weight and residual) are those of the fp32 sum: the backward keeps ``x`` and ``residual``, not ``h``."""
     out = (_host or _native()).rms_norm(x, weight, eps, residual)
     return out if out is not None else _refuse_rms("rms_norm_rows", x, weight, residual, False)
 

@@ -725,7 +725,8 @@ int dgcn_rows_tn_colsum_f32(const float* g, int64_t ldg, const float* x, int64_t
  *     an infinity becomes NaN (0x7f) in its own place
  *   h (rows, C) dtype contiguous or NULL (y does not depend on h's rounding); rstd (rows) or NULL
  * Backward (rows >= 1): dx = rstd (w g - xh mean(w g xh)) [+ gh], xh = h rstd, contiguous, or NULL; dw (C) in the weight's
- *   type (fp32 with w_f32) or NULL, by way of dw_part [dgcn_rms_norm_num_partials(rows, C)][C].
+ *   type (fp32 with w_f32) or NULL, by way of dw_part [dgcn_rms_norm_num_partials(rows, C)][C].  dgcn_rms_norm_sum_bwd takes
+ *   h = x + res in fp32, as the forward's statistics do (res NULL: h = x); dgcn_rms_norm_bwd a stored h.
  * dgcn_quantize_rows_e4m3: q and scale of x itself.
  * dgcn_param_sum: out[c] = sum over p of parts[p][c], c < width, rounded to dtype; fixed order. */
 int dgcn_rms_norm_fwd(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, int32_t w_f32, float eps,
@@ -735,6 +736,9 @@ int32_t dgcn_rms_norm_num_partials(int64_t rows, int32_t C);
 int dgcn_rms_norm_bwd(const void* g, int64_t ldg, const void* gh, int64_t ldgh, const void* h, int64_t ldh, const void* w,
                       int32_t w_f32, const float* rstd, int32_t dtype, void* dx, void* dw, float* dw_part, int64_t rows,
                       int32_t C, void* stream);
+int dgcn_rms_norm_sum_bwd(const void* g, int64_t ldg, const void* gh, int64_t ldgh, const void* x, int64_t ldx, const void* res,
+                          int64_t ldr, const void* w, int32_t w_f32, const float* rstd, int32_t dtype, void* dx, void* dw,
+                          float* dw_part, int64_t rows, int32_t C, void* stream);
 int dgcn_quantize_rows_e4m3(const void* x, int64_t ldx, int32_t dtype, uint8_t* q, float* scale, int64_t rows, int32_t C,
                             void* stream);
 int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width, int32_t dtype, void* out, void* stream);

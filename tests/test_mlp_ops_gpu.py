@@ -643,3 +643,31 @@ def test_rows_e4m3_are_divided(dtype, rows, C):
     assert torch.equal(q.scale, scale.clamp_min(torch.finfo(torch.float32).tiny))
     want = (x.float() / q.scale.unsqueeze(-1)).to(torch.float8_e4m3fn)
     assert torch.equal(q.data.view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, C", [(1, 4096), (130, 513), (257, 33), (2000, 128), (17, 8191), (2, 32768)])
+def test_norm_gradients_see_the_sum(dtype, rows, C):
+    """The gradients with a residual are those of the fp32 sum x + r, not of h as it is stored: an fp32 weight's gradient
+    shows it, which has no rounding of its own.  Terms g xh with a sum of `rows` and one of C fp32 roundings."""
+    x, r = rand(rows, C, dtype=dtype, seed=1).requires_grad_(), rand(rows, C, dtype=dtype, seed=2).requires_grad_()
+    w = (1 + rand(C, dtype=torch.float32, seed=3, scale=0.3)).requires_grad_()
+    g, gh = rand(rows, C, dtype=dtype, seed=4), rand(rows, C, dtype=dtype, seed=5)
+    y, h = mlp_ops.rms_norm_rows(x, w, eps=1e-5, residual=r)
+    gx, gw, gr = torch.autograd.grad((y, h), (x, w, r), (g, gh))
+    h64, rstd, _ = norm_ref(x.detach(), w.detach(), r.detach(), 1e-5)
+    xh, g64, rel = h64 * rstd, g.double(), (C + 20) * U
+    gw64 = (g64 * xh).sum(0)
+    within(gw, gw64, (g64 * xh).abs().sum(0) * (rows + C + 20) * U + gw64.abs() * U + TINY[torch.float32], "gw")
+    gg = g64 * w.detach().double()
+    dot = (gg * xh).mean(-1, keepdim=True)
+    dx = rstd * (gg - xh * dot) + gh.double()
+    edx = rstd * (xh.abs() * (gg * xh).abs().mean(-1, keepdim=True) * rel + (xh * dot).abs() * rel + gg.abs() * rel)
+    edx = edx + rstd * (gg.abs() + (xh * dot).abs()) * 8 * U + gh.double().abs() * 2 * U
+    within(gx, dx, edx + dx.abs() * (half_step(dtype) * 1.01 + 2 * U) + TINY[dtype], "gx")
+    assert torch.equal(gx, gr)
+    one, wide = r.detach()[:1].expand(rows, C), torch.cat([x.detach(), x.detach()], 1)[:, :C]      # strides that the backward meets again
+    for a, b in ((wide, one), (one, wide)):
+        got, want = ([t.requires_grad_() for t in pair] for pair in ((a.detach(), b.detach()), (a.clone(), b.clone())))
+        both = [torch.autograd.grad(mlp_ops.rms_norm_rows(p, w, 1e-5, q)[0], (p, w, q), g) for p, q in (got, want)]
+        assert all(torch.equal(s, t) for s, t in zip(*both))
