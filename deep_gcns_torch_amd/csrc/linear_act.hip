@@ -4,8 +4,8 @@
 //   z = s_x s_w (x w^T) + b        y = act(z) + r              (s_x, s_w: the scales of e4m3 rows, else 1)
 //   dz = g act'(z)     gb = sum over rows of dz     gx = dz w     gw = dz^T x     gr = g
 //
-// Every sum is held in fp32.  For the backward the forward keeps z in fp32, or act'(z) in 16-bit fixed point where the rows
-// have 16 bits (mlp_common.h); dz is rounded to the rows' type before the two products, which take that on the matrix pipe.
+// Every sum is held in fp32.  For the backward the forward keeps z in fp32, or act'(z) as a 16-bit code where the rows have
+// 16 bits (mlp_common.h); dz is rounded to the rows' type before the two products, which take that on the matrix pipe.
 
 #include "linear_act.h"
 

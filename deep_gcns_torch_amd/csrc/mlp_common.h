@@ -201,19 +201,31 @@ __device__ __forceinline__ float act_slope(float z, int act, float slope) {
   return d;
 }
 
-// ---- what the backward of an activation in 16 bits keeps: act'(z) in fixed point, code = (act' + 1/4) 2^15 ----
-// gelu's and silu's slopes lie in (-0.13, 1.13); they come back within 2^-16, an eighth of a bf16 half step and less of
-// anything that is averaged.  (z in 16 bits would be off by half a step of z in act': measured, 1.5 times the error of the
-// bias gradient.)  relu and leakyrelu keep z > 0 as a slope of 1 or 0.  Code 0 is NaN (what the conversion makes of one).
+// ---- what the backward of an activation in 16 bits keeps: act'(z) as a 16-bit code ----
+// Codes up to kGateTail are fixed point, code = (act' + 1/4) 2^15: gelu's and silu's slopes lie in (-0.13, 1.13) and come back
+// within 2^-16, an eighth of a bf16 half step of slopes near 1.  (z in 16 bits would be off by half a step of z in act': measured,
+// 1.5 times the error of the bias gradient.)  Where a unit is saturated the slope is negative and small, and 2^-16 is too much of it
+// (3 % of gelu's at z = -4, all of it at -5): slopes from -2^-6 to -2^-45 take the codes that no fixed-point slope has, as
+// floating point with nine bits behind the leading one, within 2^-10 of themselves; what is smaller (gelu from z = -8.1, silu from
+// -34.7) is 0.  relu and leakyrelu keep z > 0 as a slope of 1 or 0.  Code 0 is NaN (what the conversion makes of one).
+constexpr uint32_t kGateTail = 45568;                      // 39 binades of 512 codes up to 65535; below it slopes up to 1.14
+constexpr uint32_t kGateLow = 0x20000 + (82 << 9);         // the top 18 bits of -2^-45
+
 __device__ __forceinline__ uint32_t gate_encode(float d) {
   uint32_t c;
   asm("v_cvt_u32_f32 %0, %1" : "=v"(c) : "v"(fmaf(d, 32768.f, 8192.5f)));
   return c;
 }
 
+__device__ __forceinline__ uint32_t gate_encode_tail(float d) {
+  const uint32_t u = ((__float_as_uint(d) + 0x2000u) >> 14) - kGateLow;
+  return u <= 0xffffu - kGateTail ? u + kGateTail : gate_encode(d);
+}
+
 __device__ __forceinline__ float gate_decode(uint32_t code, int act, float slope) {
   const float d = fmaf(static_cast<float>(code), 1.f / 32768.f, -0.25f);
   if (code == 0u) return __builtin_nanf("");
+  if (code >= kGateTail) return __uint_as_float((code - kGateTail + kGateLow) << 14);
   return act == DGCN_ACT_LEAKY_RELU && code == 8192u ? slope : d;
 }
 
@@ -237,7 +249,7 @@ template <int CNT>
 __device__ __forceinline__ void act_gate_run(float (&v)[CNT], uint32_t (&c)[CNT], int act, float slope) {
   float d;
   switch (act) {
-#define DGCN_ACT_CASE(A) case A: { _Pragma("unroll") for (int e = 0; e < CNT; ++e) { v[e] = act_both<false>(v[e], A, slope, d); c[e] = gate_encode(d); } break; }
+#define DGCN_ACT_CASE(A, ENCODE) case A: { _Pragma("unroll") for (int e = 0; e < CNT; ++e) { v[e] = act_both<false>(v[e], A, slope, d); c[e] = ENCODE(d); } break; }
     case DGCN_ACT_LEAKY_RELU: {
 #pragma unroll
       for (int e = 0; e < CNT; ++e) {
@@ -247,9 +259,9 @@ __device__ __forceinline__ void act_gate_run(float (&v)[CNT], uint32_t (&c)[CNT]
       }
       break;
     }
-    DGCN_ACT_CASE(DGCN_ACT_RELU)
-    DGCN_ACT_CASE(DGCN_ACT_GELU)
-    DGCN_ACT_CASE(DGCN_ACT_SILU)
+    DGCN_ACT_CASE(DGCN_ACT_RELU, gate_encode)
+    DGCN_ACT_CASE(DGCN_ACT_GELU, gate_encode_tail)
+    DGCN_ACT_CASE(DGCN_ACT_SILU, gate_encode_tail)
 #undef DGCN_ACT_CASE
     default: break;
   }

@@ -180,7 +180,8 @@ def linear_act(x, weight, bias=None, act: str = "none", residual=None, neg_slope
     ``x`` (..., K) and ``weight`` (N, K) in one of fp32, bf16, fp16; ``bias`` (N,) in that type or fp32; ``residual``
     (..., N) in that type; ``act`` one of :data:`ACTIVATIONS` (``neg_slope``: of leakyrelu, gelu: ``z Phi(z)``).  Gradients
     of all four; for them the forward keeps, where there is an activation, one value per result: the pre-activation of fp32
-    rows, the activation's slope in 16-bit fixed point of 16-bit ones."""
+    rows, the activation's slope as a 16-bit code of 16-bit
+    ones (within 2^-16, and within 2^-10 of itself where a unit is saturated, from -2^-6 to -2^-45; what is smaller is 0)."""
     code = _act_code("linear_act", act)
     y = (_host or _native()).linear_act(x, weight, bias, code, residual, neg_slope)
     if y is None:

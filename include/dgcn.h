@@ -749,8 +749,9 @@ int dgcn_param_sum(const float* parts, int32_t nparts, int64_t width, int32_t dt
  *   x (rows, K) row stride ldx, w (N, K) row stride ldw, both in in_type; K, N <= 2^20
  *   in_type DGCN_T_E4M3: x_scale (rows) and w_scale (N) are required and out_type is free; otherwise out_type = in_type
  *   bias (N) in out_type or, with bias_f32, fp32, or NULL; res (rows, N) out_type, row stride ldr, or NULL
- *   z (rows, N) contiguous, or NULL: kept for the backward -- z in fp32, or in the 16-bit types act'(z) in 16-bit fixed
- *     point (code 2^-15 - 1/4; 0 is NaN; relu and leakyrelu: z > 0 as 1 or 0); y (rows, N) out_type contiguous
+ *   z (rows, N) contiguous, or NULL: kept for the backward -- z in fp32, or in the 16-bit types act'(z) as a
+ *     16-bit code (below 45568 fixed point, code 2^-15 - 1/4, and 0 is NaN; from there -2^-45 to -2^-6 in steps of
+ *     2^-9 of a power of two; relu and leakyrelu: z > 0 as 1 or 0); y (rows, N) out_type contiguous
  * Backward, all in one dtype, rows >= 1:  dz = g act'(z);  dx (rows, K) = dz w, dw (N, K) = dz^T x, db (N) = sum of dz over the
  *   rows (dtype or, with db_f32, fp32), contiguous, each or NULL; z as above (NULL with DGCN_ACT_NONE)
  * Operands may start and repeat at any byte; those whose rows do not start on dwords, and in the backward those whose rows

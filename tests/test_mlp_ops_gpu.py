@@ -671,3 +671,20 @@ def test_norm_gradients_see_the_sum(dtype, rows, C):
         got, want = ([t.requires_grad_() for t in pair] for pair in ((a.detach(), b.detach()), (a.clone(), b.clone())))
         both = [torch.autograd.grad(mlp_ops.rms_norm_rows(p, w, 1e-5, q)[0], (p, w, q), g) for p, q in (got, want)]
         assert all(torch.equal(s, t) for s, t in zip(*both))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act, low, high", [("gelu", -7.0, -2.0), ("silu", -28.0, -3.0)])
+@pytest.mark.parametrize("rows", [9, 700])
+def test_gradients_of_saturated_units(dtype, act, low, high, rows):
+    """One product per result, so that z is x to the bit: dx = act'(z) g within, relative to it, the kept slope's half step of
+    2^-10, dz's and dx's roundings (the second of a value that has them already), and 2^-12 for the slope's own evaluation
+    (the distribution function's fit 1e-5, its difference from z times the density at most doubled from z = -2 on, the
+    exponential's argument z^2 / 2 2^-24)."""
+    x = torch.linspace(low, high, rows, device="cuda").to(dtype).view(rows, 1).requires_grad_()
+    w = torch.ones(1, 1, device="cuda", dtype=dtype)
+    g = torch.full((rows, 1), 1024.0, device="cuda", dtype=dtype)
+    gx, = torch.autograd.grad(mlp_ops.linear_act(x, w, act=act), x, g)
+    want = act_ref(x.detach().double(), act)[1] * 1024
+    within(gx, want, want.abs() * (half_step(dtype) + 2.0 ** -10 + 2.0 ** -12) + TINY[dtype], act)
+    assert (gx < 0)[want < -TINY[dtype]].all()                       # (what fp16 itself rounds to 0: 1024 slope under 2^-25)
