@@ -3,8 +3,9 @@
 // Bound by reading the weight once (2 rows flop a byte in 16 bits).  A workgroup owns 16 channels and all of K, its eight or
 // sixteen waves take the 128-byte steps of the reduction in turn, straight from memory into matrix fragments (no LDS: nothing of
 // the weight is used twice), UNROLL steps requested ahead; the waves' sums meet in LDS in wave order.  Rows may start at any
-// byte, so odd strides and lengths need no copy of the weight.  Measured: 4096 x 4096 bf16, one row 7.8 us (4.3 TB/s);
-// 16,384 x 4096 e4m3, 16 rows 14.7 us (4.6 TB/s).
+// byte, so odd strides and lengths need no copy of the weight.  Measured: 4096 x 4096 bf16, one row 7.8 us (4.3 TB/s),
+// the same over 24 weights in turn, which no cache holds; 16,384 x 4096 e4m3, 16 rows 14.4 us (4.7 TB/s), over 12 weights in
+// turn 17.6 (3.8 TB/s); 4096 x 4096 fp32, one row 17.2 us (3.9 TB/s), over 12 weights in turn 18.0.
 #pragma once
 
 #include "linear_tile.h"
@@ -48,16 +49,8 @@ template <> struct MatIn<float> {
   }
 };
 
-template <> struct MatIn<uint8_t> {
-  static constexpr int ES = 1;
-  typedef i8v Frag;
-  static __device__ __forceinline__ Frag prep(const u4v (&r)[2]) {
-    return __builtin_bit_cast(i8v, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
-  }
-  static __device__ __forceinline__ void one_tile(const Frag& b, const Frag& a, f32x4& c) {
-    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, 127, 0, 127);
-  }
-};
+// e4m3: exact products, summed in fp32 (the 8-bit instruction would cut them, see TileIn<uint8_t>; here the pipe has time:
+// 16,384 x 4096, 16 rows, 14.9 us with either)
 template <> struct MatIn<WideE4m3> {
   static constexpr int ES = 1;
   struct Frag { u4v r[4]; };
@@ -192,7 +185,8 @@ int small_go(const MatParams& P, bool shift, hipStream_t s) {
 
 // Sixteen waves where the channels give at most one workgroup a CU and each wave still has four steps (4096 x 4096 bf16: one
 // row 7.9 us against 9.4 with eight, 16 rows 10.0 against 10.3); 32 channels a workgroup for e4m3 where they give every CU one
-// (16,384 x 4096, 16 rows: 17.2 us against 20.3; one row 16.3 against 16.9; in 16 bits it is slower, 35.5 against 34.1).
+// (16,384 x 4096, 16 rows: 14.4 us against 17.8, one row 13.4 against 16.1; 8192 x 8192, which gives each just one: 19.9
+// against 16.9; in 16 bits it is slower, 35.5 against 34.1).
 template <class T, class O>
 int small_launch(const MatParams& P, hipStream_t s) {
   constexpr int ES = MatIn<T>::ES;

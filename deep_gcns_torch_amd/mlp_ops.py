@@ -197,9 +197,10 @@ def linear_act_e4m3(x: RowsE4M3, weight: RowsE4M3, bias=None, act: str = "none",
                     out_dtype=torch.bfloat16, neg_slope: float = 0.2):
     """``act((x.data * x.scale) @ (weight.data * weight.scale).T + bias) + residual``: ``x`` rows (..., K), ``weight`` rows
     (N, K) (``quantize_rows`` of an nn.Linear weight, once); the result, ``residual`` and ``bias`` (or an fp32 bias) in
-    ``out_dtype``; the scales join behind the sum.  For an fp32 result the products are summed in fp32; for a 16-bit one on
-    the 8-bit matrix pipe at twice the rate, which cuts products that lie more than 2^13 below the largest of eight
-    neighbouring ones (about 6e-5 of the result's root mean square over normal rows).  No gradient."""
+    ``out_dtype``; the scales join behind the sum.  For an fp32 result, and for up to 16 rows (but
+    where few channels meet a long K), the products are summed in fp32; for a 16-bit one of more rows on the 8-bit matrix
+    pipe at twice the rate, which cuts products that lie more than 2^13 below the largest of eight neighbouring ones (about
+    6e-5 of the result's root mean square over normal rows).  No gradient."""
     what = "linear_act_e4m3"
     if out_dtype not in _ROW_TYPES:
         raise TypeError(f"{what}: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")

@@ -688,3 +688,16 @@ def test_gradients_of_saturated_units(dtype, act, low, high, rows):
     want = act_ref(x.detach().double(), act)[1] * 1024
     within(gx, want, want.abs() * (half_step(dtype) + 2.0 ** -10 + 2.0 ** -12) + TINY[dtype], act)
     assert (gx < 0)[want < -TINY[dtype]].all()                       # (what fp16 itself rounds to 0: 1024 slope under 2^-25)
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("rows, N", [(1, 40), (4, 64), (16, 8200), (16, 4096)])
+def test_few_e4m3_rows_are_summed_in_fp32(out, rows, N):
+    """2^16 - 2^16 + 2^(16 - d): up to 16 rows nothing is cut from a product, whatever the result's type."""
+    for where, d in ((2, 13), (2, 14), (7, 18), (8, 20), (40, 26)):
+        x, w = torch.zeros(rows, 160, device="cuda"), torch.zeros(N, 160, device="cuda")
+        x[:, 0], w[:, 0], x[:, 1], w[:, 1] = 256.0, 256.0, 256.0, -256.0
+        x[:, where], w[:, where] = 2.0 ** ((17 - d) // 2), 2.0 ** (16 - d - (17 - d) // 2)
+        rows8 = [RowsE4M3(t.to(torch.float8_e4m3fn), torch.ones(t.size(0), device="cuda")) for t in (x, w)]
+        y = mlp_ops.linear_act_e4m3(*rows8, out_dtype=out)
+        assert torch.equal(y.float(), torch.full((rows, N), 2.0 ** (16 - d), device="cuda")), (where, d)
