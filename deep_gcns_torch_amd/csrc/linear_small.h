@@ -149,6 +149,22 @@ __global__ __launch_bounds__(WAVES * 64) void small_kernel(const MatParams P) {
     for (int t = 0; t < MT; ++t) { rx[t][0] = x_row(t).end(at + at0, bytes); rx[t][1] = x_row(t).end(at + at1, bytes); }
     add(rw, rx);
   }
+  if constexpr (std::is_same<T, float>::value) {           // see f32_kinds
+#pragma unroll
+    for (int t = 0; t < MT * NT; ++t) {
+      f32x4& c = acc[t / NT][t % NT];
+      if (!any_nan(c)) continue;
+      auto of = [&](const Row<SHIFT>& row, int64_t at) {
+        const f32x4 lo = __builtin_bit_cast(f32x4, row.end(at + at0, bytes)), hi = __builtin_bit_cast(f32x4, row.end(at + at1, bytes));
+        const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        return f32_kinds(v);
+      };
+      f32x4 kinds = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int64_t at = 128 * wave; at < bytes; at += 128 * WAVES) kinds = MatIn16<__bf16>::one(of(w_row(t % NT), at), of(x_row(t / NT), at), kinds);
+      take_kinds(c, kinds);
+    }
+  }
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
 #pragma unroll

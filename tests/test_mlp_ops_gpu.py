@@ -701,3 +701,40 @@ def test_few_e4m3_rows_are_summed_in_fp32(out, rows, N):
         rows8 = [RowsE4M3(t.to(torch.float8_e4m3fn), torch.ones(t.size(0), device="cuda")) for t in (x, w)]
         y = mlp_ops.linear_act_e4m3(*rows8, out_dtype=out)
         assert torch.equal(y.float(), torch.full((rows, N), 2.0 ** (16 - d), device="cuda")), (where, d)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, K, N", [(1, 1, 1), (3, 64, 40), (16, 1030, 70), (70, 96, 40), (300, 130, 264), (130, 6152, 136), (40, 33, 4100)])
+def test_infinite_operands_of_products(dtype, rows, K, N):
+    """Infinities, NaN and zeros against them give what the products of the definition give, in the forward and in both
+    products of the backward; everything else keeps its bounds."""
+    x, w, g = (rand(*s, dtype=dtype, seed=k, scale=c) for k, (s, c) in enumerate((((rows, K), 1.0), ((N, K), K ** -0.5), ((rows, N), 1.0))))
+    inf, nan = float("inf"), float("nan")
+    x[0, K // 2] = inf
+    w[N // 2, K // 2] = 0.0                                          # against the infinity: NaN
+    if rows > 2:
+        x[rows - 1, K - 1], x[1, 0] = -inf, nan
+        w[N - 1, 0] = -inf
+        g[rows // 2, N // 3] = inf
+        x[rows // 2, K // 3] = 0.0
+
+    def like(got, want, bound, what):
+        got, finite = got.double(), torch.isfinite(want)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+        assert torch.equal(got.isposinf(), want.isposinf()) and torch.equal(got.isneginf(), want.isneginf()), what
+        assert ((got - want).abs()[finite] <= bound[finite]).all(), what
+
+    def product(a, b):                                               # (..., k) x (n, k), and the sum of its finite terms' magnitudes
+        a, b = a.double().cpu(), b.double().cpu()
+        return (a @ b.t()).cuda(), (a.abs().nan_to_num(0, 0, 0) @ b.abs().nan_to_num(0, 0, 0).t()).cuda()
+
+    def bounds(z, mag, k):
+        return mag * (6 * k + 12) * U + z.abs() * half_step(dtype) * 1.01 + TINY[dtype]
+    z, mag = product(x, w)
+    like(mlp_ops.linear_act(x, w), z, bounds(z, mag, K), "z")
+    y = torch.where(z < 0, torch.zeros_like(z), z)                   # relu keeps NaN, and takes -inf to 0
+    like(mlp_ops.linear_act(x, w, act="relu"), y, bounds(z.nan_to_num(0, 0, 0), mag, K), "relu")
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    dx, dw = torch.autograd.grad(mlp_ops.linear_act(a, b), (a, b), g)
+    for got, (want, mag), k, what in ((dx, product(g, w.t()), N, "dx"), (dw, product(g.t(), x.t()), rows, "dw")):
+        like(got, want, bounds(want, mag, k), what)
