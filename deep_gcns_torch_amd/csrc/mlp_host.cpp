@@ -48,10 +48,16 @@ void check(int rc, const char* what) {
   TORCH_CHECK(rc == 0, what, " failed (rc=", rc, "): ", lib.strerror(rc));
 }
 
+// A tensor that carries a tangent (torch.autograd.forward_ad), whatever the gradient mode: no operator here has a derivative
+// for it, and a result without one would read as a derivative of zero.
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool dual(const OptTensor& t) { return t.has_value() && dual(*t); }
+
 // The gradients of a backward pass that has none of its own: under create_graph they are made outside the graph, and
 // differentiating them again raises.
 template <class Run>
-variable_list once_differentiable(const char* what, Run run) {
+variable_list once_differentiable(const char* what, const variable_list& upstream, Run run) {
+  for (const Tensor& g : upstream) TORCH_CHECK(!dual(g), what, " has no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return run();
   variable_list grads;
   {
@@ -162,7 +168,7 @@ struct RmsFn : torch::autograd::Function<RmsFn> {
     return {o.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    return once_differentiable("rms_norm_rows", [&] { return run(ctx, grads); });
+    return once_differentiable("rms_norm_rows", grads, [&] { return run(ctx, grads); });
   }
   static variable_list run(AutogradContext* ctx, const variable_list& grads) {
     const bool has_w = ctx->saved_data["weight"].toBool(), has_r = ctx->saved_data["residual"].toBool();
@@ -204,6 +210,7 @@ py::object rms_norm(const Tensor& x, const OptTensor& weight, double eps, const 
   if (row_type(type) < 0 || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > kMaxNormC || !x.is_cuda()) return py::none();
   const auto d = x.get_device();
   if (!param_ok(weight, x.size(-1), type) || !same_rows(residual, x, x.size(-1), type) || !on(weight, d) || !on(residual, d)) return py::none();
+  if (dual(x) || dual(weight) || dual(residual)) return py::none();
   if (at::GradMode::is_enabled() && (x.requires_grad() || wants(weight) || wants(residual))) {
     if constexpr (e4m3) return py::none();
     variable_list o;
@@ -220,7 +227,7 @@ py::object rms_norm(const Tensor& x, const OptTensor& weight, double eps, const 
 
 py::object quantize_rows(const Tensor& x) {
   if (row_type(x.scalar_type()) < 0 || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > kMaxNormC || !x.is_cuda()) return py::none();
-  if (at::GradMode::is_enabled() && x.requires_grad()) return py::none();
+  if (dual(x) || (at::GradMode::is_enabled() && x.requires_grad())) return py::none();
   const Rows in(x);
   Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
   Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
@@ -270,7 +277,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     return {y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    return once_differentiable("linear_act", [&] { return run(ctx, grads); });
+    return once_differentiable("linear_act", grads, [&] { return run(ctx, grads); });
   }
   static variable_list run(AutogradContext* ctx, const variable_list& grads) {
     const int64_t act = ctx->saved_data["act"].toInt(), bias_type = ctx->saved_data["bias"].toInt();
@@ -315,7 +322,7 @@ bool linear_ok(const Tensor& x, const Tensor& weight, const OptTensor& bias, con
   const int64_t N = weight.size(0), K = weight.size(1);
   const auto d = x.get_device();
   return K == x.size(-1) && N >= 1 && K >= 1 && N <= kMaxK && K <= kMaxK && on(weight, d) && on(bias, d) && on(residual, d) &&
-         param_ok(bias, N, out) && same_rows(residual, x, N, out);
+         param_ok(bias, N, out) && same_rows(residual, x, N, out) && !dual(x) && !dual(weight) && !dual(bias) && !dual(residual);
 }
 
 py::object linear_act(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t act, const OptTensor& residual, double slope) {
@@ -336,7 +343,8 @@ py::object linear_act_e4m3(const Tensor& x, const Tensor& sx, const Tensor& weig
                            const OptTensor& residual, at::ScalarType out, double slope) {
   if (row_type(out) < 0 || x.scalar_type() != at::kFloat8_e4m3fn || weight.scalar_type() != at::kFloat8_e4m3fn || sx.scalar_type() != at::kFloat ||
       sw.scalar_type() != at::kFloat || x.dim() < 1 || weight.dim() != 2 || sx.sizes() != x.sizes().slice(0, x.dim() - 1) ||
-      sw.sizes() != weight.sizes().slice(0, 1) || !linear_ok(x, weight, bias, residual, out) || !on(sx, x.get_device()) || !on(sw, x.get_device()))
+      sw.sizes() != weight.sizes().slice(0, 1) || !linear_ok(x, weight, bias, residual, out) || !on(sx, x.get_device()) || !on(sw, x.get_device()) ||
+      dual(sx) || dual(sw))
     return py::none();
   if (at::GradMode::is_enabled() && (sx.requires_grad() || sw.requires_grad() || wants(bias) || wants(residual))) return py::none();
   return py::cast(linear_run(x, weight, sx.contiguous(), sw.contiguous(), bias, residual, act, slope, DGCN_T_E4M3, out, false).first);

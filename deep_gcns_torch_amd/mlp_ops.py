@@ -12,7 +12,7 @@ whose rows are wider than 256 channels, or kept in bf16, fp16 or 8 bits:
 
 Rows are the last dimension; leading dimensions are free and may be empty.  Sums and statistics are fp32, every result is
 rounded once to its type.  Work runs on the current stream of the inputs' device; results do not depend on timing (no
-atomics).  What an operator does not take raises, nothing falls back.
+atomics).  What an operator does not take raises, nothing falls back; so do forward-mode and second derivatives.
 """
 from __future__ import annotations
 
@@ -21,6 +21,7 @@ from typing import NamedTuple
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -95,6 +96,8 @@ def _refuse_residual(r, x: torch.Tensor, n: int, dtype) -> None:
 def _refuse_rest(what: str, tensors, no_grad=False):
     """The checks common to all, and the end of a refusal: always raises."""
     _lib.require_device(*tensors)                # raises: a CPU tensor, or two devices
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
     if no_grad and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or on tensors that require none")
     raise RuntimeError(f"{what} does not take these arguments")

@@ -738,3 +738,33 @@ def test_infinite_operands_of_products(dtype, rows, K, N):
     dx, dw = torch.autograd.grad(mlp_ops.linear_act(a, b), (a, b), g)
     for got, (want, mag), k, what in ((dx, product(g, w.t()), N, "dx"), (dw, product(g.t(), x.t()), rows, "dw")):
         like(got, want, bounds(want, mag, k), what)
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_raises(grad_mode):
+    """A tangent is never dropped: neither operator has a forward-mode derivative, and each says so."""
+    import torch.autograd.forward_ad as fw
+    x, w = rand(40, 64, dtype=torch.float32, seed=1), rand(64, 64, dtype=torch.float32, seed=2)
+    b, q = rand(64, dtype=torch.float32, seed=3), mlp_ops.quantize_rows(rand(40, 64, dtype=torch.float32, seed=4))
+    with torch.set_grad_enabled(grad_mode), fw.dual_level():
+        d, dw, db = fw.make_dual(x, x), fw.make_dual(w, w), fw.make_dual(b, b)
+        ds = RowsE4M3(q.data, fw.make_dual(q.scale, q.scale))
+        q40 = RowsE4M3(q.data, q.scale)
+        for call in (lambda: mlp_ops.linear_act(d, w), lambda: mlp_ops.linear_act(x, dw), lambda: mlp_ops.linear_act(x, w, db),
+                     lambda: mlp_ops.linear_act(x, w, residual=d), lambda: mlp_ops.rms_norm_rows(d), lambda: mlp_ops.rms_norm_rows(x, db),
+                     lambda: mlp_ops.rms_norm_rows(x, b, residual=d), lambda: mlp_ops.rms_norm_rows_e4m3(d, b),
+                     lambda: mlp_ops.quantize_rows(d), lambda: mlp_ops.linear_act_e4m3(ds, q40, out_dtype=torch.float32),
+                     lambda: mlp_ops.linear_act_e4m3(q40, ds, out_dtype=torch.float32)):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+    with fw.dual_level():                                            # a tangent of the gradient that a backward is given
+        for out, leaf in (((lambda t: mlp_ops.linear_act(t, w)), x), (mlp_ops.rms_norm_rows, x)):
+            leaf = leaf.clone().requires_grad_()
+            y = out(leaf)
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                torch.autograd.grad(y, leaf, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+    for op in (lambda t: mlp_ops.linear_act(t, w), mlp_ops.rms_norm_rows, lambda t: mlp_ops.quantize_rows(t).scale):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(op, (x,), (x,))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(op)(x)
