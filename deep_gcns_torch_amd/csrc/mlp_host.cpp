@@ -346,7 +346,9 @@ py::object linear_act_e4m3(const Tensor& x, const Tensor& sx, const Tensor& weig
       sw.sizes() != weight.sizes().slice(0, 1) || !linear_ok(x, weight, bias, residual, out) || !on(sx, x.get_device()) || !on(sw, x.get_device()) ||
       dual(sx) || dual(sw))
     return py::none();
-  if (at::GradMode::is_enabled() && (sx.requires_grad() || sw.requires_grad() || wants(bias) || wants(residual))) return py::none();
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || sx.requires_grad() || weight.requires_grad() || sw.requires_grad() || wants(bias) || wants(residual)))
+    return py::none();
   return py::cast(linear_run(x, weight, sx.contiguous(), sw.contiguous(), bias, residual, act, slope, DGCN_T_E4M3, out, false).first);
 }
 

@@ -768,3 +768,15 @@ def test_forward_mode_raises(grad_mode):
             torch.func.jvp(op, (x,), (x,))
         with pytest.raises(RuntimeError):
             torch.func.vmap(op)(x)
+
+
+def test_e4m3_values_that_want_a_gradient_raise():
+    x = rand(20, 64, dtype=torch.float32, seed=1)
+    one = torch.ones(20, device="cuda")
+    plain, wants = RowsE4M3(x.to(torch.float8_e4m3fn), one), RowsE4M3(x.clone().requires_grad_().to(torch.float8_e4m3fn), one)
+    assert wants.data.requires_grad
+    for args in ((wants, plain), (plain, wants)):
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            mlp_ops.linear_act_e4m3(*args)
+        with torch.no_grad():
+            assert torch.equal(mlp_ops.linear_act_e4m3(*args), mlp_ops.linear_act_e4m3(plain, plain))
