@@ -158,6 +158,19 @@ class ResMLPE4M3(torch.nn.Module):
             self.register_buffer(f"scale{i}", w.scale)
             self.register_buffer(f"bias{i}", None if lin.bias is None else lin.bias.detach().clone())
 
+    def _apply(self, fn, *args, **kwargs):
+        """Moves everything; ``.to(dtype)``, ``.half()`` and their like, to which 8 bits are a floating-point type as any,
+        leave the weights and their scales as they are."""
+        rows = {k: self._buffers[k] for k in ("weight1", "scale1", "weight2", "scale2")}
+        moved = {k: fn(t) for k, t in rows.items()}
+        self._buffers.update(dict.fromkeys(rows))
+        try:
+            super()._apply(fn, *args, **kwargs)
+        finally:
+            self._buffers.update(rows)
+        self._buffers.update({k: t if t.dtype == rows[k].dtype else rows[k].to(t.device) for k, t in moved.items()})
+        return self
+
     @torch.no_grad()
     def forward(self, x, residual=None):
         out = mlp_ops.rms_norm_rows_e4m3(x, self.norm_weight, self.eps, residual)

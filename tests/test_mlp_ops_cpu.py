@@ -103,3 +103,25 @@ def test_missing_host_extension_raises(monkeypatch):
     monkeypatch.setitem(sys.modules, "deep_gcns_torch_amd._mlp_host", None)
     with pytest.raises(RuntimeError, match="python -m deep_gcns_torch_amd.build"):
         mlp_ops.quantize_rows(torch.zeros(2, 8))
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.float(), lambda m: torch.nn.Sequential(m).bfloat16()[0],
+                                  lambda m: m.to("cpu", torch.float16), lambda m: m.to("meta")])
+def test_casts_leave_e4m3_weights(cast, monkeypatch):
+    """A module's cast converts its parameters in 16 and 32 bits, and neither the 8-bit weights nor their scales."""
+    def plain(x):
+        scale = x.abs().amax(-1) / 448
+        return RowsE4M3((x / scale.unsqueeze(-1)).to(torch.float8_e4m3fn), scale)
+    monkeypatch.setattr(mlp_ops, "quantize_rows", plain)
+    m = blocks.ResMLP(24, 40).e4m3()
+    before, names = {k: v.clone() for k, v in m.state_dict().items()}, list(m.state_dict())
+    got = cast(m)
+    assert list(got.state_dict()) == names
+    for k in ("weight1", "scale1", "weight2", "scale2"):
+        t = got.state_dict()[k]
+        assert t.dtype == before[k].dtype and t.shape == before[k].shape
+        if t.device.type == "cpu":
+            view = torch.uint8 if "weight" in k else torch.int32
+            assert torch.equal(t.view(view), before[k].view(view))
+    assert len({got.state_dict()[k].device for k in names}) == 1
+    assert len({got.state_dict()[k].dtype for k in ("norm_weight", "bias1", "bias2")}) == 1
