@@ -780,3 +780,35 @@ def test_e4m3_values_that_want_a_gradient_raise():
             mlp_ops.linear_act_e4m3(*args)
         with torch.no_grad():
             assert torch.equal(mlp_ops.linear_act_e4m3(*args), mlp_ops.linear_act_e4m3(plain, plain))
+
+
+def test_work_is_on_the_current_stream():
+    """Inputs that the side stream writes behind a long product: work on any other stream would read what was there before."""
+    dtype = torch.bfloat16
+    first, second = rand(300, 256, dtype=dtype, seed=1), rand(300, 256, dtype=dtype, seed=2)
+    w, n = rand(512, 256, dtype=dtype, seed=3, scale=0.06), rand(256, dtype=dtype, seed=4)
+    w8 = mlp_ops.quantize_rows(w)
+
+    def step(x):
+        leaf, wl = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = mlp_ops.linear_act(mlp_ops.rms_norm_rows(leaf, n), wl, act="gelu")
+        grads = torch.autograd.grad(y, (leaf, wl), torch.ones_like(y))
+        with torch.no_grad():
+            q = mlp_ops.quantize_rows(x)
+            return [y.detach(), *grads, q.data.view(torch.uint8), q.scale, mlp_ops.linear_act_e4m3(q, w8),
+                    mlp_ops.rms_norm_rows_e4m3(x, n)[0].view(torch.uint8)]
+    want, old = step(second), step(first)
+    x, big = first.clone(), torch.randn(8192, 8192, device="cuda")
+    out = torch.empty_like(big)
+    torch.mm(big, big, out=out)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(4):
+            torch.mm(big, big, out=out)
+        x.copy_(second)
+        got = step(x)
+        assert not side.query()                                      # all of it was queued while the product ran
+    side.synchronize()
+    for a, b, c in zip(got, want, old):
+        assert torch.equal(a, b) and not torch.equal(a, c)
