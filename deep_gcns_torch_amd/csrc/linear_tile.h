@@ -196,9 +196,9 @@ __device__ __forceinline__ i4v tile_buffer(const char* p, int bytes) {
 // 16 bytes a lane from a buffer to LDS, `to` + 16 lane.  Written out because the compiler, which cannot tell which LDS bytes a
 // transposing read takes, waits for every copy before each of them (measured on dw of 16384 x 4096 x 8192: 1.14 ms against 0.9);
 // the kernel counts its copies itself (meet).  Nothing is returned in registers; the waits that the instruction needs behind
-// writes of m0 (which nothing else here uses) and of its scalar operands are in the text.
+// writes of m0 and of its scalar operands are in the text.
 __device__ __forceinline__ void copy16(i4v buffer, unsigned off, unsigned to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(buffer), "s"(uni(static_cast<int>(to))) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(buffer), "s"(uni(static_cast<int>(to))) : "memory", "m0");
 }
 
 template <int N>

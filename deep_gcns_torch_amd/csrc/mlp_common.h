@@ -132,11 +132,6 @@ __device__ __forceinline__ void load_param_chunk(const void* p, bool f32, int st
   }
 }
 
-template <class T>
-__device__ __forceinline__ float load_param(const void* p, bool f32, int64_t i) {
-  return f32 ? static_cast<const float*>(p)[i] : static_cast<float>(static_cast<const T*>(p)[i]);
-}
-
 // four fp32 values -> four e4m3 bytes, to nearest even (|v| <= 448 up to rounding; anything not finite -> NaN, 0x7f)
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
