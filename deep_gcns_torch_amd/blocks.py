@@ -121,7 +121,7 @@ class ResPlusLayer(torch.nn.Module):
 
 
 class ResMLP(torch.nn.Module):
-    """``h + W2 act(W1 rmsnorm(h) + b1) + b2`` over node rows in three launches: the norm (which also adds ``residual``, the
+    """``h + W2 act(W1 rmsnorm(h) + b1) + b2`` over node rows in three operators: the norm (which also adds ``residual``, the
     rows an aggregation leaves: ``h = x + residual``), the product with bias and activation, the product with bias and
     ``h``.  fp32, bf16 or fp16; ``act`` one of ``mlp_ops.ACTIVATIONS``.  ``e4m3()``: the same block in 8 bits, for serving."""
 
@@ -146,7 +146,8 @@ class ResMLP(torch.nn.Module):
 
 class ResMLPE4M3(torch.nn.Module):
     """A :class:`ResMLP` whose two products run in 8 bits: the weights' rows are laid out once, the norm's output and the
-    activations are rounded row by row on the way.  The stream ``h`` keeps its type.  No gradient."""
+    activations are rounded row by row on the way.  The stream ``h`` keeps its type.  No gradient.  Casts of the module leave
+    the 8-bit weights and their scales."""
 
     def __init__(self, mlp: ResMLP):
         super().__init__()

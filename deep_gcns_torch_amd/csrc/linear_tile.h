@@ -6,12 +6,14 @@
 // The fragments of a half lie in registers already while the next half's are read from LDS, and the stage after next is
 // requested as soon as every wave has read the second half of this one: the matrix instructions wait for neither, and a
 // stage costs one barrier.  (Four to six stages under way, for grids of one workgroup a CU, change nothing: 1024 x 1024 x 2048
-// fp16 12.0 us with two, 12.1 with three, 12.9 with six.  Nor do four waves of 128 x 128 with a third fewer LDS reads: 8192^3 e4m3
-// 463 us against 416, 8192 x 4096 x 16,384 bf16 944 against 878: one wave a SIMD leaves the pipe idle at each barrier.)
+// fp16 12.0 us with two, 12.1 with three, 12.9 with six.  Nor do four waves of 128 x 128 with a third fewer LDS reads, products
+// without bias, activation and residual: 8192^3 e4m3 463 us against 416, 8192 x 4096 x 16,384 bf16 944 against 878: one wave a
+// SIMD leaves the pipe idle at each barrier.)
 //
-// Measured: 8192 x 4096 x 16,384 bf16 1.01 ms forward with gelu (1.09 PFLOP/s; the library's bare product 0.88), 0.88 dx and
-// 0.91 dw (1.25, 1.21); 8192^3 e4m3 0.49 ms (2.26 PFLOP/s; the library 0.36); 169,343 x 128 x 256 fp32 0.150 ms forward (2.9
-// TB/s with z), 0.090 dx, 0.073 dw.
+// Measured, best of a case's launches on normal operands: 8192 x 4096 x 16,384 bf16 0.91 ms bare (1.21 PFLOP/s; the library's
+// product 0.71), 0.95 with bias and gelu, 1.00 where the slopes are kept too, 0.88 dx and 0.93 dw (1.25, 1.18; the library's 0.80 and
+// 0.92); 8192^3 e4m3 0.42 ms bare (2.6 PFLOP/s; the library 0.36), 0.48 with bias and residual, 0.78 for an fp32 result;
+// 8192 x 2048 x 2048 fp32 0.31 ms; 169,343 x 128 x 256 fp32 0.150 ms forward (2.9 TB/s with z), 0.090 dx, 0.073 dw.
 #pragma once
 
 #include <type_traits>

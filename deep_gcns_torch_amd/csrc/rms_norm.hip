@@ -9,13 +9,13 @@
 // waves or a part of a wave a row), the sum of squares is joined by shuffles (and LDS between waves), and everything
 // that depends on the row is written from the same registers.  The statistics use the fp32 sum x + r, of which h is the
 // rounding to the rows' type; the backward adds x and r again (the stored h instead is one row less to read and to keep,
-// 16,384 x 4096 bf16 114 us against 141, but half a step of it is off in every term of the weight's gradient: bf16 2.3e-3 of its
+// 16,384 x 4096 bf16 114 us against 145, but half a step of it is off in every term of the weight's gradient: bf16 2.3e-3 of its
 // norm against 1.7e-3 that its own rounding costs).  The weight's gradient stays in registers over all rows of a workgroup and leaves as one
 // partial per workgroup, summed in a fixed order by a second launch: no atomics, the same bits every time.
 //
 // Measured (a copy of 1 GiB reaches 5.1 TB/s; what fits the 256 MB of memory-side cache goes faster): 16,384 x 4096 bf16 with
-// residual 86 us forward (6.2 TB/s over x, r, h, y) and 114 us backward (4.7 over g, g_h, h, gx); 169,343 x 128 fp32 28 and
-// 48 us (6.2 and 5.5); to e4m3 rows 8192 x 8192 bf16 with residual 114 us (4.1), the rounding alone of 8192 x 16,384 91 us (4.4).
+// residual 84 us forward (6.4 TB/s over x, r, h, y) and 145 us backward (4.6 over g, g_h, x, r, gx); 169,343 x 128 fp32 28 and
+// 48 us (6.2 and 5.5); to e4m3 rows 8192 x 8192 bf16 with residual 116 us (4.0), the rounding alone of 8192 x 16,384 95 us (4.2).
 
 #include "mlp_common.h"
 
@@ -357,7 +357,8 @@ int rms_fwd(const RmsParams& P, hipStream_t s) {
   if (chunks <= 256) return RmsFwd<T, 256, 1>::template go<NORM, Q8>(P, s);
   if (chunks <= 512) return RmsFwd<T, 512, 1>::template go<NORM, Q8>(P, s);
   // one barrier a row: more waves with less each (8192 x 8192 bf16 98 us against 111); two: the other way (112 against 129);
-  // none of a norm, from 8193 channels on: half the waves (8192 x 16,384 90 us against 102)
+  // none of a norm, from 8193 channels on: half the waves (8192 x 16,384 94 us; 90 against 102 before values were divided to the
+  // last bit)
   if (chunks <= 1024) return Q8 ? RmsFwd<T, 512, 2>::template go<NORM, Q8>(P, s) : RmsFwd<T, 1024, 1>::template go<NORM, Q8>(P, s);
   if (chunks <= 2048) return NORM ? RmsFwd<T, 1024, 2>::template go<NORM, Q8>(P, s) : RmsFwd<T, 512, 4>::template go<NORM, Q8>(P, s);
   return RmsFwd<T, 1024, 4>::template go<NORM, Q8>(P, s);
