@@ -407,6 +407,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(const MatParams P
       f32x16& c = acc[t >> 1][t & 1];
       if (!any_nan(c)) continue;
       const int64_t m = m0 + (wm * TM + (t >> 1)) * 32 + i, n = n0 + wn * 64 + 32 * (t & 1) + i;
+      bool stored = false;                                              // (what lies behind the matrix may be NaN and does not count)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) stored = stored || (c[e] != c[e] && m < P.M && n - i + 8 * (e >> 2) + 4 * h + (e & 3) < P.N);
+      if (!__any(stored)) continue;
       f32x16 kinds = {};
 #pragma unroll 1
       for (int64_t k = k0 + 8 * h; k - 8 * h < k1; k += 16) {
