@@ -125,3 +125,20 @@ def test_casts_leave_e4m3_weights(cast, monkeypatch):
             assert torch.equal(t.view(view), before[k].view(view))
     assert len({got.state_dict()[k].device for k in names}) == 1
     assert len({got.state_dict()[k].dtype for k in ("norm_weight", "bias1", "bias2")}) == 1
+
+
+def test_norm_of_a_sum_backward_argument_errors_do_not_launch():
+    lib = _lib.load()
+    buf = (C.c_float * 64)()
+    p = (C.addressof(buf) + 15) & ~15
+    bwd = lib.dgcn_rms_norm_sum_bwd
+    ok = dict(g=p, ldg=8, gh=None, ldgh=0, x=p, ldx=8, res=p, ldr=8, w=None, w_f32=0, rstd=p, dtype=0, dx=p, dw=None, parts=None,
+              rows=1, C=8, stream=None)
+
+    def rc(**change):
+        return bwd(*{**ok, **change}.values())
+    for change in (dict(g=None), dict(x=None), dict(rstd=None), dict(dx=None), dict(dw=p)):
+        assert rc(**change) == -1, change                                     # (dw without its partials)
+    for change in (dict(rows=0), dict(C=0), dict(C=32769), dict(ldx=-1), dict(ldr=-1), dict(ldg=-1), dict(gh=p, ldgh=-1)):
+        assert rc(**change) == -2, change
+    assert rc(dtype=3) == -4

@@ -812,3 +812,24 @@ def test_work_is_on_the_current_stream():
     side.synchronize()
     for a, b, c in zip(got, want, old):
         assert torch.equal(a, b) and not torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_backward_entry_of_a_stored_sum(dtype):
+    """dgcn_rms_norm_bwd takes h itself: without a residual the same bits as the operator's backward."""
+    from deep_gcns_torch_amd import _lib
+    lib, rows, C = _lib.load(), 70, 513
+    h, g = rand(rows, C, dtype=dtype, seed=1), rand(rows, C, dtype=dtype, seed=2)
+    w = (1 + rand(C, dtype=torch.float32, seed=3, scale=0.3)).requires_grad_()
+    leaf = h.clone().requires_grad_()
+    want = torch.autograd.grad(mlp_ops.rms_norm_rows(leaf, w), (leaf, w), g)
+    code, y, rstd = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype], torch.empty_like(h), torch.empty(rows, device="cuda")
+    dx, dw = torch.empty_like(h), torch.empty(C, device="cuda")
+    parts = torch.empty(lib.dgcn_rms_norm_num_partials(rows, C), C, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.dgcn_rms_norm_fwd(h.data_ptr(), C, None, 0, w.data_ptr(), 1, 1e-6, code, y.data_ptr(), None, None, None, rstd.data_ptr(),
+                                 rows, C, stream) == 0
+    assert lib.dgcn_rms_norm_bwd(g.data_ptr(), C, None, 0, h.data_ptr(), C, w.data_ptr(), 1, rstd.data_ptr(), code, dx.data_ptr(),
+                                 dw.data_ptr(), parts.data_ptr(), rows, C, stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
